@@ -231,6 +231,97 @@ tb_status tb_linear(tb_ctx* ctx, int64_t m, int k, int n, const void* a, const v
 tb_status tb_layer_norm(tb_ctx* ctx, const void* x, tb_dtype x_dtype, int64_t n, int c, const float* w,
                         const float* b, float eps, tb_epilogue act, tb_dtype out_dtype, void* out);
 
+/* ---- transformer operators over packed sets ------------------------------------------------
+ * No reference counterpart in include/sparse.h: the layers of a transformer over the same packed
+ * voxel (or token) rows, next to tb_linear and tb_layer_norm. Packed: the rows of one array hold
+ * one set (object, sequence) after another, set s in rows offsets[s] .. offsets[s+1]-1 of a device
+ * int32 table [nset+1]; a set may be empty. Rows before the first and behind the last set are
+ * neither read nor written. A null table with nset 1 is one set of all rows. At most 65536 sets. The
+ * tables are read on the device when the call runs, so a captured call follows their contents; a
+ * table that descends or leaves the array is clamped and reported by tb_ctx_check_device
+ * (TB_ERR_DEVICE). Workspace is the caller's (two captured graphs share one only if the caller
+ * gives both the same), 16-byte aligned, of at least the bytes that the matching query names for
+ * the same arguments, and free for reuse once the call has run.
+ *
+ * tb_attention: for query row i and head h of a set, with the keys and values of head
+ * h / (heads / kv_heads):
+ *   out[i][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q_i . k_j)
+ * over the set's keys j; causal keeps j <= i + keys - queries (i, j from the sets' first rows), so
+ * the last query sees every key, and one query row is a new token against all keys. lse (float32
+ * [nq][heads], may be NULL) = log sum_j p_j. A row that sees no key gives 0, and -inf in lse.
+ *   - q [nq][heads][head_dim], k, v [nk][kv_heads][head_dim], out as q: rows and heads are the given
+ *     numbers of elements apart, multiples of 16 bytes, values of a head contiguous. head_dim a
+ *     multiple of 8 up to 128, at most 64 heads a key head, scale > 0.
+ *   - q_offsets and k_offsets are given together; their set s belong to each other.
+ *   - dtype TB_BF16 / TB_F16: tcgen05 tensor cores, fp32 scores, softmax and accumulation; the
+ *     p_j are rounded to the operand type before their product with v. TB_F32: CUDA cores.
+ *   - out_dtype: TB_F32 or the operand dtype. out must not overlap q, k or v.
+ *   - Values behind a set's last key have no effect, not a number included. A key that causal
+ *     hides from some rows of its set must be finite: the rows' products multiply it by 0.
+ *
+ * tb_rope: rotary positions along 1 to 4 axes. Pair p of each head of row i turns by
+ * pos[i][axis(p)] * f_p: (a, b) -> (a cos - b sin, a sin + b cos). The first sections[0] pairs of a
+ * head take axis 0, the next sections[1] axis 1, ...; pairs behind the last section are copied.
+ *   - coords int32 [n][coord_stride]: the last `axes` columns are the positions (voxel rows (x,y,z)
+ *     or (b,x,y,z)); any value, negative included.
+ *   - layout: TB_ROPE_PAIRS turns elements 2p, 2p+1; TB_ROPE_HALVES elements p, p + head_dim/2.
+ *   - freqs: TB_ROPE_FREQS_AXIS f_p = theta^(-j/sections[axis]) with j the pair's place in its section;
+ *     TB_ROPE_FREQS_JOINT f_p = theta^(-p/(head_dim/2)).
+ *   - inverse != 0 turns by the negative angles (the transpose: carries gradients back).
+ *   - x, out [n][heads][head_dim] of dtype, strides as in tb_attention; out may be x with the same
+ *     strides. The first heads of wider rows (q and k of one q|k|v product) are one call. head_dim a
+ *     multiple of 8 up to 256. Angles are reduced in 64 bits.
+ *
+ * tb_group_norm: out = act((x - mean) / sqrt(var + eps) * w + b), mean and variance of each set over
+ * its rows and each group's c / groups consecutive channels. x [n][c] of x_dtype, out [n][c] of
+ * out_dtype (TB_F32 or x_dtype; may be x); c a multiple of 8 up to 2048; w, b float32 [c], each may be
+ * NULL. Statistics in fp32 pieces joined in 64 bits in a fixed order. */
+typedef enum tb_rope_layout { TB_ROPE_PAIRS = 0, TB_ROPE_HALVES = 1 } tb_rope_layout;
+typedef enum tb_rope_freqs { TB_ROPE_FREQS_AXIS = 0, TB_ROPE_FREQS_JOINT = 1 } tb_rope_freqs;
+
+typedef struct tb_attention_params {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    float* lse;
+    const int32_t* q_offsets;
+    const int32_t* k_offsets;
+    int64_t nq, nk;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+    int nset, heads, kv_heads, head_dim;
+    float scale;
+    int causal;
+    tb_dtype dtype, out_dtype;
+    void* workspace;
+    size_t workspace_bytes;
+} tb_attention_params;
+
+typedef struct tb_rope_params {
+    const void* x;
+    void* out;
+    const int32_t* coords;
+    int64_t n;
+    int64_t x_row, x_head, out_row, out_head;
+    int coord_stride, axes;
+    int sections[4];
+    int heads, head_dim;
+    double theta;
+    tb_rope_layout layout;
+    tb_rope_freqs freqs;
+    int inverse;
+    tb_dtype dtype;
+} tb_rope_params;
+
+/* Workspace of tb_attention for these parameters (pointers are not looked at); 0 when none is needed. */
+size_t tb_attention_workspace_bytes(const tb_ctx* ctx, const tb_attention_params* params);
+tb_status tb_attention(tb_ctx* ctx, const tb_attention_params* params);
+tb_status tb_rope(tb_ctx* ctx, const tb_rope_params* params);
+size_t tb_group_norm_workspace_bytes(const tb_ctx* ctx, int64_t n, int groups, int nset);
+tb_status tb_group_norm(tb_ctx* ctx, const void* x, tb_dtype x_dtype, const int32_t* offsets, int nset, int64_t n, int c,
+                        int groups, const float* w, const float* b, float eps, tb_epilogue act, tb_dtype out_dtype,
+                        void* out, void* workspace, size_t workspace_bytes);
+
 /* ---- SparseResBlockC2S3d ------------------------------------------------------------------
  * Parameters of one C2S up-block, device pointers named after the reference's tensors under
  * the block prefix (src/sparse.cpp:186-187,259-261,279,316). */

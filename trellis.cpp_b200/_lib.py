@@ -16,6 +16,8 @@ STATUS = {0: "TB_OK", 1: "TB_ERR_INVALID_ARG", 2: "TB_ERR_UNSUPPORTED", 3: "TB_E
           4: "TB_ERR_OUT_OF_MEMORY", 5: "TB_ERR_DEVICE", 6: "TB_ERR_TOO_LARGE"}
 TB_F32, TB_F16, TB_BF16 = 0, 1, 2
 TB_EPI_NONE, TB_EPI_SILU = 0, 1
+TB_ROPE_PAIRS, TB_ROPE_HALVES = 0, 1
+TB_ROPE_FREQS_AXIS, TB_ROPE_FREQS_JOINT = 0, 1
 TB_CONV_AUTO, TB_CONV_GATHER, TB_CONV_BRICK, TB_CONV_PAIR = 0, 1, 2, 3
 
 # Every symbol include/tb_sparse.h declares, with (restype, argtypes).
@@ -41,6 +43,23 @@ class ZSlab(ctypes.Structure):
     """tb_zslab (include/tb_sparse.h)."""
     _fields_ = [("z_lo", _i32), ("z_hi", _i32), ("n_local", _i64), ("n_owned", _i64), ("owned_begin", _i64),
                 ("n_halo_lo", _i64), ("n_halo_hi", _i64), ("n_edge_lo", _i64), ("n_edge_hi", _i64)]
+
+
+class AttentionParams(ctypes.Structure):
+    """tb_attention_params (include/tb_sparse.h)."""
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("lse", _vp), ("q_offsets", _vp), ("k_offsets", _vp),
+                ("nq", _i64), ("nk", _i64), ("q_row", _i64), ("q_head", _i64), ("k_row", _i64), ("k_head", _i64),
+                ("v_row", _i64), ("v_head", _i64), ("out_row", _i64), ("out_head", _i64), ("nset", _int),
+                ("heads", _int), ("kv_heads", _int), ("head_dim", _int), ("scale", ctypes.c_float), ("causal", _int),
+                ("dtype", _int), ("out_dtype", _int), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class RopeParams(ctypes.Structure):
+    """tb_rope_params (include/tb_sparse.h)."""
+    _fields_ = [("x", _vp), ("out", _vp), ("coords", _vp), ("n", _i64), ("x_row", _i64), ("x_head", _i64),
+                ("out_row", _i64), ("out_head", _i64), ("coord_stride", _int), ("axes", _int), ("sections", _int * 4),
+                ("heads", _int), ("head_dim", _int), ("theta", ctypes.c_double), ("layout", _int), ("freqs", _int),
+                ("inverse", _int), ("dtype", _int)]
 
 
 SIGNATURES = {
@@ -72,6 +91,12 @@ SIGNATURES = {
                                  _vp]),
     "tb_linear": (_st, [_vp, _i64, _int, _int, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _vp]),
     "tb_layer_norm": (_st, [_vp, _vp, _int, _i64, _int, _vp, _vp, ctypes.c_float, _int, _int, _vp]),
+    "tb_attention_workspace_bytes": (ctypes.c_size_t, [_vp, ctypes.POINTER(AttentionParams)]),
+    "tb_attention": (_st, [_vp, ctypes.POINTER(AttentionParams)]),
+    "tb_rope": (_st, [_vp, ctypes.POINTER(RopeParams)]),
+    "tb_group_norm_workspace_bytes": (ctypes.c_size_t, [_vp, _i64, _int, _int]),
+    "tb_group_norm": (_st, [_vp, _vp, _int, _vp, _int, _i64, _int, _int, _vp, _vp, ctypes.c_float, _int, _int, _vp, _vp,
+                            ctypes.c_size_t]),
     "tb_gguf_open": (_st, [ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "tb_gguf_close": (None, [_vp]),
     "tb_gguf_n_tensors": (_i64, [_vp]),

@@ -1,0 +1,20 @@
+// Arguments shared by the attention kernels (tb_attention.cu, tb_attention_tc.cu).
+#pragma once
+
+#include "tb_common.cuh"
+
+struct AttnArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    float* lse;                      // [nq][heads] or null
+    const int32_t* q_off;
+    const int32_t* k_off;
+    int64_t nq, nk;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;   // in elements
+    int nset, heads, kv_heads, group, dim, causal;
+    int unit;                        // query tokens of a block
+    float scale_log2;                // scale * log2(e): scores in powers of two
+    int* err;
+};

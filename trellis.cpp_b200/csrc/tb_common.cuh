@@ -15,6 +15,7 @@ enum tb_device_error : int {
     TB_DEVERR_HASH_PROBE = 1,     // hash insert/lookup exceeded its probe bound
     TB_DEVERR_WAIT_TIMEOUT = 2,   // a bounded mbarrier wait in the conv kernel ran out
     TB_DEVERR_TMEM_ALLOC = 3,     // TMEM allocation returned an unusable address
+    TB_DEVERR_BAD_OFFSETS = 4,    // an offset table of packed sets descends or leaves the array
 };
 
 struct tb_ctx {
@@ -87,6 +88,13 @@ inline size_t tb_dtype_size(tb_dtype d) { return d == TB_F32 ? 4 : 2; }
 // SiLU v / (1 + e^-v) with the fast exponential and divide (a few ulp); for large negative v the
 // denominator exceeds 2^126 and the result is 0 (the exact value is below 2^-100 in magnitude).
 __device__ __forceinline__ float tb_silu(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
+
+// Whether the dim-element vectors of n rows x heads, `row` and `head` elements apart, share no
+// element (an output's strides).
+inline bool tb_rows_disjoint(int64_t n, int64_t row, int64_t heads, int64_t head, int64_t dim) {
+    if (n <= 1 || heads <= 1) return (n <= 1 || row >= dim) && (heads <= 1 || head >= dim);
+    return (head >= dim && row >= (heads - 1) * head + dim) || (row >= dim && head >= (n - 1) * row + dim);
+}
 
 inline bool tb_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -1,0 +1,139 @@
+// Packed sets: rows of one array that hold one set (object, sequence) after another, set s in
+// rows offsets[s] .. offsets[s+1]-1 of an int32 device array [nset + 1]. Shared by the operators
+// over packed sets (tb_attention*.cu, tb_group_norm.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "tb_common.cuh"
+
+namespace tbpk {
+
+// Rows [lo, hi) of a set. The table lives in device memory, so it is checked here: an offset that
+// is negative, smaller than the one before it or past the array's n rows is clamped (no kernel
+// reads or writes outside the array) and reported through the context's error word.
+__device__ __forceinline__ void set_range(const int32_t* off, int s, int64_t n, int64_t& lo, int64_t& hi, int* err) {
+    if (!off) {
+        lo = 0;
+        hi = n;
+        return;
+    }
+    const int64_t a = off[s], b = off[s + 1];
+    if (a < 0 || b < a || b > n) atomicCAS(err, 0, TB_DEVERR_BAD_OFFSETS);
+    lo = a < 0 ? 0 : (a > n ? n : a);
+    hi = b < lo ? lo : (b > n ? n : b);
+}
+
+struct Item {
+    int set;        // -1: the index is past the last item
+    uint32_t item;  // which piece of the set
+    uint32_t items; // pieces of the set
+    int64_t lo, hi; // the set's rows
+};
+
+// Piece `idx` of the list that cuts every set, in order, into pieces of `unit` rows. All threads of
+// the block call it (at most 1024); each sums the pieces of its share of the sets, a scan over the
+// threads finds the owner of `idx`, which walks its share. One table read per thread up to
+// blockDim.x sets. `res` and `warp_sum` (32 words) are shared memory.
+__device__ __forceinline__ void find_item(const int32_t* off, int nset, int64_t n, int unit, uint32_t idx, int* err,
+                                          Item* res, uint32_t* warp_sum) {
+    const int t = threadIdx.x, nt = blockDim.x, lane = t & 31, warp = t >> 5;
+    const int per = (nset + nt - 1) / nt;
+    const int s0 = min(nset, t * per), s1 = min(nset, s0 + per);
+    uint32_t sum = 0;
+    int64_t lo = 0, hi = 0;
+    for (int s = s0; s < s1; ++s) {
+        set_range(off, s, n, lo, hi, err);
+        sum += (uint32_t)((hi - lo + unit - 1) / unit);
+    }
+    uint32_t inc = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += v;
+    }
+    if (lane == 31) warp_sum[warp] = inc;
+    if (t == 0) res->set = -1;
+    __syncthreads();
+    uint32_t base = 0;
+    for (int w = 0; w < warp; ++w) base += warp_sum[w];
+    uint32_t first = base + inc - sum;
+    if (idx >= first && idx - first < sum) {
+        for (int s = s0; s < s1; ++s) {
+            if (s1 - s0 > 1) set_range(off, s, n, lo, hi, err);
+            const uint32_t c = (uint32_t)((hi - lo + unit - 1) / unit);
+            if (idx - first < c) {
+                res->set = s;
+                res->item = idx - first;
+                res->items = c;
+                res->lo = lo;
+                res->hi = hi;
+                break;
+            }
+            first += c;
+        }
+    }
+    __syncthreads();
+}
+
+// ---- 8 consecutive elements of a 16-byte aligned row as float ------------------------------------
+template <class T> __device__ __forceinline__ void load8(const T* p, float* v);
+template <> __device__ __forceinline__ void load8<float>(const float* p, float* v) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void unpack2(uint32_t w, float* v, __nv_bfloat16) {
+    v[0] = __uint_as_float(w << 16);
+    v[1] = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack2(uint32_t w, float* v, __half) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    v[0] = f.x;
+    v[1] = f.y;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <class T> __device__ __forceinline__ void unpack8(uint4 w, float* v) {
+    unpack2(w.x, v, T());
+    unpack2(w.y, v + 2, T());
+    unpack2(w.z, v + 4, T());
+    unpack2(w.w, v + 6, T());
+}
+template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float* v) {
+    unpack8<__nv_bfloat16>(*reinterpret_cast<const uint4*>(p), v);
+}
+template <> __device__ __forceinline__ void load8<__half>(const __half* p, float* v) {
+    unpack8<__half>(*reinterpret_cast<const uint4*>(p), v);
+}
+template <class T> __device__ __forceinline__ void store8(T* p, const float* v) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()),
+                                              pack2(v[6], v[7], T()));
+}
+template <> __device__ __forceinline__ void store8<float>(float* p, const float* v) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+}  // namespace tbpk
+
+// The calling thread's current device is put back when the call returns.
+struct tb_device_guard {
+    int prev = -1;
+    cudaError_t enter(int device) {
+        cudaError_t e = cudaGetDevice(&prev);
+        if (e == cudaSuccess && prev != device) return cudaSetDevice(device);
+        prev = -1;
+        return e;
+    }
+    ~tb_device_guard() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+};

@@ -1,0 +1,196 @@
+// Rotary positions with several axes: the pair p of every head of row i turns by the angle
+//   pos[i][axis(p)] * f_p,   (a, b) -> (a cos - b sin, a sin + b cos),
+// where the first sections[0] pairs of a head take axis 0 (a voxel's x), the next sections[1] axis
+// 1, and so on; pairs past the last section keep their values. f_p = theta^(-j / sections[axis])
+// with j the pair's place in its section, or theta^(-p / (head_dim/2)) with frequencies shared by
+// the axes. inverse turns by the negative angle, which is the transpose: the gradient's way back.
+//
+// Angles: far positions times a 32-bit frequency lose the phase (position 1e5 at f = 1: 4e-3), so
+// the angle is counted in revolutions in 64 bits, its whole part dropped, and the rest given to
+// sincospif in 32 bits. A thread owns a few pairs of one row and computes their sines once for
+// all heads it turns. Bound by memory: each value is read and written once.
+#include "tb_packed.cuh"
+
+#include <cmath>
+
+namespace {
+
+using namespace tbpk;
+
+constexpr int kRopeThreads = 256;
+constexpr int kRopeMaxPairs = 128;
+
+struct RopeArgs {
+    const void* x;
+    void* out;
+    const int32_t* pos;       // column of axis 0 of row 0
+    int64_t n, x_row, x_head, out_row, out_head;
+    int pos_stride, heads, half, chunks, heads_per;
+    float sign;               // -1 turns backwards
+    double freq[kRopeMaxPairs];      // revolutions per position; 0: the pair is kept
+    uint8_t axis[kRopeMaxPairs];
+};
+
+// P pairs of one head. PAIRS: elements 2p, 2p+1; otherwise p and p + half.
+template <class T, int P, bool PAIRS>
+__device__ __forceinline__ void rope_load(const T* h, int p0, int half, float* a, float* b) {
+    if (PAIRS) {
+        float v[2 * P];
+#pragma unroll
+        for (int i = 0; i < 2 * P; i += 8) load8<T>(h + 2 * p0 + i, v + i);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            a[i] = v[2 * i];
+            b[i] = v[2 * i + 1];
+        }
+    } else if (P == 8) {
+        load8<T>(h + p0, a);
+        load8<T>(h + half + p0, b);
+    } else if (sizeof(T) == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(h + p0), v = *reinterpret_cast<const float4*>(h + half + p0);
+        a[0] = u.x; a[1] = u.y; a[2] = u.z; a[3] = u.w;
+        b[0] = v.x; b[1] = v.y; b[2] = v.z; b[3] = v.w;
+    } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(h + p0), v = *reinterpret_cast<const uint2*>(h + half + p0);
+        using H = typename std::conditional<sizeof(T) == 4, __half, T>::type;
+        unpack2(u.x, a, H()); unpack2(u.y, a + 2, H());
+        unpack2(v.x, b, H()); unpack2(v.y, b + 2, H());
+    }
+}
+
+template <class T, int P, bool PAIRS>
+__device__ __forceinline__ void rope_store(T* h, int p0, int half, const float* a, const float* b) {
+    if (PAIRS) {
+        float v[2 * P];
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            v[2 * i] = a[i];
+            v[2 * i + 1] = b[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * P; i += 8) store8<T>(h + 2 * p0 + i, v + i);
+    } else if (P == 8) {
+        store8<T>(h + p0, a);
+        store8<T>(h + half + p0, b);
+    } else if (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(h + p0) = make_float4(a[0], a[1], a[2], a[3]);
+        *reinterpret_cast<float4*>(h + half + p0) = make_float4(b[0], b[1], b[2], b[3]);
+    } else {
+        using H = typename std::conditional<sizeof(T) == 4, __half, T>::type;
+        *reinterpret_cast<uint2*>(h + p0) = make_uint2(pack2(a[0], a[1], H()), pack2(a[2], a[3], H()));
+        *reinterpret_cast<uint2*>(h + half + p0) = make_uint2(pack2(b[0], b[1], H()), pack2(b[2], b[3], H()));
+    }
+}
+
+template <class T, int P, bool PAIRS>
+__global__ void __launch_bounds__(kRopeThreads) k_rope(const __grid_constant__ RopeArgs r) {
+    const int64_t t = (int64_t)blockIdx.x * kRopeThreads + threadIdx.x;
+    const int64_t row = t / r.chunks;
+    if (row >= r.n) return;
+    const int p0 = (int)(t - row * r.chunks) * P;
+    const int h0 = blockIdx.y * r.heads_per, h1 = min(r.heads, h0 + r.heads_per);
+    float c[P], s[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const double turns = (double)r.pos[row * r.pos_stride + r.axis[p0 + i]] * r.freq[p0 + i];
+        sincospif(2.f * (float)(turns - rint(turns)), s + i, c + i);
+        s[i] *= r.sign;
+    }
+    const T* x = reinterpret_cast<const T*>(r.x) + row * r.x_row + h0 * r.x_head;
+    T* o = reinterpret_cast<T*>(r.out) + row * r.out_row + h0 * r.out_head;
+#pragma unroll 4
+    for (int h = h0; h < h1; ++h, x += r.x_head, o += r.out_head) {
+        float a[P], b[P], ya[P], yb[P];
+        rope_load<T, P, PAIRS>(x, p0, r.half, a, b);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            ya[i] = a[i] * c[i] - b[i] * s[i];
+            yb[i] = a[i] * s[i] + b[i] * c[i];
+        }
+        rope_store<T, P, PAIRS>(o, p0, r.half, ya, yb);
+    }
+}
+
+template <class T>
+void launch_rope(const RopeArgs& r, bool pairs, int per, dim3 grid, cudaStream_t stream) {
+    if (pairs) k_rope<T, 4, true><<<grid, kRopeThreads, 0, stream>>>(r);
+    else if (per == 8) k_rope<T, 8, false><<<grid, kRopeThreads, 0, stream>>>(r);
+    else k_rope<T, 4, false><<<grid, kRopeThreads, 0, stream>>>(r);
+}
+
+}  // namespace
+
+extern "C" tb_status tb_rope(tb_ctx* ctx, const tb_rope_params* p) {
+    if (!ctx) return TB_ERR_INVALID_ARG;
+    if (!p) return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: null parameters");
+    if (p->dtype != TB_F32 && p->dtype != TB_F16 && p->dtype != TB_BF16)
+        return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: bad dtype");
+    if (p->n < 0 || p->heads < 1) return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: n < 0 or heads < 1");
+    if (p->head_dim < 8 || p->head_dim % 8 != 0 || p->head_dim > 2 * kRopeMaxPairs)
+        return tb_fail(ctx, TB_ERR_UNSUPPORTED, "tb_rope: head_dim must be a multiple of 8 up to 256");
+    if (p->layout != TB_ROPE_PAIRS && p->layout != TB_ROPE_HALVES)
+        return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: bad layout");
+    if (p->freqs != TB_ROPE_FREQS_AXIS && p->freqs != TB_ROPE_FREQS_JOINT)
+        return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: bad frequency rule");
+    if (p->axes < 1 || p->axes > 4 || p->coord_stride < p->axes)
+        return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: needs 1 to 4 axes and coord_stride >= axes");
+    if (!(p->theta > 0) || !std::isfinite(p->theta)) return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: theta must be positive");
+    const int half = p->head_dim / 2;
+    int64_t total = 0;
+    for (int a = 0; a < p->axes; ++a) {
+        if (p->sections[a] < 1) return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: a section needs at least one pair");
+        total += p->sections[a];
+    }
+    if (total > half) return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: the sections have more pairs than a head");
+    if (p->n == 0) return TB_OK;
+    if (p->n >= (int64_t)INT32_MAX) return tb_fail(ctx, TB_ERR_TOO_LARGE, "tb_rope: n must be < 2^31-1");
+    if (!p->x || !p->out || !p->coords) return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: null pointer");
+    const int64_t unit = 16 / (int64_t)tb_dtype_size(p->dtype);
+    const bool rows = p->n > 1, hds = p->heads > 1;          // a single row's or head's stride is not used
+    if (!tb_aligned16(p->x) || !tb_aligned16(p->out) || (rows && (p->x_row % unit || p->out_row % unit)) ||
+        (hds && (p->x_head % unit || p->out_head % unit)))
+        return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: pointers and strides must be multiples of 16 bytes");
+    if (!tb_rows_disjoint(p->n, p->out_row, p->heads, p->out_head, p->head_dim))
+        return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: rows or heads of out overlap");
+    if (p->out == p->x && ((rows && p->out_row != p->x_row) || (hds && p->out_head != p->x_head)))
+        return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: in place needs equal strides");
+
+    RopeArgs r;
+    r.x = p->x;
+    r.out = p->out;
+    r.pos = p->coords + (p->coord_stride - p->axes);
+    r.n = p->n;
+    r.x_row = p->x_row;
+    r.x_head = p->x_head;
+    r.out_row = p->out_row;
+    r.out_head = p->out_head;
+    r.pos_stride = p->coord_stride;
+    r.heads = p->heads;
+    r.half = half;
+    r.sign = p->inverse ? -1.f : 1.f;
+    const double lg = std::log2(p->theta), turn = 0.15915494309189533577;   // 1 / (2 pi)
+    int q = 0;
+    for (int a = 0; a < p->axes; ++a)
+        for (int j = 0; j < p->sections[a]; ++j, ++q) {
+            const double power = p->freqs == TB_ROPE_FREQS_JOINT ? (double)q / half : (double)j / p->sections[a];
+            r.freq[q] = turn * std::exp2(-power * lg);
+            r.axis[q] = (uint8_t)a;
+        }
+    for (; q < half; ++q) {
+        r.freq[q] = 0.0;
+        r.axis[q] = 0;
+    }
+    const bool pairs = p->layout == TB_ROPE_PAIRS;
+    const int per = !pairs && p->dtype != TB_F32 && half % 8 == 0 ? 8 : 4;
+    r.chunks = half / per;
+    const int64_t blocks = (p->n * r.chunks + kRopeThreads - 1) / kRopeThreads;
+    r.heads_per = p->heads;
+    tb_device_guard guard;
+    TB_CUDA_TRY(ctx, guard.enter(ctx->device));
+    const dim3 grid((unsigned)blocks, (unsigned)((p->heads + r.heads_per - 1) / r.heads_per));
+    if (p->dtype == TB_F32) launch_rope<float>(r, pairs, per, grid, ctx->stream);
+    else if (p->dtype == TB_F16) launch_rope<__half>(r, pairs, per, grid, ctx->stream);
+    else launch_rope<__nv_bfloat16>(r, pairs, per, grid, ctx->stream);
+    TB_LAUNCH_CHECK(ctx, "k_rope");
+    return TB_OK;
+}

@@ -12,6 +12,9 @@ Names and argument meanings follow pwilkin/trellis.cpp's ``include/sparse.h``:
 * :func:`sparse_c2s` -- ``trellis::sparse_c2s`` (sparse.h:27-35), the whole C2S up-block
 * :func:`submconv_stack_host` -- a host-buffer stage run (upload, map, convs, read back), the
   shape of ``run1`` / ``GraphRun::run`` (src/shape_decoder.cpp:34-51)
+* :func:`attention`, :func:`rope`, :func:`group_norm` -- the layers of a transformer over packed
+  voxel or token sets (no counterpart in the reference's sparse.h), next to :func:`linear` and
+  :func:`layer_norm`
 
 Device tensors are torch CUDA tensors used only as memory; every computation runs in
 libtb_sparse.so. Errors raise :class:`TBError` (the reference throws std::runtime_error).
@@ -265,6 +268,159 @@ def layer_norm(x: torch.Tensor, w=None, b=None, eps: float = 1e-6, act: str = "n
     ctx = context(x.device)
     check(_lib.load().tb_layer_norm(ctx, _ptr(x), _DT[x.dtype], n, c, _ptr(w), _ptr(b), eps, _EPI[act], _DT[od],
                                     _ptr(out)), "tb_layer_norm", ctx)
+    return out
+
+
+# ---- transformer operators over packed sets -------------------------------------------------
+_LAYOUT = {"pairs": _lib.TB_ROPE_PAIRS, "halves": _lib.TB_ROPE_HALVES}
+_FREQS = {"axis": _lib.TB_ROPE_FREQS_AXIS, "joint": _lib.TB_ROPE_FREQS_JOINT}
+
+
+def _need_heads(t: torch.Tensor, name: str):
+    if not t.is_cuda or t.dim() != 3 or t.dtype not in _DT or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError(f"{name} must be a CUDA tensor [N, heads, head_dim] of float32/float16/bfloat16 with "
+                         "contiguous heads")
+
+
+def _same_device(first: torch.Tensor, *ts):
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise ValueError("all tensors must be on one device")
+
+
+def _offsets(t, name: str):
+    if not t.is_cuda or t.dtype != torch.int32 or t.dim() != 1 or t.numel() < 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 CUDA tensor [sets + 1]")
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor | None = None,
+              k_offsets: torch.Tensor | None = None, causal: bool = False, scale: float | None = None, out_dtype=None,
+              out: torch.Tensor | None = None, return_lse: bool = False):
+    """softmax(scale * q k^T) v within each packed set (tb_attention).
+
+    q [Nq, H, D], k and v [Nk, Hk, D] of one dtype, H a multiple of Hk (head h reads key head
+    h // (H // Hk)); rows and heads may be strided (views of one q|k|v product). Set s has query rows
+    q_offsets[s]:q_offsets[s+1] and key rows k_offsets[s]:k_offsets[s+1] (int32, device; k_offsets
+    None: the same table; both None: one set). ``causal``: a query sees the keys up to its own
+    place, counted from the ends of both. ``scale``: 1/sqrt(D) when None. Rows without a key give
+    0; rows outside every set are not written (with ``out`` None: undefined). ``return_lse``: also
+    the float32 [Nq, H] log of each row's softmax sum."""
+    _need_heads(q, "q")
+    _need_heads(k, "k")
+    _need_heads(v, "v")
+    _same_device(q, k, v, q_offsets, k_offsets, out)
+    nq, h, d = q.shape
+    nk, hk, _ = k.shape
+    if k.dtype != q.dtype or v.dtype != q.dtype or v.shape != k.shape or k.shape[2] != d:
+        raise ValueError("q [Nq,H,D], k and v [Nk,Hk,D] must share a dtype and D")
+    if q_offsets is None:
+        if k_offsets is not None:
+            raise ValueError("k_offsets needs q_offsets")
+        nset = 1
+    else:
+        _offsets(q_offsets, "q_offsets")
+        if k_offsets is None:
+            k_offsets = q_offsets
+        else:
+            _offsets(k_offsets, "k_offsets")
+        nset = q_offsets.numel() - 1
+        if k_offsets.numel() != nset + 1:
+            raise ValueError("q_offsets and k_offsets must have the same number of sets")
+    if out is None:
+        out = torch.empty((nq, h, d), dtype=q.dtype if out_dtype is None else out_dtype, device=q.device)
+    else:
+        _need_heads(out, "out")
+        if tuple(out.shape) != (nq, h, d) or (out_dtype is not None and out.dtype != out_dtype):
+            raise ValueError("out must be [Nq, H, D] of out_dtype")
+    lse = torch.empty((nq, h), dtype=torch.float32, device=q.device) if return_lse else None
+    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
+    p = _lib.AttentionParams(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
+        None if q_offsets is None else q_offsets.data_ptr(), None if k_offsets is None else k_offsets.data_ptr(),
+        nq, nk, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], nset, h, hk, d,
+        d ** -0.5 if scale is None else scale, 1 if causal else 0, _DT[q.dtype], _DT[out.dtype], None, 0)
+    ctx = context(q.device)
+    lib = _lib.load()
+    need = lib.tb_attention_workspace_bytes(ctx, p)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), need
+    st = lib.tb_attention(ctx, p)
+    if st:
+        check(st, "tb_attention", ctx)
+    return (out, lse) if return_lse else out
+
+
+def rope(x: torch.Tensor, coords: torch.Tensor, sections, theta: float = 10000.0, layout: str = "pairs",
+         freqs: str = "axis", inverse: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions along the axes of ``coords`` (tb_rope).
+
+    x [N, H, D] (rows and heads may be strided: the q and k heads of one q|k|v product are one
+    call); coords int32 [N, axes] or [N, axes + 1] with the batch in front, as voxel rows have it;
+    ``sections[a]`` pairs of each head turn with axis a, the rest are copied. ``layout``: pairs
+    (2p, 2p+1) or halves (p, p + D/2). ``freqs``: theta**(-j/sections[a]) within each axis, or
+    "joint": theta**(-p/(D/2)). ``inverse`` turns back (and carries gradients). ``out`` may be x."""
+    _need_heads(x, "x")
+    n, h, d = x.shape
+    axes = len(sections)
+    if not 1 <= axes <= 4:
+        raise ValueError("1 to 4 sections")
+    if not coords.is_cuda or coords.dtype != torch.int32 or coords.dim() != 2 or not coords.is_contiguous() \
+            or coords.shape[0] != n or coords.shape[1] not in (axes, axes + 1):
+        raise ValueError("coords must be a contiguous int32 CUDA tensor [N, axes] or [N, axes + 1]")
+    if layout not in _LAYOUT or freqs not in _FREQS:
+        raise ValueError('layout must be "pairs" or "halves", freqs "axis" or "joint"')
+    _same_device(x, coords, out)
+    if out is None:
+        out = torch.empty((n, h, d), dtype=x.dtype, device=x.device)
+    else:
+        _need_heads(out, "out")
+        if out.shape != x.shape or out.dtype != x.dtype:
+            raise ValueError("out must be [N, H, D] of x's dtype")
+    xs, os_ = x.stride(), out.stride()
+    p = _lib.RopeParams(x.data_ptr(), out.data_ptr(), coords.data_ptr(), n, xs[0], xs[1], os_[0], os_[1], coords.shape[1],
+                        axes, tuple(sections), h, d, theta, _LAYOUT[layout], _FREQS[freqs], 1 if inverse else 0,
+                        _DT[x.dtype])
+    ctx = context(x.device)
+    st = _lib.load().tb_rope(ctx, p)
+    if st:
+        check(st, "tb_rope", ctx)
+    return out
+
+
+def group_norm(x: torch.Tensor, groups: int, w=None, b=None, offsets: torch.Tensor | None = None, eps: float = 1e-5,
+               act: str = "none", out_dtype=None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """act(GroupNorm(x) * w + b) of each packed set over its rows and a group's channels (tb_group_norm).
+
+    x [N, C]; w, b float32 [C] or None; set s is rows offsets[s]:offsets[s+1] (int32, device; None:
+    one set). Rows outside every set are not written (with ``out`` None: undefined). ``out`` may be x."""
+    _need_cuda(x)
+    if x.dim() != 2 or x.dtype not in _DT:
+        raise ValueError("x must be [N, C] of float32/float16/bfloat16")
+    n, c = x.shape
+    for t, name in ((w, "w"), (b, "b")):
+        if t is not None:
+            _f32_vec(t, c, name)
+    nset = 1
+    if offsets is not None:
+        _offsets(offsets, "offsets")
+        nset = offsets.numel() - 1
+    _same_device(x, w, b, offsets, out)
+    if out is None:
+        out = torch.empty((n, c), dtype=x.dtype if out_dtype is None else out_dtype, device=x.device)
+    else:
+        _need_cuda(out)
+        if out.shape != x.shape or out.dtype not in _DT or (out_dtype is not None and out.dtype != out_dtype):
+            raise ValueError("out must be [N, C] of out_dtype")
+    ctx = context(x.device)
+    lib = _lib.load()
+    need = lib.tb_group_norm_workspace_bytes(ctx, n, groups, nset)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    st = lib.tb_group_norm(ctx, x.data_ptr(), _DT[x.dtype], None if offsets is None else offsets.data_ptr(), nset, n, c,
+                           groups, None if w is None else w.data_ptr(), None if b is None else b.data_ptr(), eps,
+                           _EPI[act], _DT[out.dtype], out.data_ptr(), None if ws is None else ws.data_ptr(), need)
+    if st:
+        check(st, "tb_group_norm", ctx)
     return out
 
 
