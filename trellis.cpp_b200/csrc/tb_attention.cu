@@ -264,7 +264,10 @@ tb_status attn_args(tb_ctx* ctx, const tb_attention_params* p, AttnArgs& a) {
 }  // namespace
 
 extern "C" size_t tb_attention_workspace_bytes(const tb_ctx* ctx, const tb_attention_params* p) {
-    return 0;
+    if (!ctx || !p || (p->dtype != TB_F16 && p->dtype != TB_BF16) || p->heads < 1 || p->kv_heads < 1 ||
+        p->heads % p->kv_heads != 0 || p->heads / p->kv_heads > 64 || p->head_dim < 1)
+        return 0;
+    return tb_attn_tc_workspace(ctx, p->nq, p->nk, p->nset, p->heads, p->kv_heads, p->head_dim);
 }
 
 extern "C" tb_status tb_attention(tb_ctx* ctx, const tb_attention_params* p) {
@@ -273,9 +276,14 @@ extern "C" tb_status tb_attention(tb_ctx* ctx, const tb_attention_params* p) {
     const tb_status s = attn_args(ctx, p, a);
     if (s != TB_OK) return s;
     if (a.nq == 0 || a.nset == 0) return TB_OK;
+    const size_t need = tb_attention_workspace_bytes(ctx, p);
+    if (need && (!p->workspace || p->workspace_bytes < need || !tb_aligned16(p->workspace)))
+        return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_attention: workspace too small or not 16-byte aligned");
     tb_device_guard guard;
     TB_CUDA_TRY(ctx, guard.enter(ctx->device));
     if (p->dtype == TB_F32) return launch_cc_dim<float, float>(ctx, a);
+    if (a.nk > 0) return tb_attn_tc_launch(ctx, a, p->dtype, p->out_dtype, p->workspace);
+    // no key rows to describe to the tensor cores' loads: every row is 0
     if (p->dtype == TB_F16)
         return p->out_dtype == TB_F32 ? launch_cc_dim<__half, float>(ctx, a) : launch_cc_dim<__half, __half>(ctx, a);
     return p->out_dtype == TB_F32 ? launch_cc_dim<__nv_bfloat16, float>(ctx, a)

@@ -18,3 +18,7 @@ struct AttnArgs {
     float scale_log2;                // scale * log2(e): scores in powers of two
     int* err;
 };
+
+// 16-bit operands on tensor cores; nq, nk, nset > 0.
+size_t tb_attn_tc_workspace(const tb_ctx* ctx, int64_t nq, int64_t nk, int nset, int heads, int kv_heads, int dim);
+tb_status tb_attn_tc_launch(tb_ctx* ctx, const AttnArgs& args, tb_dtype dtype, tb_dtype out_dtype, void* workspace);
