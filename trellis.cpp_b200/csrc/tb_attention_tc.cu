@@ -6,7 +6,7 @@
 // blocks of 128: S = Q K^T into 128 TMEM columns a tile, softmax by one warpgroup a tile (a thread
 // owns a row: no exchange between threads), P over S's columns as the A operand of O += P V, which
 // stays in TMEM. While one tile's warpgroup computes its softmax the tensor pipe works on the other
-// tile. Warp 9 streams Q, K and V by TMA, warp 8 issues the MMAs.
+// tile. One warp streams Q, K and V by TMA, one a tile issues the MMAs.
 //
 // The running maximum moves only when a block's exceeds it by more than 2^8 (in units of p): until
 // then p grows to at most 2^8, which the 32-bit sums hold as well, and O need not be scaled; the
@@ -28,9 +28,20 @@ namespace {
 using namespace tbtc;
 using namespace tbpk;
 
-constexpr int kThreads = 320;          // warps 0-3 and 4-7 softmax, 8 MMA, 9 TMA
+constexpr int kThreads = 384;          // warps 0-3 and 4-7 softmax, 8 and 9 MMA, 10 TMA, 11 idle
+// Registers: 65536 / 384 threads allows 168 at launch; the third warpgroup gives up what the two
+// softmax warpgroups need to hold a row of S. 2 * 208 + 88 = 3 * 168.
+constexpr int kRegsSoftmax = 208, kRegsOther = 88;
 constexpr int kKeys = 128;             // keys of a block
 constexpr float kRaise = 8.f;          // the maximum follows when a block's is 2^8 above it
+#ifndef TB_FIRST
+#define TB_FIRST 96
+#endif
+constexpr int kFirst = TB_FIRST;             // keys of a block whose p the products may read early
+#ifndef TB_POLY
+#define TB_POLY 3
+#endif
+constexpr int kPoly = TB_POLY;         // of every 8 pairs of exponentials, those by polynomial
 
 struct TcArgs {
     AttnArgs a;
@@ -45,7 +56,7 @@ template <int D, bool ALT> struct Geom {
     static constexpr int kTileBytes = kBoxes * 16384;         // 128 rows x D, boxes of 64 columns
     static constexpr int kQTiles = ALT ? 1 : 2;
     static constexpr int kStages = D == 64 ? 10 : (ALT ? 6 : 5);
-    static constexpr int kBars = 2 * kStages + 1 + 2 + 2 + 2 + 1;
+    static constexpr int kBars = 2 * kStages + 1 + 2 + 2 + 2 + 2 + 2 + 1;
     static constexpr size_t kSmem = (size_t)(kQTiles + kStages) * kTileBytes + 8 * kBars + 16 + 1024;
 };
 
@@ -54,12 +65,11 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
                  " [%0], [%1, {%2, %3, %4}], [%5];"
                  :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
-// V's tile as the B operand with its N dimension (the head's columns) contiguous: boxes of 64
-// columns 16384 bytes apart, groups of 8 keys 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc_v(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
-           (2ull << 61);
-}
+// Shared-memory descriptors of tiles in the 128-byte swizzle: low word (address >> 4) | leading
+// offset << 16, high word 8-row groups 1024 bytes apart. Q and K have their K dimension (the head's
+// columns) contiguous; V is the B operand with N (the head's columns) contiguous, its boxes of 64
+// columns 16384 bytes apart.
+__device__ __forceinline__ uint64_t desc64(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -75,6 +85,100 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, float* v) {
                    "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]),
                    "=f"(v[30]), "=f"(v[31])
                  : "r"(taddr));
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// ---- two 32-bit values in one instruction ---------------------------------------------------------
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack(float a, float b) {
+    f2 y;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float2 unpack(f2 x) {
+    float2 y;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
+    return y;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+    return y;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 y;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 y;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+// 2^x of two values on the FMA pipes, beside the exponential unit: x = i + f with i the nearest whole
+// number, 2^f by the cubic of least relative error on [-1/2, 1/2] (exchange method, 7.5e-5: an
+// eighth of a half step of f16), times 2^i put together from its bits. x is taken at -126 at
+// least; a value that is no number stays one (the product keeps it).
+__device__ __forceinline__ float2 ex2_poly(f2 x) {
+    float2 v = unpack(x);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-126.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-126.f));
+    x = pack(v.x, v.y);
+    const f2 r = add2(x, pack(12582912.f, 12582912.f));                     // 1.5 * 2^23: whole numbers
+    const f2 f = fma2(add2(r, pack(-12582912.f, -12582912.f)), pack(-1.f, -1.f), x);
+    f2 y = fma2(pack(0.0551716685f, 0.0551716685f), f, pack(0.242611125f, 0.242611125f));
+    y = fma2(y, f, pack(0.693260968f, 0.693260968f));
+    y = fma2(y, f, pack(0.999928057f, 0.999928057f));
+    const float2 i = unpack(r);
+    const float e0 = __uint_as_float((__float_as_uint(i.x) << 23) + 0x3f800000u);
+    const float e1 = __uint_as_float((__float_as_uint(i.y) << 23) + 0x3f800000u);
+    return unpack(mul2(y, pack(e0, e1)));
+}
+
+// p = 2^(s c + ref) of a row's 128 scores, left in s and, rounded to T, in the TMEM columns from `ts`.
+// NPOLY of every 8 pairs go by polynomial, which shares the work between the exponential unit (4
+// lanes a cycle and scheduler: 1024 cycles a block and warp, as long as the tile's products) and the
+// FMA pipes. A hidden score (-inf) has to give exactly 0: masked blocks use NPOLY 0.
+template <class T, int NPOLY>
+__device__ __forceinline__ void exp_block(float* s, float c, float ref, uint32_t ts, uint32_t half_bar, int lane) {
+    const f2 c2 = pack(c, c), ref2 = pack(ref, ref);
+#pragma unroll
+    for (int quarter = 0; quarter < 4; ++quarter) {
+        float* v = s + quarter * 32;
+#pragma unroll
+        for (int q = 0; q < 32; q += 2) {
+            const float2 x = unpack(fma2(pack(v[q], v[q + 1]), c2, ref2));
+            v[q] = x.x;
+            v[q + 1] = x.y;
+        }
+#pragma unroll
+        for (int q = 0; q < 16; ++q)
+            if ((q & 7) * NPOLY / 8 == ((q & 7) + 1) * NPOLY / 8) {
+                v[2 * q] = ex2(v[2 * q]);
+                v[2 * q + 1] = ex2(v[2 * q + 1]);
+            }
+#pragma unroll
+        for (int q = 0; q < 16; ++q)
+            if ((q & 7) * NPOLY / 8 != ((q & 7) + 1) * NPOLY / 8) {
+                const float2 y = ex2_poly(pack(v[2 * q], v[2 * q + 1]));
+                v[2 * q] = y.x;
+                v[2 * q + 1] = y.y;
+            }
+        uint32_t w[16];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) w[q] = pack2(v[2 * q], v[2 * q + 1], T());
+        tmem_st_x16(ts + quarter * 16, w);
+        if (quarter == kFirst / 32 - 1) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(half_bar);
+        }
+    }
 }
 
 // What one CTA works on, in shared memory.
@@ -96,7 +200,7 @@ k_attn_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUte
     __shared__ uint32_t scan[32];
     uint8_t* smem = smem_align1024(smem_raw);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (G::kQTiles + G::kStages) * G::kTileBytes);
-    uint32_t* s_misc = reinterpret_cast<uint32_t*>(bars + G::kBars);       // [0] tmem, [1] abort, [2] consumed
+    uint32_t* s_misc = reinterpret_cast<uint32_t*>(bars + G::kBars);       // [0] tmem, [1] abort
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_misc + 1);
     const uint32_t b0 = smem_u32(bars);
     auto full = [&](int s) { return b0 + 8u * s; };
@@ -105,7 +209,9 @@ k_attn_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUte
     auto sfull = [&](int i) { return bq + 8u * (1 + i); };
     auto pfull = [&](int i) { return bq + 8u * (3 + i); };
     auto ofull = [&](int i) { return bq + 8u * (5 + i); };
-    const uint32_t drain = bq + 8u * 7;
+    auto phalf = [&](int i) { return bq + 8u * (7 + i); };
+    auto turn = [&](int i) { return bq + 8u * (9 + i); };
+    const uint32_t drain = bq + 8u * 11;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const AttnArgs& a = p.a;
 
@@ -142,17 +248,18 @@ k_attn_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUte
     if (threadIdx.x == 0) {
         for (int s = 0; s < G::kStages; ++s) {
             mbar_init(full(s), 1);
-            mbar_init(empty(s), 1);
+            mbar_init(empty(s), ALT ? 1 : 2);        // every tile that reads it
         }
         mbar_init(bq, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(sfull(i), 1);
             mbar_init(pfull(i), 4);
+            mbar_init(phalf(i), 4);
+            mbar_init(turn(i), 1);
             mbar_init(ofull(i), 1);
         }
-        mbar_init(drain, 1);
+        mbar_init(drain, 2);
         s_misc[1] = 0;
-        s_misc[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 8) {
@@ -167,7 +274,9 @@ k_attn_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUte
     const uint32_t sq = smem_u32(smem), skv = sq + G::kQTiles * G::kTileBytes;
     int issued = 0;
 
-    if (warp == 9) {
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsOther));
+    if (warp == 10) {
         // ------------------------------------------------------------------ TMA producer
         if (nmax > 0 && elect_one()) {
             const bool two = !ALT && j.n[1] > 0;
@@ -196,48 +305,88 @@ k_attn_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUte
         }
         issued = __shfl_sync(0xffffffffu, __reduce_max_sync(0xffffffffu, issued), 0);
         __syncwarp();
-    } else if (warp == 8) {
-        // ------------------------------------------------------------------ MMA issuer
+    } else if (warp < 10) {
+        // ------------------------------------------------------------------ MMA issuers, one a tile
+        // A wait costs some 150 cycles of dependent instructions even when its phase is over, and one
+        // warp for both tiles left the tensor pipe idle for 1600 of 3600 cycles a block; so each tile
+        // has its own, the ring's place is counted along and descriptors differ by constants.
+        const int i = warp - 8;
         bool ok = nmax > 0;
-        const int ks = (a.dim + 15) / 16;
+        uint32_t stage = 0, round = 0;               // ring place of the next item
         auto wait = [&](uint32_t bar, uint32_t par) {
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, par, s_abort, a.err));
-            tc_fence_after();
             return ok;
         };
-        auto need = [&](int it) { return wait(full(it % G::kStages), (uint32_t)((it / G::kStages) & 1)); };
-        auto free_stage = [&](int it) {
-            if (elect_one()) tc_commit(empty(it % G::kStages));
-            __syncwarp();
-            if (lane == 0) s_misc[2] = (uint32_t)(it + 1);
+        auto take = [&]() {                          // the next ring item once it has landed
+            const uint32_t st = stage;
+            wait(full(st), round);
+            if (++stage == G::kStages) {
+                stage = 0;
+                round ^= 1;
+            }
+            return st;
         };
-        // S of tile i = Q K^T, ring item `it` holding K; `next` is committed with it
-        auto mma_s = [&](int i, int it) {
+        auto release = [&](uint32_t st) {
+            if (elect_one()) tc_commit(empty(st));
+            __syncwarp();
+        };
+        const uint32_t qlo = (sq >> 4) | (1u << 16), klo = (skv >> 4) | (1u << 16), vlo = (skv >> 4) | (1024u << 16);
+        constexpr uint32_t kHi = 64u | (1u << 14) | (2u << 29);
+        // S of tile i = Q K^T with K in ring place st
+        auto mma_s = [&](uint32_t st) {
+            const uint32_t ql = qlo + (ALT ? 0u : (uint32_t)(i * (G::kTileBytes >> 4))), kl = klo + st * (G::kTileBytes >> 4);
+            tc_fence_after();
             if (elect_one()) {
-                const uint32_t qa = sq + (ALT ? 0 : i) * G::kTileBytes, ka = skv + (it % G::kStages) * G::kTileBytes;
-                for (int k = 0; k < ks; ++k) {
-                    const uint32_t o = (uint32_t)((k >> 2) * 16384 + (k & 3) * 32);
-                    tc_mma(tmem + (uint32_t)(i * 128), smem_desc<128>(qa + o), smem_desc<128>(ka + o), p.idesc_s, k ? 1u : 0u);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t o = (uint32_t)((k >> 2) * 1024 + (k & 3) * 2);
+                    if (k * 16 < a.dim)
+                        tc_mma(tmem + (uint32_t)(i * 128), desc64(ql + o, kHi), desc64(kl + o, kHi), p.idesc_s, k ? 1u : 0u);
                 }
                 tc_commit(sfull(i));
             }
             __syncwarp();
         };
-        // O of tile i += P V over the block's first `keys` keys
-        auto mma_o = [&](int i, int it, bool first, int keys) {
+        // The tiles take turns, a block's P V and the next S together: issued at once they would finish
+        // together, and both softmaxes would then wait for the tensor pipe and it for them.
+        auto my_turn = [&](int k) {
+            if (!ALT && (i || k)) wait(turn(i), (uint32_t)((k - 1 + i) & 1));
+            return ok;
+        };
+        auto pass = [&]() {
+            if (!ALT && lane == 0) mbar_arrive(turn(1 - i));
+        };
+        // O of tile i += P V over the block's first `keys` keys, the early ones as soon as their p is there
+        auto mma_o = [&](uint32_t st, int blk, bool first, int keys, uint32_t par) {
+            const uint32_t vl = vlo + st * (G::kTileBytes >> 4);
+            const uint32_t td = tmem + 256u + (uint32_t)(i * D), ta = tmem + (uint32_t)(i * 128);
+            if (!my_turn(blk + 1) || !wait(phalf(i), par)) return false;
+            tc_fence_after();
             if (elect_one()) {
-                const uint32_t va = skv + (it % G::kStages) * G::kTileBytes;
-                for (int k = 0; k < (keys + 15) / 16; ++k)
-                    tc_mma_ts(tmem + 256u + (uint32_t)(i * D), tmem + (uint32_t)(i * 128 + k * 8), desc_v(va + k * 2048),
-                              p.idesc_o, first && k == 0 ? 0u : 1u);
+#pragma unroll
+                for (int k = 0; k < kFirst / 16; ++k)
+                    if (k * 16 < keys) tc_mma_ts(td, ta + k * 8, desc64(vl + k * 128, kHi), p.idesc_o, first && k == 0 ? 0u : 1u);
             }
+            __syncwarp();
+            if (!wait(pfull(i), par)) return false;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+                for (int k = kFirst / 16; k < kKeys / 16; ++k)
+                    if (k * 16 < keys) tc_mma_ts(td, ta + k * 8, desc64(vl + k * 128, kHi), p.idesc_o, 1u);
+            }
+            __syncwarp();
+            return true;
+        };
+        auto last = [&]() {
+            if (elect_one()) tc_commit(ofull(i));
             __syncwarp();
         };
         // The rows of V behind the set's last key belong to others and may hold no numbers, which a
         // p of 0 would not cancel: those of the last 16 that the products read become 0.
-        auto clean = [&](int it, int keys) {
+        auto clean = [&](uint32_t st, int keys) {
             if (keys >= kKeys || (keys & 15) == 0) return;
-            uint8_t* v = smem + (G::kQTiles + it % G::kStages) * G::kTileBytes;
+            uint8_t* v = smem + (G::kQTiles + st) * G::kTileBytes;
             for (int c = lane; c < (16 - (keys & 15)) * 8 * G::kBoxes; c += 32) {
                 const int row = keys + c / (8 * G::kBoxes), x = c % (8 * G::kBoxes);
                 *reinterpret_cast<uint4*>(v + (x >> 3) * 16384 + row * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -245,57 +394,69 @@ k_attn_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUte
             fence_proxy_async_smem();
             __syncwarp();
         };
-        auto keys_of = [&](int blk) { return min(kKeys, j.nk - (j.blk0 + blk) * kKeys); };
+        int keys = j.nk - j.blk0 * kKeys;            // left from the block on
         wait(bq, 0);
         if (!ALT) {
-            if (ok && need(0)) {
-                if (j.n[0] > 0) mma_s(0, 0);
-                if (j.n[1] > 0) mma_s(1, 0);
-                free_stage(0);
+            const int n = j.n[i];                    // the other tile may have more blocks: their places pass
+            const uint32_t k0 = take();
+            if (my_turn(0)) {
+                if (n > 0) mma_s(k0);
+                pass();
+                release(k0);
             }
-            for (int b = 0; b < nmax && ok; ++b) {
-                const int iv = 2 * b + 1, ik = 2 * b + 2;
-                if (!need(iv)) break;
-                clean(iv, keys_of(b));
-                if (b + 1 < nmax && !need(ik)) break;
-                for (int i = 0; i < 2; ++i) {
-                    if (b >= j.n[i]) continue;
-                    if (!wait(pfull(i), (uint32_t)(b & 1))) break;
-                    mma_o(i, iv, b == 0, keys_of(b));
-                    if (b + 1 < j.n[i]) mma_s(i, ik);
-                    else {
-                        if (elect_one()) tc_commit(ofull(i));
-                        __syncwarp();
-                    }
+            for (int b = 0; b < nmax && ok; ++b, keys -= kKeys) {
+                const uint32_t v = take(), k = b + 1 < nmax ? take() : 0;
+                if (!ok) break;
+                if (b < n) {
+                    clean(v, keys);
+                    if (!mma_o(v, b, b == 0, keys, (uint32_t)(b & 1))) break;
+                    if (b + 1 < n) mma_s(k);
+                    else last();
+                } else if (!my_turn(b + 1)) {
+                    break;
                 }
-                free_stage(iv);
-                if (b + 1 < nmax) free_stage(ik);
+                pass();
+                release(v);
+                if (b + 1 < nmax) release(k);
             }
         } else {
+            // ring: K0 K1 V0 K2 V1 ...; this tile's blocks are i, i + 2, ...
             const int n = nmax;
-            if (ok && need(0)) {
-                mma_s(0, 0);
-                free_stage(0);
-            }
-            if (n > 1 && ok && need(1)) {
-                mma_s(1, 1);
-                free_stage(1);
-            }
-            for (int b = 0; b < n && ok; ++b) {
-                const int i = b & 1, iv = b == n - 1 ? 2 * n - 1 : 2 * b + 2, ik = 2 * b + 3;
-                if (!need(iv)) break;
-                clean(iv, keys_of(b));
-                if (!wait(pfull(i), (uint32_t)((b >> 1) & 1))) break;
-                mma_o(i, iv, b < 2, keys_of(b));
-                free_stage(iv);
-                if (b + 2 < n) {
-                    if (!need(ik)) break;
-                    mma_s(i, ik);
-                    free_stage(ik);
-                } else {
-                    if (elect_one()) tc_commit(ofull(i));
-                    __syncwarp();
+            auto skip = [&]() {
+                if (++stage == G::kStages) {
+                    stage = 0;
+                    round ^= 1;
                 }
+            };
+            if (i == 0) {
+                const uint32_t k = take();
+                if (ok) {
+                    mma_s(k);
+                    release(k);
+                }
+                if (n > 1) skip();
+            } else if (n > 1) {
+                skip();
+                const uint32_t k = take();
+                if (ok) {
+                    mma_s(k);
+                    release(k);
+                }
+            }
+            for (int b = 0; b < n && ok; ++b, keys -= kKeys) {
+                if ((b & 1) != i) {                  // the other tile's V and K
+                    skip();
+                    if (b + 2 < n) skip();
+                    continue;
+                }
+                const uint32_t v = take(), k = b + 2 < n ? take() : 0;
+                if (!ok) break;
+                clean(v, keys);
+                if (!mma_o(v, b, b < 2, keys, (uint32_t)((b >> 1) & 1))) break;
+                if (b + 2 < n) mma_s(k);
+                else last();
+                release(v);
+                if (b + 2 < n) release(k);
             }
         }
         // every MMA has completed before the TMEM is freed (also after an abort)
@@ -303,7 +464,9 @@ k_attn_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUte
         __syncwarp();
         const long long t0 = clock64();
         while (!mbar_try_wait(drain, 0) && clock64() - t0 < kWaitCycles) { }
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kRegsSoftmax));
         // ------------------------------------------------------------------ softmax and output
         const int i = warp >> 2, r = (warp & 3) * 32 + lane;
         const int t = j.t0 + (ALT ? 0 : i * p.tile_tokens) + r / a.group;
@@ -327,17 +490,20 @@ k_attn_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUte
 #pragma unroll
             for (int q = 0; q < 4; ++q) tmem_ld_x32(ts + q * 32, s + q * 32);
             tmem_wait_ld();
-            if (wlim < key0 + kKeys) {
+            const bool masked = wlim < key0 + kKeys;
+            if (masked) {
                 const int left = lim - key0;
 #pragma unroll
                 for (int q = 0; q < 128; ++q) s[q] = q < left ? s[q] : -INFINITY;
             }
             float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int q = 4; q < 128; q += 4) {
+            for (int q = 4; q < 124; q += 8) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[q + e]);
+                for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[q + e], s[q + 4 + e]);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[124 + e]);
             const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
             if (b == 0) {
                 m = mn;
@@ -356,25 +522,21 @@ k_attn_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUte
                 }
             }
             const float ref = lift - (m == -INFINITY ? 0.f : m * c);
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t w[32];
-#pragma unroll
-                for (int q = 0; q < 32; ++q) {
-                    const int e = half * 64 + 2 * q;
-                    const float x = ex2(fmaf(s[e], c, ref)), y = ex2(fmaf(s[e + 1], c, ref));
-                    sum[q & 1] += x;
-                    sum[2 + (q & 1)] += y;
-                    w[q] = pack2(x, y, T());
-                }
-                tmem_st_x32(ts + half * 32, w);
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            // p in quarters of 32 keys; the products start on the first kFirst keys
+            if (masked) exp_block<T, 0>(s, c, ref, ts, phalf(i), lane);
+            else exp_block<T, kPoly>(s, c, ref, ts, phalf(i), lane);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(pfull(i));
+            f2 sum[2] = {pack(s[0], s[1]), pack(s[2], s[3])};
+#pragma unroll
+            for (int q = 4; q < 128; q += 4) {
+                sum[0] = add2(sum[0], pack(s[q], s[q + 1]));
+                sum[1] = add2(sum[1], pack(s[q + 2], s[q + 3]));
+            }
+            const float2 both = unpack(add2(sum[0], sum[1]));
+            l += both.x + both.y;
         }
         if (n > 0 && ok) {
             ok = __all_sync(0xffffffffu, mbar_wait(ofull(i), 0, s_abort, a.err));
@@ -427,16 +589,12 @@ k_attn_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUte
         tc_fence_before();
     }
     __syncthreads();
-    if (warp == 9 && lane == 0) {
-        // TMA loads still in flight after an abort land before the CTA exits
-        for (int it = (int)s_misc[2]; it < issued; ++it) {
-            const long long t0 = clock64();
+    if (warp == 10 && lane == 0 && *s_abort) {
+        // after an abort, TMA loads still in flight land before the CTA exits
+        const long long t0 = clock64();
+        for (int it = max(0, issued - G::kStages); it < issued; ++it)
             while (!mbar_try_wait(full(it % G::kStages), (uint32_t)((it / G::kStages) & 1)) && clock64() - t0 < kWaitCycles) { }
-        }
-        if (nmax > 0) {
-            const long long t0 = clock64();
-            while (!mbar_try_wait(bq, 0) && clock64() - t0 < kWaitCycles) { }
-        }
+        while (nmax > 0 && !mbar_try_wait(bq, 0) && clock64() - t0 < kWaitCycles) { }
     }
     __syncthreads();
     if (warp == 8) {
