@@ -275,7 +275,7 @@ tb_status tb_layer_norm(tb_ctx* ctx, const void* x, tb_dtype x_dtype, int64_t n,
  * tb_group_norm: out = act((x - mean) / sqrt(var + eps) * w + b), mean and variance of each set over
  * its rows and each group's c / groups consecutive channels. x [n][c] of x_dtype, out [n][c] of
  * out_dtype (TB_F32 or x_dtype; may be x); c a multiple of 8 up to 2048; w, b float32 [c], each may be
- * NULL. Statistics in fp32 pieces joined in 64 bits in a fixed order. */
+ * NULL. Statistics in fp32, of pieces joined in a fixed order: results repeat to the bit. */
 typedef enum tb_rope_layout { TB_ROPE_PAIRS = 0, TB_ROPE_HALVES = 1 } tb_rope_layout;
 typedef enum tb_rope_freqs { TB_ROPE_FREQS_AXIS = 0, TB_ROPE_FREQS_JOINT = 1 } tb_rope_freqs;
 
@@ -317,7 +317,7 @@ typedef struct tb_rope_params {
 size_t tb_attention_workspace_bytes(const tb_ctx* ctx, const tb_attention_params* params);
 tb_status tb_attention(tb_ctx* ctx, const tb_attention_params* params);
 tb_status tb_rope(tb_ctx* ctx, const tb_rope_params* params);
-size_t tb_group_norm_workspace_bytes(const tb_ctx* ctx, int64_t n, int groups, int nset);
+size_t tb_group_norm_workspace_bytes(const tb_ctx* ctx, int64_t n, int c, int groups, int nset);
 tb_status tb_group_norm(tb_ctx* ctx, const void* x, tb_dtype x_dtype, const int32_t* offsets, int nset, int64_t n, int c,
                         int groups, const float* w, const float* b, float eps, tb_epilogue act, tb_dtype out_dtype,
                         void* out, void* workspace, size_t workspace_bytes);

@@ -106,7 +106,7 @@ int main() {
     ROPE((p.out = (void*)p.x, p.out_row = 512), TB_ERR_INVALID_ARG);
     ROPE(p.n = (int64_t)1 << 31, TB_ERR_TOO_LARGE);
 
-    const size_t need = tb_group_norm_workspace_bytes(&ctx, 100, 4, 1);
+    const size_t need = tb_group_norm_workspace_bytes(&ctx, 10000, 32, 4, 1);
     auto gn = [&](const void* x, tb_dtype dt, const int32_t* off, int nset, int64_t n, int c, int groups, float eps, int act,
                   tb_dtype od, void* out, void* ws, size_t wb) {
         return tb_group_norm(&ctx, x, dt, off, nset, n, c, groups, nullptr, nullptr, eps, (tb_epilogue)act, od, out, ws, wb);
@@ -129,8 +129,8 @@ int main() {
     want("gn null", gn(nullptr, TB_F32, off, 1, 100, 32, 4, 1e-5f, 0, TB_F32, out, mem, need), TB_ERR_INVALID_ARG);
     want("gn alignment", gn(mem + 4, TB_F32, off, 1, 100, 32, 4, 1e-5f, 0, TB_F32, out, mem, need), TB_ERR_INVALID_ARG);
     want("gn in place", gn(mem, TB_F16, off, 1, 100, 32, 4, 1e-5f, 0, TB_F32, mem, mem, need), TB_ERR_INVALID_ARG);
-    want("gn workspace", gn(mem, TB_F32, off, 1, 100, 32, 4, 1e-5f, 0, TB_F32, out, nullptr, 0), TB_ERR_INVALID_ARG);
-    want("gn small workspace", gn(mem, TB_F32, off, 1, 100, 32, 4, 1e-5f, 0, TB_F32, out, mem, need - 1), TB_ERR_INVALID_ARG);
+    want("gn workspace", gn(mem, TB_F32, off, 1, 10000, 32, 4, 1e-5f, 0, TB_F32, out, nullptr, 0), TB_ERR_INVALID_ARG);
+    want("gn small workspace", gn(mem, TB_F32, off, 1, 10000, 32, 4, 1e-5f, 0, TB_F32, out, mem, need - 1), TB_ERR_INVALID_ARG);
     std::printf(failed ? "failed\n" : "refusals ok\n");
     return failed;
 }

@@ -94,7 +94,7 @@ SIGNATURES = {
     "tb_attention_workspace_bytes": (ctypes.c_size_t, [_vp, ctypes.POINTER(AttentionParams)]),
     "tb_attention": (_st, [_vp, ctypes.POINTER(AttentionParams)]),
     "tb_rope": (_st, [_vp, ctypes.POINTER(RopeParams)]),
-    "tb_group_norm_workspace_bytes": (ctypes.c_size_t, [_vp, _i64, _int, _int]),
+    "tb_group_norm_workspace_bytes": (ctypes.c_size_t, [_vp, _i64, _int, _int, _int]),
     "tb_group_norm": (_st, [_vp, _vp, _int, _vp, _int, _i64, _int, _int, _vp, _vp, ctypes.c_float, _int, _int, _vp, _vp,
                             ctypes.c_size_t]),
     "tb_gguf_open": (_st, [ctypes.c_char_p, ctypes.POINTER(_vp)]),

@@ -70,11 +70,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 // columns) contiguous; V is the B operand with N (the head's columns) contiguous, its boxes of 64
 // columns 16384 bytes apart.
 __device__ __forceinline__ uint64_t desc64(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, float* v) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
                  "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -90,33 +85,6 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, float* v) {
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-    return y;
-}
-// ---- two 32-bit values in one instruction ---------------------------------------------------------
-typedef unsigned long long f2;
-__device__ __forceinline__ f2 pack(float a, float b) {
-    f2 y;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
-    return y;
-}
-__device__ __forceinline__ float2 unpack(f2 x) {
-    float2 y;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
-    return y;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-    f2 y;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
-    return y;
-}
-__device__ __forceinline__ f2 add2(f2 a, f2 b) {
-    f2 y;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
-    return y;
-}
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-    f2 y;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
     return y;
 }
 // 2^x of two values on the FMA pipes, beside the exponential unit: x = i + f with i the nearest whole

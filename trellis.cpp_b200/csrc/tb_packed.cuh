@@ -77,6 +77,56 @@ __device__ __forceinline__ void find_item(const int32_t* off, int nset, int64_t 
     __syncthreads();
 }
 
+// ---- two 32-bit values in one instruction ----------------------------------------------------------
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack(float a, float b) {
+    f2 y;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float2 unpack(f2 x) {
+    float2 y;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
+    return y;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+    return y;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 y;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+__device__ __forceinline__ f2 sub2(f2 a, f2 b) {
+    f2 y;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 y;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+// 2^x, about 2 steps off; 0 far below, inf far above
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// v / (1 + e^-v) of two values. Far below zero the sum is inf, its reciprocal 0.
+__device__ __forceinline__ f2 silu2(f2 v) {
+    const float2 e = unpack(mul2(v, pack(-1.44269504088896340736f, -1.44269504088896340736f)));
+    const float2 d = unpack(add2(pack(ex2(e.x), ex2(e.y)), pack(1.f, 1.f)));
+    return mul2(v, pack(rcp(d.x), rcp(d.y)));
+}
+
 // ---- 8 consecutive elements of a 16-byte aligned row as float ------------------------------------
 template <class T> __device__ __forceinline__ void load8(const T* p, float* v);
 template <> __device__ __forceinline__ void load8<float>(const float* p, float* v) {

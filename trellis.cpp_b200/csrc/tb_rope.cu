@@ -11,6 +11,7 @@
 // all heads it turns. Bound by memory: each value is read and written once.
 #include "tb_packed.cuh"
 
+#include <algorithm>
 #include <cmath>
 
 namespace {
@@ -31,64 +32,101 @@ struct RopeArgs {
     uint8_t axis[kRopeMaxPairs];
 };
 
-// P pairs of one head. PAIRS: elements 2p, 2p+1; otherwise p and p + half.
-template <class T, int P, bool PAIRS>
-__device__ __forceinline__ void rope_load(const T* h, int p0, int half, float* a, float* b) {
-    if (PAIRS) {
-        float v[2 * P];
+// P pairs of one head as they lie in memory: elements 2p, 2p+1 (PAIRS), otherwise p and p + half. Words
+// of 16 bytes, of 8 where a half of a head is no multiple of them; streamed past the caches' end.
+template <class T, int P, bool PAIRS> struct Pairs {
+    static constexpr int kBytes = PAIRS ? 2 * P * (int)sizeof(T) : P * (int)sizeof(T);   // of each run
+    static constexpr int kRuns = PAIRS ? 1 : 2;
+    using W = typename std::conditional<kBytes % 16 == 0, uint4, uint2>::type;
+    static constexpr int kWords = kBytes / (int)sizeof(W);
+    W w[kRuns * kWords];
+    __device__ __forceinline__ void load(const T* h, int p0, int half) {
 #pragma unroll
-        for (int i = 0; i < 2 * P; i += 8) load8<T>(h + 2 * p0 + i, v + i);
+        for (int r = 0; r < kRuns; ++r)
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            a[i] = v[2 * i];
-            b[i] = v[2 * i + 1];
-        }
-    } else if (P == 8) {
-        load8<T>(h + p0, a);
-        load8<T>(h + half + p0, b);
-    } else if (sizeof(T) == 4) {
-        const float4 u = *reinterpret_cast<const float4*>(h + p0), v = *reinterpret_cast<const float4*>(h + half + p0);
-        a[0] = u.x; a[1] = u.y; a[2] = u.z; a[3] = u.w;
-        b[0] = v.x; b[1] = v.y; b[2] = v.z; b[3] = v.w;
-    } else {
-        const uint2 u = *reinterpret_cast<const uint2*>(h + p0), v = *reinterpret_cast<const uint2*>(h + half + p0);
-        using H = typename std::conditional<sizeof(T) == 4, __half, T>::type;
-        unpack2(u.x, a, H()); unpack2(u.y, a + 2, H());
-        unpack2(v.x, b, H()); unpack2(v.y, b + 2, H());
+            for (int i = 0; i < kWords; ++i)
+                w[r * kWords + i] = __ldcs(reinterpret_cast<const W*>(h + (PAIRS ? 2 * p0 : r * half + p0)) + i);
     }
-}
+    __device__ __forceinline__ void store(T* h, int p0, int half) const {
+#pragma unroll
+        for (int r = 0; r < kRuns; ++r)
+#pragma unroll
+            for (int i = 0; i < kWords; ++i)
+                __stcs(reinterpret_cast<W*>(h + (PAIRS ? 2 * p0 : r * half + p0)) + i, w[r * kWords + i]);
+    }
+    // turns the pairs by c, s
+    __device__ __forceinline__ void turn(const float* c, const float* s) {
+        uint32_t* u = reinterpret_cast<uint32_t*>(w);
+        constexpr int per = 4 / (int)sizeof(T);                   // elements of a 32-bit word
+#pragma unroll
+        for (int i = 0; i < P; i += (PAIRS ? 1 : per)) {
+            float a[per], b[per];
+            if (PAIRS) {
+                get(u, 2 * i, a, b);
+            } else {
+#pragma unroll
+                for (int e = 0; e < per; ++e) {
+                    a[e] = value(u, i + e);
+                    b[e] = value(u, P + i + e);
+                }
+            }
+            if (PAIRS) {
+                put(u, 2 * i, a[0] * c[i] - b[0] * s[i], a[0] * s[i] + b[0] * c[i]);
+            } else {
+                float x[2], y[2];
+#pragma unroll
+                for (int e = 0; e < per; ++e) {
+                    x[e] = a[e] * c[i + e] - b[e] * s[i + e];
+                    y[e] = a[e] * s[i + e] + b[e] * c[i + e];
+                }
+                if (per == 2) {
+                    put(u, i, x[0], x[1]);
+                    put(u, P + i, y[0], y[1]);
+                } else {
+                    u[i] = __float_as_uint(x[0]);
+                    u[P + i] = __float_as_uint(y[0]);
+                }
+            }
+        }
+    }
 
-template <class T, int P, bool PAIRS>
-__device__ __forceinline__ void rope_store(T* h, int p0, int half, const float* a, const float* b) {
-    if (PAIRS) {
-        float v[2 * P];
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            v[2 * i] = a[i];
-            v[2 * i + 1] = b[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 2 * P; i += 8) store8<T>(h + 2 * p0 + i, v + i);
-    } else if (P == 8) {
-        store8<T>(h + p0, a);
-        store8<T>(h + half + p0, b);
-    } else if (sizeof(T) == 4) {
-        *reinterpret_cast<float4*>(h + p0) = make_float4(a[0], a[1], a[2], a[3]);
-        *reinterpret_cast<float4*>(h + half + p0) = make_float4(b[0], b[1], b[2], b[3]);
-    } else {
-        using H = typename std::conditional<sizeof(T) == 4, __half, T>::type;
-        *reinterpret_cast<uint2*>(h + p0) = make_uint2(pack2(a[0], a[1], H()), pack2(a[2], a[3], H()));
-        *reinterpret_cast<uint2*>(h + half + p0) = make_uint2(pack2(b[0], b[1], H()), pack2(b[2], b[3], H()));
+private:
+    using H = typename std::conditional<sizeof(T) == 4, __half, T>::type;
+    static __device__ __forceinline__ float value(const uint32_t* u, int i) {
+        if (sizeof(T) == 4) return __uint_as_float(u[i]);
+        float v[2];
+        unpack2(u[i / 2], v, H());
+        return v[i % 2];
     }
-}
+    // elements i (even) and i + 1
+    static __device__ __forceinline__ void get(const uint32_t* u, int i, float* a, float* b) {
+        a[0] = value(u, i);
+        b[0] = value(u, i + 1);
+    }
+    static __device__ __forceinline__ void put(uint32_t* u, int i, float x, float y) {
+        if (sizeof(T) == 4) {
+            u[i] = __float_as_uint(x);
+            u[i + 1] = __float_as_uint(y);
+        } else {
+            u[i / 2] = pack2(x, y, H());
+        }
+    }
+};
 
 template <class T, int P, bool PAIRS>
 __global__ void __launch_bounds__(kRopeThreads) k_rope(const __grid_constant__ RopeArgs r) {
+    constexpr int kBatch = 4;                       // heads whose loads go before the first store
     const int64_t t = (int64_t)blockIdx.x * kRopeThreads + threadIdx.x;
     const int64_t row = t / r.chunks;
     if (row >= r.n) return;
     const int p0 = (int)(t - row * r.chunks) * P;
     const int h0 = blockIdx.y * r.heads_per, h1 = min(r.heads, h0 + r.heads_per);
+    const T* x = reinterpret_cast<const T*>(r.x) + row * r.x_row + h0 * r.x_head;
+    T* o = reinterpret_cast<T*>(r.out) + row * r.out_row + h0 * r.out_head;
+    Pairs<T, P, PAIRS> v[kBatch];
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q)
+        if (h0 + q < h1) v[q].load(x + q * r.x_head, p0, r.half);
     float c[P], s[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
@@ -96,18 +134,18 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope(const __grid_constant__ R
         sincospif(2.f * (float)(turns - rint(turns)), s + i, c + i);
         s[i] *= r.sign;
     }
-    const T* x = reinterpret_cast<const T*>(r.x) + row * r.x_row + h0 * r.x_head;
-    T* o = reinterpret_cast<T*>(r.out) + row * r.out_row + h0 * r.out_head;
-#pragma unroll 4
-    for (int h = h0; h < h1; ++h, x += r.x_head, o += r.out_head) {
-        float a[P], b[P], ya[P], yb[P];
-        rope_load<T, P, PAIRS>(x, p0, r.half, a, b);
+    for (int h = h0; h < h1; h += kBatch) {
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            ya[i] = a[i] * c[i] - b[i] * s[i];
-            yb[i] = a[i] * s[i] + b[i] * c[i];
-        }
-        rope_store<T, P, PAIRS>(o, p0, r.half, ya, yb);
+        for (int q = 0; q < kBatch; ++q)
+            if (h + q < h1) {
+                v[q].turn(c, s);
+                v[q].store(o + q * r.out_head, p0, r.half);
+            }
+        x += kBatch * r.x_head;
+        o += kBatch * r.out_head;
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q)
+            if (h + kBatch + q < h1) v[q].load(x + q * r.x_head, p0, r.half);
     }
 }
 
@@ -184,7 +222,10 @@ extern "C" tb_status tb_rope(tb_ctx* ctx, const tb_rope_params* p) {
     const int per = !pairs && p->dtype != TB_F32 && half % 8 == 0 ? 8 : 4;
     r.chunks = half / per;
     const int64_t blocks = (p->n * r.chunks + kRopeThreads - 1) / kRopeThreads;
-    r.heads_per = p->heads;
+    // A thread turns as many heads as leave four blocks an SM: its sines serve them all, but 600 rows of
+    // 64 on one block each 24 heads leave most SMs idle (10 us against 3 with the heads spread).
+    const int64_t split = std::max<int64_t>(1, std::min<int64_t>(p->heads, 4ll * ctx->num_sms / blocks));
+    r.heads_per = (int)((p->heads + split - 1) / split);
     tb_device_guard guard;
     TB_CUDA_TRY(ctx, guard.enter(ctx->device));
     const dim3 grid((unsigned)blocks, (unsigned)((p->heads + r.heads_per - 1) / r.heads_per));

@@ -32,6 +32,16 @@ from ._lib import TBError, check  # noqa: F401
 _DT = {torch.float32: _lib.TB_F32, torch.float16: _lib.TB_F16, torch.bfloat16: _lib.TB_BF16}
 _EPI = {"none": _lib.TB_EPI_NONE, None: _lib.TB_EPI_NONE, "silu": _lib.TB_EPI_SILU}
 _ctxs: dict = {}
+_streams: dict = {}      # the stream each context is bound to
+
+
+def _raw_stream(index: int) -> int:
+    """torch's current stream on a device, as a cudaStream_t."""
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):       # the same without a Stream object, 2 us less a call
+    _raw_stream = torch._C._cuda_getCurrentRawStream     # noqa: F811
 
 # Kernels one tb_build_neighbor_map call launches: the order and range check, then five that
 # branch on the layout decided on the device (sorted, block or voxel hash); with the sorted
@@ -47,17 +57,22 @@ def context(device=None):
     """The per-device tb_ctx, bound to torch's current stream on that device (the current device
     when `device` is None or names no index). One context per device is shared by every caller
     in the process; like the C contexts it wraps, it is not safe to use from two threads at once."""
-    idx = None if device is None else torch.device(device).index
-    dev = torch.device("cuda", torch.cuda.current_device() if idx is None else idx)
+    idx = device
+    if type(idx) is not int:
+        idx = None if device is None else torch.device(device).index
+        if idx is None:
+            idx = torch.cuda.current_device()
     lib = _lib.load()
-    h = _ctxs.get(dev.index)
-    stream = torch.cuda.current_stream(dev).cuda_stream
+    h = _ctxs.get(idx)
+    stream = _raw_stream(idx)
     if h is None:
         h = ctypes.c_void_p()
-        check(lib.tb_ctx_create(dev.index, ctypes.c_void_p(stream), ctypes.byref(h)), "tb_ctx_create")
-        _ctxs[dev.index] = h
-    else:
+        check(lib.tb_ctx_create(idx, ctypes.c_void_p(stream), ctypes.byref(h)), "tb_ctx_create")
+        _ctxs[idx] = h
+        _streams[idx] = stream
+    elif _streams[idx] != stream:
         check(lib.tb_ctx_set_stream(h, ctypes.c_void_p(stream)), "tb_ctx_set_stream", h)
+        _streams[idx] = stream
     return h
 
 
@@ -277,20 +292,26 @@ _FREQS = {"axis": _lib.TB_ROPE_FREQS_AXIS, "joint": _lib.TB_ROPE_FREQS_JOINT}
 
 
 def _need_heads(t: torch.Tensor, name: str):
-    if not t.is_cuda or t.dim() != 3 or t.dtype not in _DT or (t.shape[2] > 1 and t.stride(2) != 1):
+    if not t.is_cuda or t.dim() != 3 or t.dtype not in _DT or (t.stride(2) != 1 and t.shape[2] > 1):
         raise ValueError(f"{name} must be a CUDA tensor [N, heads, head_dim] of float32/float16/bfloat16 with "
                          "contiguous heads")
 
 
-def _same_device(first: torch.Tensor, *ts):
+def _same_device(index: int, *ts):
     for t in ts:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
             raise ValueError("all tensors must be on one device")
 
 
 def _offsets(t, name: str):
     if not t.is_cuda or t.dtype != torch.int32 or t.dim() != 1 or t.numel() < 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 CUDA tensor [sets + 1]")
+
+
+def _out_code(dtype) -> int:
+    if dtype not in _DT:
+        raise ValueError("out_dtype must be float32/float16/bfloat16")
+    return _DT[dtype]
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor | None = None,
@@ -308,7 +329,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torc
     _need_heads(q, "q")
     _need_heads(k, "k")
     _need_heads(v, "v")
-    _same_device(q, k, v, q_offsets, k_offsets, out)
+    dev = q.get_device()
+    _same_device(dev, k, v, q_offsets, k_offsets, out)
     nq, h, d = q.shape
     nk, hk, _ = k.shape
     if k.dtype != q.dtype or v.dtype != q.dtype or v.shape != k.shape or k.shape[2] != d:
@@ -327,23 +349,23 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torc
         if k_offsets.numel() != nset + 1:
             raise ValueError("q_offsets and k_offsets must have the same number of sets")
     if out is None:
-        out = torch.empty((nq, h, d), dtype=q.dtype if out_dtype is None else out_dtype, device=q.device)
+        out = q.new_empty((nq, h, d), dtype=out_dtype)
     else:
         _need_heads(out, "out")
         if tuple(out.shape) != (nq, h, d) or (out_dtype is not None and out.dtype != out_dtype):
             raise ValueError("out must be [Nq, H, D] of out_dtype")
-    lse = torch.empty((nq, h), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = q.new_empty((nq, h), dtype=torch.float32) if return_lse else None
     qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
     p = _lib.AttentionParams(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
         None if q_offsets is None else q_offsets.data_ptr(), None if k_offsets is None else k_offsets.data_ptr(),
         nq, nk, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1], nset, h, hk, d,
-        d ** -0.5 if scale is None else scale, 1 if causal else 0, _DT[q.dtype], _DT[out.dtype], None, 0)
-    ctx = context(q.device)
+        d ** -0.5 if scale is None else scale, 1 if causal else 0, _DT[q.dtype], _out_code(out.dtype), None, 0)
+    ctx = context(dev)
     lib = _lib.load()
     need = lib.tb_attention_workspace_bytes(ctx, p)
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = q.new_empty(need, dtype=torch.uint8)
         p.workspace, p.workspace_bytes = ws.data_ptr(), need
     st = lib.tb_attention(ctx, p)
     if st:
@@ -370,9 +392,10 @@ def rope(x: torch.Tensor, coords: torch.Tensor, sections, theta: float = 10000.0
         raise ValueError("coords must be a contiguous int32 CUDA tensor [N, axes] or [N, axes + 1]")
     if layout not in _LAYOUT or freqs not in _FREQS:
         raise ValueError('layout must be "pairs" or "halves", freqs "axis" or "joint"')
-    _same_device(x, coords, out)
+    dev = x.get_device()
+    _same_device(dev, coords, out)
     if out is None:
-        out = torch.empty((n, h, d), dtype=x.dtype, device=x.device)
+        out = x.new_empty((n, h, d))
     else:
         _need_heads(out, "out")
         if out.shape != x.shape or out.dtype != x.dtype:
@@ -381,7 +404,7 @@ def rope(x: torch.Tensor, coords: torch.Tensor, sections, theta: float = 10000.0
     p = _lib.RopeParams(x.data_ptr(), out.data_ptr(), coords.data_ptr(), n, xs[0], xs[1], os_[0], os_[1], coords.shape[1],
                         axes, tuple(sections), h, d, theta, _LAYOUT[layout], _FREQS[freqs], 1 if inverse else 0,
                         _DT[x.dtype])
-    ctx = context(x.device)
+    ctx = context(dev)
     st = _lib.load().tb_rope(ctx, p)
     if st:
         check(st, "tb_rope", ctx)
@@ -405,20 +428,22 @@ def group_norm(x: torch.Tensor, groups: int, w=None, b=None, offsets: torch.Tens
     if offsets is not None:
         _offsets(offsets, "offsets")
         nset = offsets.numel() - 1
-    _same_device(x, w, b, offsets, out)
+    dev = x.get_device()
+    _same_device(dev, w, b, offsets, out)
     if out is None:
-        out = torch.empty((n, c), dtype=x.dtype if out_dtype is None else out_dtype, device=x.device)
+        out = x.new_empty((n, c), dtype=out_dtype)
     else:
         _need_cuda(out)
-        if out.shape != x.shape or out.dtype not in _DT or (out_dtype is not None and out.dtype != out_dtype):
+        if out.shape != x.shape or (out_dtype is not None and out.dtype != out_dtype):
             raise ValueError("out must be [N, C] of out_dtype")
-    ctx = context(x.device)
+    code = _out_code(out.dtype)
+    ctx = context(dev)
     lib = _lib.load()
-    need = lib.tb_group_norm_workspace_bytes(ctx, n, groups, nset)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    need = lib.tb_group_norm_workspace_bytes(ctx, n, c, groups, nset)
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
     st = lib.tb_group_norm(ctx, x.data_ptr(), _DT[x.dtype], None if offsets is None else offsets.data_ptr(), nset, n, c,
                            groups, None if w is None else w.data_ptr(), None if b is None else b.data_ptr(), eps,
-                           _EPI[act], _DT[out.dtype], out.data_ptr(), None if ws is None else ws.data_ptr(), need)
+                           _EPI[act], code, out.data_ptr(), None if ws is None else ws.data_ptr(), need)
     if st:
         check(st, "tb_group_norm", ctx)
     return out
