@@ -217,8 +217,9 @@ tb_status attn_args(tb_ctx* ctx, const tb_attention_params* p, AttnArgs& a) {
         return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_attention: give both offset tables, or neither with nset 1");
     if (!(p->scale > 0.f) || !std::isfinite(p->scale))
         return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_attention: scale must be positive and finite");
-    if (p->nq >= (int64_t)INT32_MAX || p->nk >= (int64_t)INT32_MAX || p->nset > 65536 || p->heads > 65536)
-        return tb_fail(ctx, TB_ERR_TOO_LARGE, "tb_attention: rows must be < 2^31-1, sets and heads at most 65536");
+    // a tile past the last row still has a 32-bit row number
+    if (p->nq > (int64_t)INT32_MAX - 1024 || p->nk > (int64_t)INT32_MAX - 1024 || p->nset > 65536 || p->heads > 65536)
+        return tb_fail(ctx, TB_ERR_TOO_LARGE, "tb_attention: rows must be <= 2^31-1025, sets and heads at most 65536");
     const int64_t unit = 16 / (int64_t)tb_dtype_size(p->dtype), ounit = 16 / (int64_t)tb_dtype_size(p->out_dtype);
     if (bad_stride(p->nq, p->q_row, unit) || bad_stride(p->heads, p->q_head, unit) || bad_stride(p->nk, p->k_row, unit) ||
         bad_stride(p->kv_heads, p->k_head, unit) || bad_stride(p->nk, p->v_row, unit) ||

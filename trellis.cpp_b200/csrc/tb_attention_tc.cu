@@ -1,21 +1,26 @@
 // Attention within packed sets on tcgen05 (bf16 / f16 operands); the mathematics and the entry point
 // are in tb_attention.cu.
 //
-// One CTA takes 256 query rows of one key head as two tiles of 128 (a row is a token and one of the
-// heads that share the key head, so the keys of a group are read once) and walks the keys in
-// blocks of 128: S = Q K^T into 128 TMEM columns a tile, softmax by one warpgroup a tile (a thread
-// owns a row: no exchange between threads), P over S's columns as the A operand of O += P V, which
-// stays in TMEM. While one tile's warpgroup computes its softmax the tensor pipe works on the other
-// tile. One warp streams Q, K and V by TMA, one a tile issues the MMAs.
+// A CTA takes 128 query rows of one key head (a row is a token and one of the heads that share the key
+// head, so a group reads its keys once) and walks the keys in blocks of 128: S = Q K^T into one of
+// three 128-column TMEM buffers, softmax by a thread a row (no exchange), P over its S as the A operand
+// of O += P V, which stays in TMEM. Two softmax warpgroups take every other block; with three buffers
+// one block's S is ready and another's P V in work while they compute, so neither they nor the tensor
+// pipe wait for the other's latencies. (Two tiles of rows a CTA with one buffer each, the other way
+// to overlap them, left a chain S - softmax - P V of 3450 cycles for work of 2050 a pair of blocks.)
 //
-// The running maximum moves only when a block's exceeds it by more than 2^8 (in units of p): until
-// then p grows to at most 2^8, which the 32-bit sums hold as well, and O need not be scaled; the
-// result is the same since the sum carries the same factor. A block's S is committed after the
-// tile's last P V, so O is at rest while the softmax warps scale it.
+// Heads of more than 64 columns (PAIR): two CTAs of a cluster share each product as M = 256: each holds
+// its own rows' Q, S, P and O, one half of each block's keys for S and one half of the head's columns
+// of V for P V. Per CTA that halves the keys' way from L2 and the shared-memory reads, which a lone
+// CTA's products would saturate.
 //
-// With few query rows a set (ALT) one tile holds them and the two halves of the CTA take every
-// other block of keys; with few CTAs the keys are also cut into `nsplit` ranges. Both leave partial
-// rows (32 bits, normalised, with their log sums) that k_attn_join adds up in a fixed order.
+// The rows' reference (the running maximum, as a whole power of two) moves only when a block's maximum
+// exceeds it by more than 2^8: until then p grows to at most 2^8, which the 32-bit sums hold as well.
+// The warpgroups hand it on from block to block through shared memory; the one that raises it waits
+// until the block before has been added and scales O.
+//
+// With few CTAs the keys are cut into `nsplit` ranges, which leave partial rows (32 bits, normalised,
+// with their log sums) that k_attn_join adds up in a fixed order.
 #include "tb_packed.cuh"
 #include "tb_tc_ptx.cuh"
 
@@ -28,18 +33,16 @@ namespace {
 using namespace tbtc;
 using namespace tbpk;
 
-constexpr int kThreads = 384;          // warps 0-3 and 4-7 softmax, 8 and 9 MMA, 10 TMA, 11 idle
+constexpr int kThreads = 384;          // warps 0-3 and 4-7 softmax, 8 S, 9 P V, 10 TMA, 11 idle
 // Registers: 65536 / 384 threads allows 168 at launch; the third warpgroup gives up what the two
 // softmax warpgroups need to hold a row of S. 2 * 208 + 88 = 3 * 168.
 constexpr int kRegsSoftmax = 208, kRegsOther = 88;
 constexpr int kKeys = 128;             // keys of a block
-constexpr float kRaise = 8.f;          // the maximum follows when a block's is 2^8 above it
-#ifndef TB_FIRST
-#define TB_FIRST 96
-#endif
-constexpr int kFirst = TB_FIRST;             // keys of a block whose p the products may read early
+constexpr int kBufs = 3;               // S buffers
+constexpr float kRaise = 8.f;          // the reference follows when a block's maximum is 2^8 above it
+constexpr float kFar = 2097152.f;      // 2^21: references that ex2_poly can add 1.5 * 2^23 to
 #ifndef TB_POLY
-#define TB_POLY 3
+#define TB_POLY 2
 #endif
 constexpr int kPoly = TB_POLY;         // of every 8 pairs of exponentials, those by polynomial
 
@@ -48,16 +51,16 @@ struct TcArgs {
     float* part;                       // [nsp][nq][heads][dim] partial rows, null without splits
     float* part_lse;                   // [nsp][nq][heads], base 2
     int nsplit, tile_tokens;           // key ranges; tokens of a 128-row tile
-    uint32_t idesc_s, idesc_o, q_bytes;
+    uint32_t idesc_s, idesc_o, q_bytes;   // q_bytes: what one tile's boxes deliver
 };
 
-template <int D, bool ALT> struct Geom {
+template <int D, bool PAIR> struct Geom {
     static constexpr int kBoxes = D / 64;
-    static constexpr int kTileBytes = kBoxes * 16384;         // 128 rows x D, boxes of 64 columns
-    static constexpr int kQTiles = ALT ? 1 : 2;
-    static constexpr int kStages = D == 64 ? 10 : (ALT ? 6 : 5);
-    static constexpr int kBars = 2 * kStages + 1 + 2 + 2 + 2 + 2 + 2 + 1;
-    static constexpr size_t kSmem = (size_t)(kQTiles + kStages) * kTileBytes + 8 * kBars + 16 + 1024;
+    static constexpr int kQBytes = kBoxes * 16384;                // 128 rows x D, boxes of 64 columns
+    static constexpr int kBytes = kBoxes * 16384 / (PAIR ? 2 : 1);   // a CTA's share of a block's K, of its V
+    static constexpr int kStages = (196608 / 2) / kBytes;         // of K, and of V
+    static constexpr int kBars = 4 * kStages + 1 + 3 * kBufs + 1 + 8 + 4 + 1;
+    static constexpr size_t kSmem = (size_t)kQBytes + 2 * kStages * kBytes + 512 + 8 * kBars + 16 + 1024;
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -82,421 +85,379 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, float* v) {
                  : "r"(taddr));
 }
 
+// The maximum that keeps a value that is no number: it then makes its whole row none.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
-// 2^x of two values on the FMA pipes, beside the exponential unit: x = i + f with i the nearest whole
-// number, 2^f by the cubic of least relative error on [-1/2, 1/2] (exchange method, 7.5e-5: an
-// eighth of a half step of f16), times 2^i put together from its bits. x is taken at -126 at
-// least; a value that is no number stays one (the product keeps it).
-__device__ __forceinline__ float2 ex2_poly(f2 x) {
-    float2 v = unpack(x);
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-126.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-126.f));
-    x = pack(v.x, v.y);
-    const f2 r = add2(x, pack(12582912.f, 12582912.f));                     // 1.5 * 2^23: whole numbers
-    const f2 f = fma2(add2(r, pack(-12582912.f, -12582912.f)), pack(-1.f, -1.f), x);
+__device__ __forceinline__ float max2(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+// 2^(s c + ref) of two scores on the FMA pipes, beside the exponential unit. ref is a whole number,
+// so one fused product with ref + 1.5 * 2^23 (`lifted`) rounds the exponent to the nearest whole i in
+// its low bits, a second leaves the rest f = s c - (i - ref) without another rounding; 2^f by the
+// cubic of least relative error on [-1/2, 1/2] (exchange method, 7.5e-5: an eighth of a half step of
+// f16), and i is added to its exponent bits. Scores are taken at `least` (2^-120) at least.
+__device__ __forceinline__ float2 ex2_poly(float s0, float s1, float least, f2 c, f2 lifted) {
+    const f2 s = pack(max2(s0, least), max2(s1, least));
+    const f2 r = fma2(s, c, lifted);
+    const f2 f = fma2(s, c, sub2(lifted, r));
     f2 y = fma2(pack(0.0551716685f, 0.0551716685f), f, pack(0.242611125f, 0.242611125f));
     y = fma2(y, f, pack(0.693260968f, 0.693260968f));
     y = fma2(y, f, pack(0.999928057f, 0.999928057f));
-    const float2 i = unpack(r);
-    const float e0 = __uint_as_float((__float_as_uint(i.x) << 23) + 0x3f800000u);
-    const float e1 = __uint_as_float((__float_as_uint(i.y) << 23) + 0x3f800000u);
-    return unpack(mul2(y, pack(e0, e1)));
+    const float2 i = unpack(r), v = unpack(y);
+    return make_float2(__int_as_float(__float_as_int(v.x) + (__float_as_int(i.x) << 23)),
+                       __int_as_float(__float_as_int(v.y) + (__float_as_int(i.y) << 23)));
 }
 
 // p = 2^(s c + ref) of a row's 128 scores, left in s and, rounded to T, in the TMEM columns from `ts`.
 // NPOLY of every 8 pairs go by polynomial, which shares the work between the exponential unit (4
-// lanes a cycle and scheduler: 1024 cycles a block and warp, as long as the tile's products) and the
-// FMA pipes. A hidden score (-inf) has to give exactly 0: masked blocks use NPOLY 0.
+// lanes a cycle and scheduler: 1024 cycles a block, as long as its products) and the FMA pipes. A
+// hidden score (-inf) has to give exactly 0: masked blocks use NPOLY 0.
 template <class T, int NPOLY>
-__device__ __forceinline__ void exp_block(float* s, float c, float ref, uint32_t ts, uint32_t half_bar, int lane) {
-    const f2 c2 = pack(c, c), ref2 = pack(ref, ref);
+__device__ __forceinline__ void exp_block(float* s, float c, float ref, uint32_t ts) {
+    const f2 c2 = pack(c, c), ref2 = pack(ref, ref), lifted = add2(ref2, pack(12582912.f, 12582912.f));
+    const float least = NPOLY ? __fdividef(-120.f - ref, c) : 0.f;
 #pragma unroll
     for (int quarter = 0; quarter < 4; ++quarter) {
         float* v = s + quarter * 32;
-#pragma unroll
-        for (int q = 0; q < 32; q += 2) {
-            const float2 x = unpack(fma2(pack(v[q], v[q + 1]), c2, ref2));
-            v[q] = x.x;
-            v[q + 1] = x.y;
-        }
-#pragma unroll
-        for (int q = 0; q < 16; ++q)
-            if ((q & 7) * NPOLY / 8 == ((q & 7) + 1) * NPOLY / 8) {
-                v[2 * q] = ex2(v[2 * q]);
-                v[2 * q + 1] = ex2(v[2 * q + 1]);
-            }
-#pragma unroll
-        for (int q = 0; q < 16; ++q)
-            if ((q & 7) * NPOLY / 8 != ((q & 7) + 1) * NPOLY / 8) {
-                const float2 y = ex2_poly(pack(v[2 * q], v[2 * q + 1]));
-                v[2 * q] = y.x;
-                v[2 * q + 1] = y.y;
-            }
         uint32_t w[16];
 #pragma unroll
-        for (int q = 0; q < 16; ++q) w[q] = pack2(v[2 * q], v[2 * q + 1], T());
-        tmem_st_x16(ts + quarter * 16, w);
-        if (quarter == kFirst / 32 - 1) {
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(half_bar);
+        for (int q = 0; q < 16; ++q) {
+            float2 y;
+            if ((q & 7) * NPOLY / 8 != ((q & 7) + 1) * NPOLY / 8) {
+                y = ex2_poly(v[2 * q], v[2 * q + 1], least, c2, lifted);
+            } else {
+                y = unpack(fma2(pack(v[2 * q], v[2 * q + 1]), c2, ref2));
+                y.x = ex2(y.x);
+                y.y = ex2(y.y);
+            }
+            v[2 * q] = y.x;
+            v[2 * q + 1] = y.y;
+            w[q] = pack2(y.x, y.y, T());
         }
+        tmem_st_x16(ts + quarter * 16, w);
     }
 }
 
-// What one CTA works on, in shared memory.
-struct Job {
-    int64_t q0, k0;        // first query row and key row of the set
-    int nq, nk;            // rows of the set
-    int t0;                // first token of the CTA, in the set
-    int blk0;              // first key block
-    int n[2];              // key blocks of each tile (ALT: of the CTA, n[0])
+// Hand-offs inside a CTA, or across the pair: those order tcgen05 operations only (see tb_tc_ptx.cuh).
+template <bool PAIR> __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t par, volatile int* ab, int* err) {
+    return PAIR ? mbar_wait_cluster_relaxed(bar, par, ab, err) : mbar_wait(bar, par, ab, err);
+}
+template <bool PAIR> __device__ __forceinline__ void commit(uint32_t bar) {
+    if (PAIR) tc_commit_pair(bar, 0x3);
+    else tc_commit(bar);
+}
+
+// A place in a ring of N and the parity of its round.
+template <int N> struct Ring {
+    uint32_t at = 0, round = 0;
+    __device__ __forceinline__ void step() {
+        if (++at == N) {
+            at = 0;
+            round ^= 1;
+        }
+    }
 };
 
-template <class T, class O, int D, bool ALT>
-__global__ void __launch_bounds__(kThreads, 1)
-k_attn_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-          const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TcArgs p) {
-    using G = Geom<D, ALT>;
+template <class T, class O, int D, bool PAIR>
+__device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                                        const TcArgs& p) {
+    using G = Geom<D, PAIR>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Item it_s;
     __shared__ uint32_t scan[32];
     uint8_t* smem = smem_align1024(smem_raw);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (G::kQTiles + G::kStages) * G::kTileBytes);
-    uint32_t* s_misc = reinterpret_cast<uint32_t*>(bars + G::kBars);       // [0] tmem, [1] abort
+    uint8_t* vsm = smem + G::kQBytes + G::kStages * G::kBytes;
+    float* s_ref = reinterpret_cast<float*>(vsm + G::kStages * G::kBytes);       // [128] the rows' reference
+    uint64_t* bars = reinterpret_cast<uint64_t*>(s_ref + 128);
+    uint32_t* s_misc = reinterpret_cast<uint32_t*>(bars + G::kBars);             // [0] tmem, [1] abort
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_misc + 1);
     const uint32_t b0 = smem_u32(bars);
-    auto full = [&](int s) { return b0 + 8u * s; };
-    auto empty = [&](int s) { return b0 + 8u * (G::kStages + s); };
-    const uint32_t bq = b0 + 8u * (2 * G::kStages);
-    auto sfull = [&](int i) { return bq + 8u * (1 + i); };
-    auto pfull = [&](int i) { return bq + 8u * (3 + i); };
-    auto ofull = [&](int i) { return bq + 8u * (5 + i); };
-    auto phalf = [&](int i) { return bq + 8u * (7 + i); };
-    auto turn = [&](int i) { return bq + 8u * (9 + i); };
-    const uint32_t drain = bq + 8u * 11;
+    auto kfull = [&](uint32_t s) { return b0 + 8u * s; };
+    auto kempty = [&](uint32_t s) { return b0 + 8u * (G::kStages + s); };
+    auto vfull = [&](uint32_t s) { return b0 + 8u * (2 * G::kStages + s); };
+    auto vempty = [&](uint32_t s) { return b0 + 8u * (3 * G::kStages + s); };
+    const uint32_t bq = b0 + 8u * (4 * G::kStages);
+    auto sfull = [&](uint32_t s) { return bq + 8u * (1 + s); };
+    auto pfull = [&](uint32_t s) { return bq + 8u * (1 + kBufs + s); };
+    auto pvdone = [&](uint32_t s) { return bq + 8u * (1 + 2 * kBufs + s); };
+    const uint32_t ofull = bq + 8u * (1 + 3 * kBufs);
+    auto handed = [&](int wg, int q) { return ofull + 8u * (1 + 4 * wg + q); };  // the reference, to a warp
+    auto sums = [&](int q) { return ofull + 8u * (9 + q); };                     // both warpgroups' sums
+    const uint32_t drain = ofull + 8u * 13;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const AttnArgs& a = p.a;
+    const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
+    const bool leader = rank == 0;
 
-    uint32_t idx = blockIdx.x;
+    uint32_t idx = PAIR ? cluster_id_x() : blockIdx.x;
     const int split = idx % p.nsplit;
     idx /= p.nsplit;
     const int kvh = idx % a.kv_heads;
     find_item(a.q_off, a.nset, a.nq, a.unit, idx / a.kv_heads, a.err, &it_s, scan);
-    if (it_s.set < 0) return;
-    Job j;
-    {
-        int64_t k1;
-        set_range(a.k_off, it_s.set, a.nk, j.k0, k1, a.err);
-        j.q0 = it_s.lo;
-        j.nq = (int)(it_s.hi - it_s.lo);
-        j.nk = (int)(k1 - j.k0);
-        // causal: the last rows of a set see the most keys; they go first
-        j.t0 = (a.causal ? (int)(it_s.items - 1 - it_s.item) : (int)it_s.item) * a.unit;
-        int nb[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int first = j.t0 + (ALT ? 0 : i * p.tile_tokens), last = min(first + p.tile_tokens, j.nq) - 1;
-            const int end = a.causal ? max(0, min(j.nk, last + 1 + j.nk - j.nq)) : j.nk;
-            nb[i] = first < j.nq ? (end + kKeys - 1) / kKeys : 0;
-        }
-        const int all = max(nb[0], nb[1]);
-        j.blk0 = (int)((int64_t)all * split / p.nsplit);
-        const int blk1 = (int)((int64_t)all * (split + 1) / p.nsplit);
-        j.n[0] = max(0, min(blk1, nb[0]) - j.blk0);
-        j.n[1] = max(0, min(blk1, nb[1]) - j.blk0);
-    }
-    const int nmax = max(j.n[0], j.n[1]);
+    if (it_s.set < 0) return;              // both CTAs of a pair
+    int64_t k0, k1;
+    set_range(a.k_off, it_s.set, a.nk, k0, k1, a.err);
+    const int64_t q0 = it_s.lo;
+    const int nq = (int)(it_s.hi - it_s.lo), nk = (int)(k1 - k0);
+    // causal: the last rows of a set see the most keys; they go first
+    const int first = (a.causal ? (int)(it_s.items - 1 - it_s.item) : (int)it_s.item) * a.unit;
+    const int t0 = first + (int)rank * p.tile_tokens;                            // the CTA's first token, in the set
+    const int end = a.causal ? max(0, min(nk, min(first + a.unit, nq) + nk - nq)) : nk;
+    const int all = (end + kKeys - 1) / kKeys;
+    const int blk0 = (int)((int64_t)all * split / p.nsplit), n = (int)((int64_t)all * (split + 1) / p.nsplit) - blk0;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < G::kStages; ++s) {
-            mbar_init(full(s), 1);
-            mbar_init(empty(s), ALT ? 1 : 2);        // every tile that reads it
+        for (uint32_t s = 0; s < G::kStages; ++s) {
+            mbar_init(kfull(s), PAIR && leader ? 2 : 1);        // its own TMA and the odd CTA's, passed on
+            mbar_init(kempty(s), 1);
+            mbar_init(vfull(s), PAIR && leader ? 2 : 1);
+            mbar_init(vempty(s), 1);
         }
         mbar_init(bq, 1);
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(sfull(i), 1);
-            mbar_init(pfull(i), 4);
-            mbar_init(phalf(i), 4);
-            mbar_init(turn(i), 1);
-            mbar_init(ofull(i), 1);
+        for (uint32_t s = 0; s < kBufs; ++s) {
+            mbar_init(sfull(s), 1);
+            mbar_init(pfull(s), PAIR ? 8 : 4);                  // the warps of both CTAs, at the even one
+            mbar_init(pvdone(s), 1);
+        }
+        mbar_init(ofull, 1);
+        for (int q = 0; q < 4; ++q) {
+            mbar_init(handed(0, q), 1);
+            mbar_init(handed(1, q), 1);
+            mbar_init(sums(q), 2);
         }
         mbar_init(drain, 2);
         s_misc[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 8) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     :: "r"(smem_u32(s_misc)), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                         :: "r"(smem_u32(s_misc)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                         :: "r"(smem_u32(s_misc)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
         tc_fence_before();
     }
     __syncthreads();
+    if (PAIR) cluster_sync_all();
     tc_fence_after();
-    const uint32_t tmem = s_misc[0];
-    const uint32_t sq = smem_u32(smem), skv = sq + G::kQTiles * G::kTileBytes;
-    int issued = 0;
+    const uint32_t tmem = s_misc[0], tmem_o = tmem + kBufs * 128u;
+    const uint32_t sq = smem_u32(smem), sk = sq + G::kQBytes, sv = sk + G::kStages * G::kBytes;
 
     if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsOther));
-    if (warp == 10) {
-        // ------------------------------------------------------------------ TMA producer
-        if (nmax > 0 && elect_one()) {
-            const bool two = !ALT && j.n[1] > 0;
-            mbar_arrive_expect_tx(bq, p.q_bytes * (two ? 2u : 1u));
-            for (int t = 0; t < (two ? 2 : 1); ++t)
-                for (int b = 0; b < G::kBoxes; ++b)
-                    tma_load_3d(sq + t * G::kTileBytes + b * 16384, &qmap, b * 64, kvh * a.group,
-                                (int)j.q0 + j.t0 + t * p.tile_tokens, bq);
-            // blocks in the order in which the MMA warp needs them: K0 V0 K1 V1 ...;
-            // ALT: K0 K1 V0 K2 V1 ... (two blocks are in work)
-            for (int it = 0; it < 2 * nmax; ++it) {
-                bool is_v = it & 1;
-                int blk = it >> 1;
-                if (ALT) {
-                    is_v = it == 2 * nmax - 1 || (it > 0 && !(it & 1));
-                    blk = it == 0 ? 0 : it == 2 * nmax - 1 ? nmax - 1 : is_v ? (it - 2) / 2 : (it + 1) / 2;
-                }
-                const int s = it % G::kStages;
-                if (it >= G::kStages && !mbar_wait(empty(s), (uint32_t)((it / G::kStages - 1) & 1), s_abort, a.err)) break;
-                mbar_arrive_expect_tx(full(s), G::kTileBytes);
-                for (int b = 0; b < G::kBoxes; ++b)
-                    tma_load_3d(skv + s * G::kTileBytes + b * 16384, is_v ? &vmap : &kmap, b * 64, kvh,
-                                (int)j.k0 + (j.blk0 + blk) * kKeys, full(s));
-                issued = it + 1;
-            }
-        }
-        issued = __shfl_sync(0xffffffffu, __reduce_max_sync(0xffffffffu, issued), 0);
-        __syncwarp();
-    } else if (warp < 10) {
-        // ------------------------------------------------------------------ MMA issuers, one a tile
-        // A wait costs some 150 cycles of dependent instructions even when its phase is over, and one
-        // warp for both tiles left the tensor pipe idle for 1600 of 3600 cycles a block; so each tile
-        // has its own, the ring's place is counted along and descriptors differ by constants.
-        const int i = warp - 8;
-        bool ok = nmax > 0;
-        uint32_t stage = 0, round = 0;               // ring place of the next item
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsOther));
+        bool ok = n > 0;
         auto wait = [&](uint32_t bar, uint32_t par) {
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, par, s_abort, a.err));
+            if (ok) ok = __all_sync(0xffffffffu, wait_bar<PAIR>(bar, par, s_abort, a.err));
             return ok;
         };
-        auto take = [&]() {                          // the next ring item once it has landed
-            const uint32_t st = stage;
-            wait(full(st), round);
-            if (++stage == G::kStages) {
-                stage = 0;
-                round ^= 1;
-            }
-            return st;
-        };
-        auto release = [&](uint32_t st) {
-            if (elect_one()) tc_commit(empty(st));
-            __syncwarp();
-        };
-        const uint32_t qlo = (sq >> 4) | (1u << 16), klo = (skv >> 4) | (1u << 16), vlo = (skv >> 4) | (1024u << 16);
-        constexpr uint32_t kHi = 64u | (1u << 14) | (2u << 29);
-        // S of tile i = Q K^T with K in ring place st
-        auto mma_s = [&](uint32_t st) {
-            const uint32_t ql = qlo + (ALT ? 0u : (uint32_t)(i * (G::kTileBytes >> 4))), kl = klo + st * (G::kTileBytes >> 4);
-            tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t o = (uint32_t)((k >> 2) * 1024 + (k & 3) * 2);
-                    if (k * 16 < a.dim)
-                        tc_mma(tmem + (uint32_t)(i * 128), desc64(ql + o, kHi), desc64(kl + o, kHi), p.idesc_s, k ? 1u : 0u);
-                }
-                tc_commit(sfull(i));
-            }
-            __syncwarp();
-        };
-        // The tiles take turns, a block's P V and the next S together: issued at once they would finish
-        // together, and both softmaxes would then wait for the tensor pipe and it for them.
-        auto my_turn = [&](int k) {
-            if (!ALT && (i || k)) wait(turn(i), (uint32_t)((k - 1 + i) & 1));
-            return ok;
-        };
-        auto pass = [&]() {
-            if (!ALT && lane == 0) mbar_arrive(turn(1 - i));
-        };
-        // O of tile i += P V over the block's first `keys` keys, the early ones as soon as their p is there
-        auto mma_o = [&](uint32_t st, int blk, bool first, int keys, uint32_t par) {
-            const uint32_t vl = vlo + st * (G::kTileBytes >> 4);
-            const uint32_t td = tmem + 256u + (uint32_t)(i * D), ta = tmem + (uint32_t)(i * 128);
-            if (!my_turn(blk + 1) || !wait(phalf(i), par)) return false;
-            tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-                for (int k = 0; k < kFirst / 16; ++k)
-                    if (k * 16 < keys) tc_mma_ts(td, ta + k * 8, desc64(vl + k * 128, kHi), p.idesc_o, first && k == 0 ? 0u : 1u);
-            }
-            __syncwarp();
-            if (!wait(pfull(i), par)) return false;
-            tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-                for (int k = kFirst / 16; k < kKeys / 16; ++k)
-                    if (k * 16 < keys) tc_mma_ts(td, ta + k * 8, desc64(vl + k * 128, kHi), p.idesc_o, 1u);
-            }
-            __syncwarp();
-            return true;
-        };
-        auto last = [&]() {
-            if (elect_one()) tc_commit(ofull(i));
-            __syncwarp();
-        };
-        // The rows of V behind the set's last key belong to others and may hold no numbers, which a
-        // p of 0 would not cancel: those of the last 16 that the products read become 0.
+        // The rows of V behind the set's last key belong to others and may hold no numbers, which a p
+        // of 0 would not cancel: those of the last 16 that the products read become 0.
         auto clean = [&](uint32_t st, int keys) {
             if (keys >= kKeys || (keys & 15) == 0) return;
-            uint8_t* v = smem + (G::kQTiles + st) * G::kTileBytes;
-            for (int c = lane; c < (16 - (keys & 15)) * 8 * G::kBoxes; c += 32) {
-                const int row = keys + c / (8 * G::kBoxes), x = c % (8 * G::kBoxes);
-                *reinterpret_cast<uint4*>(v + (x >> 3) * 16384 + row * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+            constexpr int per = G::kBytes / kKeys / 16;          // 16-byte words of a key's row
+            for (int w = lane; w < (16 - (keys & 15)) * per; w += 32) {
+                const int row = keys + w / per, x = w % per;
+                *reinterpret_cast<uint4*>(vsm + st * G::kBytes + (x >> 3) * 16384 + row * 128 + (x & 7) * 16) =
+                    make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();
             __syncwarp();
         };
-        int keys = j.nk - j.blk0 * kKeys;            // left from the block on
-        wait(bq, 0);
-        if (!ALT) {
-            const int n = j.n[i];                    // the other tile may have more blocks: their places pass
-            const uint32_t k0 = take();
-            if (my_turn(0)) {
-                if (n > 0) mma_s(k0);
-                pass();
-                release(k0);
+        // Descriptors of tiles in the 128-byte swizzle: low word (address >> 4) | leading offset << 16,
+        // high word 8-row groups 1024 bytes apart. Q and K have their K dimension (the head's columns)
+        // contiguous; V is the B operand with N (the head's columns) contiguous, boxes of 64 columns
+        // 16384 bytes apart.
+        constexpr uint32_t kHi = 64u | (1u << 14) | (2u << 29);
+        if (warp == 10) {
+            // -------------------------------------------------------------- TMA producer
+            if (n > 0 && elect_one()) {
+                mbar_arrive_expect_tx(bq, p.q_bytes);
+                for (int b = 0; b < G::kBoxes; ++b)
+                    tma_load_3d(sq + b * 16384, &qmap, b * 64, kvh * a.group, (int)min((int64_t)INT32_MAX, q0 + t0), bq);
+                Ring<G::kStages> r;
+                for (int b = 0; b < n; ++b, r.step()) {
+                    const int key = (int)k0 + (blk0 + b) * kKeys;
+                    if (b >= G::kStages && !wait_bar<PAIR>(kempty(r.at), r.round ^ 1, s_abort, a.err)) break;
+                    mbar_arrive_expect_tx(kfull(r.at), G::kBytes);
+                    for (int x = 0; x < G::kBoxes; ++x)
+                        tma_load_3d(sk + r.at * G::kBytes + x * (PAIR ? 8192 : 16384), &kmap, x * 64, kvh,
+                                    key + (PAIR ? (int)rank * 64 : 0), kfull(r.at));
+                    if (b >= G::kStages && !wait_bar<PAIR>(vempty(r.at), r.round ^ 1, s_abort, a.err)) break;
+                    mbar_arrive_expect_tx(vfull(r.at), G::kBytes);
+                    for (int x = 0; x < (PAIR ? 1 : G::kBoxes); ++x)
+                        tma_load_3d(sv + r.at * G::kBytes + x * 16384, &vmap, (PAIR ? (int)rank : x) * 64, kvh, key, vfull(r.at));
+                }
             }
-            for (int b = 0; b < nmax && ok; ++b, keys -= kKeys) {
-                const uint32_t v = take(), k = b + 1 < nmax ? take() : 0;
+            __syncwarp();
+        } else if (warp == 8 && leader) {
+            // -------------------------------------------------------------- S = Q K^T
+            const uint32_t qlo = (sq >> 4) | (1u << 16);
+            uint32_t klo = (sk >> 4) | (1u << 16);
+            Ring<G::kStages> r;
+            Ring<kBufs> u;
+            wait(bq, 0);
+            for (int b = 0; b < n && ok; ++b, r.step(), u.step()) {
+                if (b >= kBufs) wait(pvdone(u.at), u.round ^ 1);
+                if (!wait(kfull(r.at), r.round)) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t kl = klo + r.at * (G::kBytes >> 4);
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint64_t qd = (uint64_t)kHi << 32 | (qlo + (k >> 2) * 1024 + (k & 3) * 2);
+                        const uint64_t kd = (uint64_t)kHi << 32 | (kl + (k >> 2) * (PAIR ? 512 : 1024) + (k & 3) * 2);
+                        if (k * 16 < a.dim) {
+                            if (PAIR) tc_mma_ss_pair(tmem + u.at * 128, qd, kd, p.idesc_s, k ? 1u : 0u);
+                            else tc_mma(tmem + u.at * 128, qd, kd, p.idesc_s, k ? 1u : 0u);
+                        }
+                    }
+                    commit<PAIR>(sfull(u.at));
+                    commit<PAIR>(kempty(r.at));
+                }
+                __syncwarp();
+            }
+            // every MMA has completed before the TMEM is freed (also after an abort)
+            if (elect_one()) PAIR ? tc_commit_pair(drain, 0x1) : tc_commit(drain);
+            __syncwarp();
+        } else if (warp == 9 && leader) {
+            // -------------------------------------------------------------- O += P V
+            const uint32_t vlo = (sv >> 4) | (1024u << 16);
+            Ring<G::kStages> r;
+            Ring<kBufs> u;
+            int keys = nk - blk0 * kKeys;
+            for (int b = 0; b < n && ok; ++b, r.step(), u.step(), keys -= kKeys) {
+                if (!wait(vfull(r.at), r.round)) break;
+                clean(r.at, keys);
+                if (!wait(pfull(u.at), u.round)) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t vl = vlo + r.at * (G::kBytes >> 4);
+#pragma unroll
+                    for (int k = 0; k < kKeys / 16; ++k) {
+                        const uint64_t vd = (uint64_t)kHi << 32 | (vl + k * 128);
+                        if (k * 16 < keys) {
+                            if (PAIR) tc_mma_ts_pair(tmem_o, tmem + u.at * 128 + k * 8, vd, p.idesc_o, b || k ? 1u : 0u);
+                            else tc_mma_ts(tmem_o, tmem + u.at * 128 + k * 8, vd, p.idesc_o, b || k ? 1u : 0u);
+                        }
+                    }
+                    commit<PAIR>(pvdone(u.at));
+                    commit<PAIR>(vempty(r.at));
+                    if (b == n - 1) commit<PAIR>(ofull);
+                }
+                __syncwarp();
+            }
+            if (elect_one()) PAIR ? tc_commit_pair(drain, 0x1) : tc_commit(drain);
+            __syncwarp();
+        } else if (PAIR && (warp == 8 || warp == 9)) {
+            // -------------------------------------------------------------- odd CTA: what has landed, passed on
+            Ring<G::kStages> r;
+            int keys = nk - blk0 * kKeys;
+            if (warp == 8 && ok) ok = __all_sync(0xffffffffu, mbar_wait(bq, 0, s_abort, a.err));
+            for (int b = 0; b < n && ok; ++b, r.step(), keys -= kKeys) {
+                const uint32_t bar = warp == 8 ? kfull(r.at) : vfull(r.at);
+                ok = __all_sync(0xffffffffu, mbar_wait(bar, r.round, s_abort, a.err));
                 if (!ok) break;
-                if (b < n) {
-                    clean(v, keys);
-                    if (!mma_o(v, b, b == 0, keys, (uint32_t)(b & 1))) break;
-                    if (b + 1 < n) mma_s(k);
-                    else last();
-                } else if (!my_turn(b + 1)) {
-                    break;
+                if (warp == 9) clean(r.at, keys);
+                if (lane == 0) {
+                    if (warp == 9 && keys < kKeys) mbar_arrive_cluster(bar, 0);     // its zeros before the products
+                    else mbar_arrive_cluster_relaxed(bar, 0);
                 }
-                pass();
-                release(v);
-                if (b + 1 < nmax) release(k);
-            }
-        } else {
-            // ring: K0 K1 V0 K2 V1 ...; this tile's blocks are i, i + 2, ...
-            const int n = nmax;
-            auto skip = [&]() {
-                if (++stage == G::kStages) {
-                    stage = 0;
-                    round ^= 1;
-                }
-            };
-            if (i == 0) {
-                const uint32_t k = take();
-                if (ok) {
-                    mma_s(k);
-                    release(k);
-                }
-                if (n > 1) skip();
-            } else if (n > 1) {
-                skip();
-                const uint32_t k = take();
-                if (ok) {
-                    mma_s(k);
-                    release(k);
-                }
-            }
-            for (int b = 0; b < n && ok; ++b, keys -= kKeys) {
-                if ((b & 1) != i) {                  // the other tile's V and K
-                    skip();
-                    if (b + 2 < n) skip();
-                    continue;
-                }
-                const uint32_t v = take(), k = b + 2 < n ? take() : 0;
-                if (!ok) break;
-                clean(v, keys);
-                if (!mma_o(v, b, b < 2, keys, (uint32_t)((b >> 1) & 1))) break;
-                if (b + 2 < n) mma_s(k);
-                else last();
-                release(v);
-                if (b + 2 < n) release(k);
             }
         }
-        // every MMA has completed before the TMEM is freed (also after an abort)
-        if (elect_one()) tc_commit(drain);
-        __syncwarp();
-        const long long t0 = clock64();
-        while (!mbar_try_wait(drain, 0) && clock64() - t0 < kWaitCycles) { }
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kRegsSoftmax));
         // ------------------------------------------------------------------ softmax and output
-        const int i = warp >> 2, r = (warp & 3) * 32 + lane;
-        const int t = j.t0 + (ALT ? 0 : i * p.tile_tokens) + r / a.group;
-        const int h = kvh * a.group + r % a.group;
-        const bool valid = r < p.tile_tokens * a.group && t < j.nq;
-        const int lim = !valid ? j.nk : a.causal ? max(0, min(j.nk, t + 1 + j.nk - j.nq)) : j.nk;   // keys the row sees
+        const int wg = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
+        const int t = t0 + r / a.group, h = kvh * a.group + r % a.group;
+        const bool valid = r < p.tile_tokens * a.group && t < nq;
+        const int lim = !valid ? nk : a.causal ? max(0, min(nk, t + 1 + nk - nq)) : nk;     // keys the row sees
         const int wlim = __reduce_min_sync(0xffffffffu, lim);
-        const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t ts = lane_base + (uint32_t)(i * 128), to = lane_base + 256u + (uint32_t)(i * D);
+        const uint32_t lane_base = (uint32_t)(quad * 32) << 16, to = tmem_o + lane_base;
         const float c = a.scale_log2;
         // p in f16 starts at 2^7 instead of 1 (2^15 after the largest rise): small p keep their digits
         constexpr float lift = std::is_same<T, __half>::value ? 7.f : 0.f;
-        const int n = ALT ? (j.n[0] + 1 - i) / 2 : j.n[i];
-        float m = -INFINITY, l = 0.f;
+        float ref = -INFINITY, l = 0.f;              // of the warpgroup's own blocks; -inf: no key so far
         bool ok = true;
-        for (int b = 0; b < n; ++b) {
-            const int key0 = (j.blk0 + (ALT ? 2 * b + i : b)) * kKeys;
-            if (!__all_sync(0xffffffffu, mbar_wait(sfull(i), (uint32_t)(b & 1), s_abort, a.err))) { ok = false; break; }
+        Ring<kBufs> u;
+        if (wg == 1) u.step();
+        for (int b = wg; b < n; b += 2) {
+            const uint32_t ts = tmem + u.at * 128u + lane_base;
+            if (!__all_sync(0xffffffffu, wait_bar<PAIR>(sfull(u.at), u.round, s_abort, a.err))) { ok = false; break; }
             tc_fence_after();
             float s[128];
 #pragma unroll
             for (int q = 0; q < 4; ++q) tmem_ld_x32(ts + q * 32, s + q * 32);
             tmem_wait_ld();
+            const int key0 = (blk0 + b) * kKeys;
             const bool masked = wlim < key0 + kKeys;
             if (masked) {
                 const int left = lim - key0;
 #pragma unroll
                 for (int q = 0; q < 128; ++q) s[q] = q < left ? s[q] : -INFINITY;
             }
-            float mx[4] = {s[0], s[1], s[2], s[3]};
+            float mx[4];
 #pragma unroll
-            for (int q = 4; q < 124; q += 8) {
+            for (int e = 0; e < 4; ++e) mx[e] = max3(s[e], s[e + 4], s[e + 8]);
+#pragma unroll
+            for (int q = 12; q < 124; q += 8) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[q + e], s[q + 4 + e]);
             }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[124 + e]);
-            const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-            if (b == 0) {
-                m = mn;
-            } else if (__any_sync(0xffffffffu, (mn - m) * c > kRaise)) {
-                const float al = mn == m ? 1.f : ex2((m - mn) * c);
-                m = mn;
-                l *= al;
-#pragma unroll 1
-                for (int q = 0; q < D; q += 32) {
-                    float o[32];
-                    tmem_ld_x32(to + q, o);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] *= al;
-                    tmem_st_x32(to + q, reinterpret_cast<const uint32_t*>(o));
-                }
+            const float top = max3(max3(mx[0], mx[1], s[124]), max3(mx[2], mx[3], s[125]), max2(s[126], s[127])) * c;
+
+            // the reference after the block before, from the other warpgroup
+            float now = -INFINITY;
+            if (b > 0) {
+                const uint32_t par = (uint32_t)((wg ? b - 1 : b - 2) >> 1 & 1);
+                if (!__all_sync(0xffffffffu, mbar_wait(handed(wg, quad), par, s_abort, a.err))) { ok = false; break; }
+                now = s_ref[r];
             }
-            const float ref = lift - (m == -INFINITY ? 0.f : m * c);
-            // p in quarters of 32 keys; the products start on the first kFirst keys
-            if (masked) exp_block<T, 0>(s, c, ref, ts, phalf(i), lane);
-            else exp_block<T, kPoly>(s, c, ref, ts, phalf(i), lane);
+            const bool raise = !(top - now <= kRaise) && !(top == -INFINITY && now == -INFINITY);
+            if (b == 0 || __any_sync(0xffffffffu, raise)) {
+                const float next = raise ? rintf(top) : now;
+                s_ref[r] = next;
+                if (b > 0) {
+                    // O is at rest once the block before has been added
+                    const uint32_t before = u.at ? u.at - 1 : kBufs - 1, par = u.at ? u.round : u.round ^ 1;
+                    if (!__all_sync(0xffffffffu, wait_bar<PAIR>(pvdone(before), par, s_abort, a.err))) { ok = false; break; }
+                    tc_fence_after();
+                    const float al = raise ? ex2(now - next) : 1.f;
+#pragma unroll 1
+                    for (int q = 0; q < D; q += 32) {
+                        float o[32];
+                        tmem_ld_x32(to + q, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] *= al;
+                        tmem_st_x32(to + q, reinterpret_cast<const uint32_t*>(o));
+                    }
+                }
+                now = next;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(handed(1 - wg, quad));
+            l = now == ref ? l : l * ex2(ref - now);
+            ref = now;
+            const bool far = __any_sync(0xffffffffu, !(fabsf(ref) < kFar) && ref != -INFINITY);
+            const float shift = lift - (ref == -INFINITY ? 0.f : ref);
+            if (masked || far) exp_block<T, 0>(s, c, shift, ts);
+            else exp_block<T, kPoly>(s, c, shift, ts);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(pfull(i));
+            if (lane == 0) {
+                if (PAIR) mbar_arrive_cluster_relaxed(pfull(u.at), 0);
+                else mbar_arrive(pfull(u.at));
+            }
             f2 sum[2] = {pack(s[0], s[1]), pack(s[2], s[3])};
 #pragma unroll
             for (int q = 4; q < 128; q += 4) {
@@ -505,49 +466,55 @@ k_attn_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUte
             }
             const float2 both = unpack(add2(sum[0], sum[1]));
             l += both.x + both.y;
+            u.step();
+            u.step();
         }
         if (n > 0 && ok) {
-            ok = __all_sync(0xffffffffu, mbar_wait(ofull(i), 0, s_abort, a.err));
+            ok = __all_sync(0xffffffffu, wait_bar<PAIR>(ofull, 0, s_abort, a.err));
             tc_fence_after();
         }
+        float total = 0.f;
+        if (n > 0 && ok) {
+            // both warpgroups' sums against the last reference, through Q's place (its products are done)
+            float2* s_sum = reinterpret_cast<float2*>(smem);
+            s_sum[wg * 128 + r] = make_float2(l, ref);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sums(quad));
+            ok = __all_sync(0xffffffffu, mbar_wait(sums(quad), 0, s_abort, a.err));
+            const float2 x = s_sum[r], y = s_sum[128 + r];
+            ref = s_ref[r];
+            total = (x.y == ref ? x.x : x.y == -INFINITY ? 0.f : x.x * ex2(x.y - ref)) +
+                    (y.y == ref ? y.x : y.y == -INFINITY ? 0.f : y.x * ex2(y.y - ref));
+        }
         if (ok) {
-            const bool none = n == 0 || lim <= (j.blk0 + (ALT ? i : 0)) * kKeys;    // the row sees no key here
-            const float inv = none ? 0.f : 1.f / l;
-            const float lg = none ? -INFINITY : m * c - lift + log2f(l);
-            const int64_t row = j.q0 + t;
-            if (p.part) {
-                const int64_t at = ((int64_t)(ALT ? 2 * split + i : split) * a.nq + row) * a.heads + h;
-                if (valid) p.part_lse[at] = lg;
-                float* out = p.part + at * a.dim;
+            const bool none = n == 0 || lim <= blk0 * kKeys;       // the row sees no key here
+            const float inv = none ? 0.f : 1.f / total;
+            const float lg = none ? -INFINITY : ref - lift + log2f(total);
+            const int64_t row = q0 + t;
+            const int64_t at = ((int64_t)split * a.nq + row) * a.heads + h;
+            if (valid && wg == 0) {
+                if (p.part) p.part_lse[at] = lg;
+                else if (a.lse) a.lse[row * a.heads + h] = lg * 0.69314718055994530942f;
+            }
+            float* part = p.part + at * a.dim;
+            O* out = reinterpret_cast<O*>(a.out) + row * a.out_row + (int64_t)h * a.out_head;
+            // each warpgroup writes half of the head's columns
+#pragma unroll 1
+            for (int q = wg * (D / 2); q < (wg + 1) * (D / 2); q += 32) {
+                float o[32];
+                __syncwarp();
                 if (n > 0) {
-#pragma unroll 1
-                    for (int q = 0; q < D; q += 32) {
-                        float o[32];
-                        __syncwarp();
-                        tmem_ld_x32(to + q, o);
-                        tmem_wait_ld();
-                        if (!valid || none) continue;
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            if (q + e < a.dim)
-                                *reinterpret_cast<float4*>(out + q + e) =
-                                    make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
-                    }
+                    tmem_ld_x32(to + q, o);
+                    tmem_wait_ld();
                 }
-            } else {
-                if (valid && a.lse) a.lse[row * a.heads + h] = lg * 0.69314718055994530942f;
-                O* out = reinterpret_cast<O*>(a.out) + row * a.out_row + (int64_t)h * a.out_head;
-#pragma unroll 1
-                for (int q = 0; q < D; q += 32) {
-                    float o[32];
-                    __syncwarp();
-                    if (n > 0) {
-                        tmem_ld_x32(to + q, o);
-                        tmem_wait_ld();
-                    }
-                    if (!valid) continue;
+                if (!valid || (p.part && none)) continue;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = none ? 0.f : o[e] * inv;
+                for (int e = 0; e < 32; ++e) o[e] = none ? 0.f : o[e] * inv;
+                if (p.part) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+                        if (q + e < a.dim) store8<float>(part + q + e, o + e);
+                } else {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8)
                         if (q + e < a.dim) store8<O>(out + q + e, o + e);
@@ -557,18 +524,35 @@ k_attn_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUte
         tc_fence_before();
     }
     __syncthreads();
-    if (warp == 10 && lane == 0 && *s_abort) {
-        // after an abort, TMA loads still in flight land before the CTA exits
-        const long long t0 = clock64();
-        for (int it = max(0, issued - G::kStages); it < issued; ++it)
-            while (!mbar_try_wait(full(it % G::kStages), (uint32_t)((it / G::kStages) & 1)) && clock64() - t0 < kWaitCycles) { }
-        while (nmax > 0 && !mbar_try_wait(bq, 0) && clock64() - t0 < kWaitCycles) { }
+    if (warp == 8 && leader) {
+        const long long w0 = clock64();
+        while (!mbar_try_wait(drain, 0) && clock64() - w0 < kWaitCycles) { }
+    }
+    if (*s_abort && threadIdx.x == 0 && n > 0) {
+        // after an abort: wait out the loads that may still be in flight
+        const long long w0 = clock64();
+        while (clock64() - w0 < 20000000) { }
     }
     __syncthreads();
+    if (PAIR) cluster_sync_all();
     if (warp == 8) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
     }
+}
+
+template <class T, class O, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+k_attn_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+          const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TcArgs p) {
+    attn_tc<T, O, D, false>(qmap, kmap, vmap, p);
+}
+template <class T, class O>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+k_attn_pair(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+            const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TcArgs p) {
+    attn_tc<T, O, 128, true>(qmap, kmap, vmap, p);
 }
 
 // Joins the partial rows: with lg_s the base-2 log sum of part s and M their maximum,
@@ -620,24 +604,23 @@ __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ TcArg
 }
 
 struct Plan {
-    bool alt;
-    int tile_tokens, unit, nsplit, nsp;
-    int64_t items;
+    bool pair;
+    int tile_tokens, unit, nsplit;
+    int64_t items;                     // CTAs, or pairs of them
 };
 
-// ALT when an average set's rows fit one tile. Keys are cut where the CTAs would not fill the SMs.
-Plan attn_plan(int num_sms, int64_t nq, int64_t nk, int nset, int kv_heads, int group) {
+// Pairs for wide heads where an average set's rows fill more than one CTA. Keys are cut where the CTAs
+// would not fill the SMs.
+Plan attn_plan(int num_sms, int64_t nq, int64_t nk, int nset, int kv_heads, int group, int dim) {
     Plan l;
     l.tile_tokens = 128 / group;
-    l.alt = (nq + nset - 1) / nset <= l.tile_tokens;
-    l.unit = l.alt ? l.tile_tokens : 2 * l.tile_tokens;
+    l.pair = dim > 64 && (nq + nset - 1) / nset > l.tile_tokens;
+    l.unit = l.pair ? 2 * l.tile_tokens : l.tile_tokens;
     const int64_t pieces = (nq + l.unit - 1) / l.unit;
-    const int64_t ctas = std::max<int64_t>(pieces, std::min<int64_t>(nset, nq)) * kv_heads;
+    const int64_t ctas = std::max<int64_t>(pieces, std::min<int64_t>(nset, nq)) * kv_heads * (l.pair ? 2 : 1);
     const int64_t blocks = (nk / nset + kKeys - 1) / kKeys;          // of an average set
     l.nsplit = 1;
-    if (ctas < 2 * num_sms)
-        l.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({4ll * num_sms / ctas, blocks / 8, 32}));
-    l.nsp = l.alt ? 2 * l.nsplit : (l.nsplit > 1 ? l.nsplit : 0);
+    if (ctas < num_sms) l.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({4ll * num_sms / ctas, blocks / 8, 32}));
     l.items = (pieces + nset) * kv_heads * l.nsplit;
     return l;
 }
@@ -662,62 +645,61 @@ tb_status encode(tb_ctx* ctx, CUtensorMap* map, tb_dtype dtype, const void* base
     return cr == CUDA_SUCCESS ? TB_OK : tb_fail(ctx, TB_ERR_CUDA, "cuTensorMapEncodeTiled failed for tb_attention");
 }
 
-template <class T, class O, int D, bool ALT>
+template <class T, class O>
 tb_status launch(tb_ctx* ctx, const TcArgs& p, const Plan& l, const CUtensorMap& qm, const CUtensorMap& km,
                  const CUtensorMap& vm) {
-    constexpr size_t sm = Geom<D, ALT>::kSmem;
+    const bool wide = p.a.dim > 64;
+    const size_t sm = l.pair ? Geom<128, true>::kSmem : wide ? Geom<128, false>::kSmem : Geom<64, false>::kSmem;
+    const void* kernel = l.pair ? (const void*)k_attn_pair<T, O>
+                                : wide ? (const void*)k_attn_tc<T, O, 128> : (const void*)k_attn_tc<T, O, 64>;
     if (sm > (size_t)ctx->max_smem_optin) return tb_fail(ctx, TB_ERR_UNSUPPORTED, "tb_attention: shared memory too small");
-    TB_CUDA_TRY(ctx, cudaFuncSetAttribute(k_attn_tc<T, O, D, ALT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
-    k_attn_tc<T, O, D, ALT><<<(unsigned)l.items, kThreads, sm, ctx->stream>>>(qm, km, vm, p);
+    TB_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
+    if (l.pair) k_attn_pair<T, O><<<(unsigned)(2 * l.items), kThreads, sm, ctx->stream>>>(qm, km, vm, p);
+    else if (wide) k_attn_tc<T, O, 128><<<(unsigned)l.items, kThreads, sm, ctx->stream>>>(qm, km, vm, p);
+    else k_attn_tc<T, O, 64><<<(unsigned)l.items, kThreads, sm, ctx->stream>>>(qm, km, vm, p);
     TB_LAUNCH_CHECK(ctx, "k_attn_tc");
     if (p.part) {
-        k_attn_join<O><<<(unsigned)((p.a.nq * p.a.heads + 7) / 8), 256, 0, ctx->stream>>>(p, l.nsp);
+        k_attn_join<O><<<(unsigned)((p.a.nq * p.a.heads + 7) / 8), 256, 0, ctx->stream>>>(p, l.nsplit);
         TB_LAUNCH_CHECK(ctx, "k_attn_join");
     }
     return TB_OK;
-}
-
-template <class T, class O>
-tb_status launch_any(tb_ctx* ctx, const TcArgs& p, const Plan& l, const CUtensorMap& qm, const CUtensorMap& km,
-                     const CUtensorMap& vm) {
-    if (p.a.dim <= 64) return l.alt ? launch<T, O, 64, true>(ctx, p, l, qm, km, vm) : launch<T, O, 64, false>(ctx, p, l, qm, km, vm);
-    return l.alt ? launch<T, O, 128, true>(ctx, p, l, qm, km, vm) : launch<T, O, 128, false>(ctx, p, l, qm, km, vm);
 }
 
 }  // namespace
 
 size_t tb_attn_tc_workspace(const tb_ctx* ctx, int64_t nq, int64_t nk, int nset, int heads, int kv_heads, int dim) {
     if (nq <= 0 || nk <= 0 || nset <= 0) return 0;
-    const Plan l = attn_plan(ctx->num_sms, nq, nk, nset, kv_heads, heads / kv_heads);
-    return (size_t)l.nsp * nq * heads * (dim + 1) * sizeof(float);
+    const Plan l = attn_plan(ctx->num_sms, nq, nk, nset, kv_heads, heads / kv_heads, dim);
+    return l.nsplit > 1 ? (size_t)l.nsplit * nq * heads * (dim + 1) * sizeof(float) : 0;
 }
 
 tb_status tb_attn_tc_launch(tb_ctx* ctx, const AttnArgs& args, tb_dtype dtype, tb_dtype out_dtype, void* workspace) {
     TcArgs p{};
     p.a = args;
     const AttnArgs& a = p.a;
-    const Plan l = attn_plan(ctx->num_sms, a.nq, a.nk, a.nset, a.kv_heads, a.group);
-    if (l.items > INT32_MAX || (l.nsp && (a.nq * a.heads + 7) / 8 > INT32_MAX))
+    const Plan l = attn_plan(ctx->num_sms, a.nq, a.nk, a.nset, a.kv_heads, a.group, a.dim);
+    if (2 * l.items > INT32_MAX || (l.nsplit > 1 && (a.nq * a.heads + 7) / 8 > INT32_MAX))
         return tb_fail(ctx, TB_ERR_TOO_LARGE, "tb_attention: too many rows times heads");
     p.a.unit = l.unit;
     p.tile_tokens = l.tile_tokens;
     p.nsplit = l.nsplit;
-    if (l.nsp) {
+    if (l.nsplit > 1) {
         p.part = reinterpret_cast<float*>(workspace);
-        p.part_lse = p.part + (size_t)l.nsp * a.nq * a.heads * a.dim;
+        p.part_lse = p.part + (size_t)l.nsplit * a.nq * a.heads * a.dim;
     }
     const uint32_t fmt = dtype == TB_BF16 ? 1u : 0u;
-    const uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | (8u << 24);
+    const uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((l.pair ? 16u : 8u) << 24);
     p.idesc_s = base | (16u << 17);
-    p.idesc_o = base | (1u << 16) | ((uint32_t)((a.dim + 15) / 16 * 2) << 17);        // B (V) with N contiguous
+    // B (V) with N contiguous; a pair's halves are 64 columns each, behind the head's last one zeros
+    p.idesc_o = base | (1u << 16) | ((l.pair ? 16u : (uint32_t)((a.dim + 15) / 16 * 2)) << 17);
     p.q_bytes = (uint32_t)((a.dim <= 64 ? 1 : 2) * 128 * a.group * l.tile_tokens);
     CUtensorMap qm, km, vm;
     tb_status s = encode(ctx, &qm, dtype, a.q, a.dim, a.heads, a.q_head, a.nq, a.q_row, (uint32_t)a.group, (uint32_t)l.tile_tokens);
-    if (s == TB_OK) s = encode(ctx, &km, dtype, a.k, a.dim, a.kv_heads, a.k_head, a.nk, a.k_row, 1, kKeys);
+    if (s == TB_OK) s = encode(ctx, &km, dtype, a.k, a.dim, a.kv_heads, a.k_head, a.nk, a.k_row, 1, l.pair ? 64 : kKeys);
     if (s == TB_OK) s = encode(ctx, &vm, dtype, a.v, a.dim, a.kv_heads, a.v_head, a.nk, a.v_row, 1, kKeys);
     if (s != TB_OK) return s;
     if (dtype == TB_F16)
-        return out_dtype == TB_F32 ? launch_any<__half, float>(ctx, p, l, qm, km, vm) : launch_any<__half, __half>(ctx, p, l, qm, km, vm);
-    return out_dtype == TB_F32 ? launch_any<__nv_bfloat16, float>(ctx, p, l, qm, km, vm)
-                               : launch_any<__nv_bfloat16, __nv_bfloat16>(ctx, p, l, qm, km, vm);
+        return out_dtype == TB_F32 ? launch<__half, float>(ctx, p, l, qm, km, vm) : launch<__half, __half>(ctx, p, l, qm, km, vm);
+    return out_dtype == TB_F32 ? launch<__nv_bfloat16, float>(ctx, p, l, qm, km, vm)
+                               : launch<__nv_bfloat16, __nv_bfloat16>(ctx, p, l, qm, km, vm);
 }
