@@ -33,7 +33,7 @@ namespace {
 using namespace tbtc;
 using namespace tbpk;
 
-constexpr int kThreads = 384;          // warps 0-3 and 4-7 softmax, 8 S, 9 P V, 10 TMA, 11 idle
+constexpr int kThreads = 384;          // warps 0-3 and 4-7 softmax, 8 products, 10 TMA, 9 (odd CTA of a pair) V passed on
 // Registers: 65536 / 384 threads allows 168 at launch; the third warpgroup gives up what the two
 // softmax warpgroups need to hold a row of S. 2 * 208 + 88 = 3 * 168.
 constexpr int kRegsSoftmax = 208, kRegsOther = 88;
@@ -113,17 +113,19 @@ __device__ __forceinline__ float2 ex2_poly(float s0, float s1, float least, f2 c
                        __int_as_float(__float_as_int(v.y) + (__float_as_int(i.y) << 23)));
 }
 
-// p = 2^(s c + ref) of a row's 128 scores, left in s and, rounded to T, in the TMEM columns from `ts`.
-// NPOLY of every 8 pairs go by polynomial, which shares the work between the exponential unit (4
-// lanes a cycle and scheduler: 1024 cycles a block, as long as its products) and the FMA pipes. A
-// hidden score (-inf) has to give exactly 0: masked blocks use NPOLY 0.
+// p = 2^(s c + ref) of a row's 128 scores, rounded to T into the TMEM columns from `ts`; returns their
+// sum. NPOLY of every 8 pairs go by polynomial, which shares the work between the exponential unit (4
+// lanes a cycle and scheduler: 1024 cycles a block, as long as its products) and the FMA pipes. The
+// sum's additions fill slots that the exponential unit leaves (after the block they took 150 to 500
+// cycles of their own). A hidden score (-inf) has to give exactly 0: masked blocks use NPOLY 0.
 template <class T, int NPOLY>
-__device__ __forceinline__ void exp_block(float* s, float c, float ref, uint32_t ts) {
+__device__ __forceinline__ float exp_block(const float* s, float c, float ref, uint32_t ts) {
     const f2 c2 = pack(c, c), ref2 = pack(ref, ref), lifted = add2(ref2, pack(12582912.f, 12582912.f));
     const float least = NPOLY ? __fdividef(-120.f - ref, c) : 0.f;
+    f2 sum[4];
 #pragma unroll
     for (int quarter = 0; quarter < 4; ++quarter) {
-        float* v = s + quarter * 32;
+        const float* v = s + quarter * 32;
         uint32_t w[16];
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
@@ -135,12 +137,13 @@ __device__ __forceinline__ void exp_block(float* s, float c, float ref, uint32_t
                 y.x = ex2(y.x);
                 y.y = ex2(y.y);
             }
-            v[2 * q] = y.x;
-            v[2 * q + 1] = y.y;
             w[q] = pack2(y.x, y.y, T());
+            sum[q & 3] = quarter || q >= 4 ? add2(sum[q & 3], pack(y.x, y.y)) : pack(y.x, y.y);
         }
         tmem_st_x16(ts + quarter * 16, w);
     }
+    const float2 all = unpack(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+    return all.x + all.y;
 }
 
 // Hand-offs inside a CTA, or across the pair: those order tcgen05 operations only (see tb_tc_ptx.cuh).
@@ -230,7 +233,7 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
             mbar_init(handed(1, q), 1);
             mbar_init(sums(q), 2);
         }
-        mbar_init(drain, 2);
+        mbar_init(drain, 1);
         s_misc[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -299,48 +302,43 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
             }
             __syncwarp();
         } else if (warp == 8 && leader) {
-            // -------------------------------------------------------------- S = Q K^T
-            const uint32_t qlo = (sq >> 4) | (1u << 16);
-            uint32_t klo = (sk >> 4) | (1u << 16);
-            Ring<G::kStages> r;
+            // -------------------------------------------------------------- the products
+            // One warp issues both: a block's P V and, into the buffer that it frees, the S three blocks on.
+            // MMAs of one thread run in order, so nothing is waited for between the two.
+            const uint32_t qlo = (sq >> 4) | (1u << 16), klo = (sk >> 4) | (1u << 16), vlo = (sv >> 4) | (1024u << 16);
+            Ring<G::kStages> rk, rv;
             Ring<kBufs> u;
-            wait(bq, 0);
-            for (int b = 0; b < n && ok; ++b, r.step(), u.step()) {
-                if (b >= kBufs) wait(pvdone(u.at), u.round ^ 1);
-                if (!wait(kfull(r.at), r.round)) break;
+            auto mma_s = [&](uint32_t buf) {
                 tc_fence_after();
                 if (elect_one()) {
-                    const uint32_t kl = klo + r.at * (G::kBytes >> 4);
+                    const uint32_t kl = klo + rk.at * (G::kBytes >> 4);
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
                         const uint64_t qd = (uint64_t)kHi << 32 | (qlo + (k >> 2) * 1024 + (k & 3) * 2);
                         const uint64_t kd = (uint64_t)kHi << 32 | (kl + (k >> 2) * (PAIR ? 512 : 1024) + (k & 3) * 2);
                         if (k * 16 < a.dim) {
-                            if (PAIR) tc_mma_ss_pair(tmem + u.at * 128, qd, kd, p.idesc_s, k ? 1u : 0u);
-                            else tc_mma(tmem + u.at * 128, qd, kd, p.idesc_s, k ? 1u : 0u);
+                            if (PAIR) tc_mma_ss_pair(tmem + buf * 128, qd, kd, p.idesc_s, k ? 1u : 0u);
+                            else tc_mma(tmem + buf * 128, qd, kd, p.idesc_s, k ? 1u : 0u);
                         }
                     }
-                    commit<PAIR>(sfull(u.at));
-                    commit<PAIR>(kempty(r.at));
+                    commit<PAIR>(sfull(buf));
+                    commit<PAIR>(kempty(rk.at));
                 }
                 __syncwarp();
-            }
-            // every MMA has completed before the TMEM is freed (also after an abort)
-            if (elect_one()) PAIR ? tc_commit_pair(drain, 0x1) : tc_commit(drain);
-            __syncwarp();
-        } else if (warp == 9 && leader) {
-            // -------------------------------------------------------------- O += P V
-            const uint32_t vlo = (sv >> 4) | (1024u << 16);
-            Ring<G::kStages> r;
-            Ring<kBufs> u;
+                rk.step();
+            };
+            wait(bq, 0);
+            for (uint32_t b = 0; b < kBufs && (int)b < n; ++b)
+                if (wait(kfull(rk.at), rk.round)) mma_s(b);
             int keys = nk - blk0 * kKeys;
-            for (int b = 0; b < n && ok; ++b, r.step(), u.step(), keys -= kKeys) {
-                if (!wait(vfull(r.at), r.round)) break;
-                clean(r.at, keys);
+            for (int b = 0; b < n && ok; ++b, rv.step(), u.step(), keys -= kKeys) {
+                wait(vfull(rv.at), rv.round);
+                if (ok) clean(rv.at, keys);
+                if (b + kBufs < n) wait(kfull(rk.at), rk.round);
                 if (!wait(pfull(u.at), u.round)) break;
                 tc_fence_after();
                 if (elect_one()) {
-                    const uint32_t vl = vlo + r.at * (G::kBytes >> 4);
+                    const uint32_t vl = vlo + rv.at * (G::kBytes >> 4);
 #pragma unroll
                     for (int k = 0; k < kKeys / 16; ++k) {
                         const uint64_t vd = (uint64_t)kHi << 32 | (vl + k * 128);
@@ -350,14 +348,16 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                         }
                     }
                     commit<PAIR>(pvdone(u.at));
-                    commit<PAIR>(vempty(r.at));
+                    commit<PAIR>(vempty(rv.at));
                     if (b == n - 1) commit<PAIR>(ofull);
                 }
                 __syncwarp();
+                if (b + kBufs < n) mma_s(u.at);
             }
+            // every MMA has completed before the TMEM is freed (also after an abort)
             if (elect_one()) PAIR ? tc_commit_pair(drain, 0x1) : tc_commit(drain);
             __syncwarp();
-        } else if (PAIR && (warp == 8 || warp == 9)) {
+        } else if (PAIR && !leader && (warp == 8 || warp == 9)) {
             // -------------------------------------------------------------- odd CTA: what has landed, passed on
             Ring<G::kStages> r;
             int keys = nk - blk0 * kKeys;
@@ -386,7 +386,8 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
         // p in f16 starts at 2^7 instead of 1 (2^15 after the largest rise): small p keep their digits
         constexpr float lift = std::is_same<T, __half>::value ? 7.f : 0.f;
         float ref = -INFINITY, l = 0.f;              // of the warpgroup's own blocks; -inf: no key so far
-        bool ok = true;
+        float shift = lift;                          // what scores are shifted by: lift - ref
+        bool ok = true, far = false;
         Ring<kBufs> u;
         if (wg == 1) u.step();
         for (int b = wg; b < n; b += 2) {
@@ -396,6 +397,13 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
             float s[128];
 #pragma unroll
             for (int q = 0; q < 4; ++q) tmem_ld_x32(ts + q * 32, s + q * 32);
+            // meanwhile: the reference after the block before, from the other warpgroup
+            float now = -INFINITY;
+            if (b > 0) {
+                const uint32_t par = (uint32_t)((wg ? b - 1 : b - 2) >> 1 & 1);
+                if (!__all_sync(0xffffffffu, mbar_wait(handed(wg, quad), par, s_abort, a.err))) { ok = false; break; }
+                now = s_ref[r];
+            }
             tmem_wait_ld();
             const int key0 = (blk0 + b) * kKeys;
             const bool masked = wlim < key0 + kKeys;
@@ -413,19 +421,11 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[q + e], s[q + 4 + e]);
             }
             const float top = max3(max3(mx[0], mx[1], s[124]), max3(mx[2], mx[3], s[125]), max2(s[126], s[127])) * c;
-
-            // the reference after the block before, from the other warpgroup
-            float now = -INFINITY;
-            if (b > 0) {
-                const uint32_t par = (uint32_t)((wg ? b - 1 : b - 2) >> 1 & 1);
-                if (!__all_sync(0xffffffffu, mbar_wait(handed(wg, quad), par, s_abort, a.err))) { ok = false; break; }
-                now = s_ref[r];
-            }
             const bool raise = !(top - now <= kRaise) && !(top == -INFINITY && now == -INFINITY);
-            if (b == 0 || __any_sync(0xffffffffu, raise)) {
+            if (far || __any_sync(0xffffffffu, raise || now != ref)) {
                 const float next = raise ? rintf(top) : now;
                 s_ref[r] = next;
-                if (b > 0) {
+                if (b > 0 && __any_sync(0xffffffffu, raise)) {
                     // O is at rest once the block before has been added
                     const uint32_t before = u.at ? u.at - 1 : kBufs - 1, par = u.at ? u.round : u.round ^ 1;
                     if (!__all_sync(0xffffffffu, wait_bar<PAIR>(pvdone(before), par, s_abort, a.err))) { ok = false; break; }
@@ -441,16 +441,13 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                         tmem_st_x32(to + q, reinterpret_cast<const uint32_t*>(o));
                     }
                 }
-                now = next;
+                l = next == ref ? l : l * ex2(ref - next);
+                ref = next;
+                shift = lift - (ref == -INFINITY ? 0.f : ref);
+                far = __any_sync(0xffffffffu, !(fabsf(ref) < kFar) && ref != -INFINITY);
             }
-            __syncwarp();
             if (lane == 0) mbar_arrive(handed(1 - wg, quad));
-            l = now == ref ? l : l * ex2(ref - now);
-            ref = now;
-            const bool far = __any_sync(0xffffffffu, !(fabsf(ref) < kFar) && ref != -INFINITY);
-            const float shift = lift - (ref == -INFINITY ? 0.f : ref);
-            if (masked || far) exp_block<T, 0>(s, c, shift, ts);
-            else exp_block<T, kPoly>(s, c, shift, ts);
+            l += masked || far ? exp_block<T, 0>(s, c, shift, ts) : exp_block<T, kPoly>(s, c, shift, ts);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -458,14 +455,6 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 if (PAIR) mbar_arrive_cluster_relaxed(pfull(u.at), 0);
                 else mbar_arrive(pfull(u.at));
             }
-            f2 sum[2] = {pack(s[0], s[1]), pack(s[2], s[3])};
-#pragma unroll
-            for (int q = 4; q < 128; q += 4) {
-                sum[0] = add2(sum[0], pack(s[q], s[q + 1]));
-                sum[1] = add2(sum[1], pack(s[q + 2], s[q + 3]));
-            }
-            const float2 both = unpack(add2(sum[0], sum[1]));
-            l += both.x + both.y;
             u.step();
             u.step();
         }
