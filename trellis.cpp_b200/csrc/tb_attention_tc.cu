@@ -33,16 +33,24 @@ namespace {
 using namespace tbtc;
 using namespace tbpk;
 
-constexpr int kThreads = 384;          // warps 0-3 and 4-7 softmax, 8 products, 10 TMA, 9 (odd CTA of a pair) V passed on
-// Registers: 65536 / 384 threads allows 168 at launch; the third warpgroup gives up what the two
-// softmax warpgroups need to hold a row of S. 2 * 208 + 88 = 3 * 168.
-constexpr int kRegsSoftmax = 208, kRegsOther = 88;
+#ifndef TB_PARTS
+#define TB_PARTS 1
+#endif
+constexpr int kParts = TB_PARTS;       // parts of a block, each a warpgroup's step
+constexpr int kWgs = 2 * kParts;       // softmax warpgroups
+constexpr int kThreads = kWgs * 128 + 128;
+constexpr int kMma = kWgs * 4;         // warps: softmax, then products (odd CTA of a pair: passes on), TMA, two idle
+constexpr int kTma = kMma + 1;
+// Registers: 65536 / kThreads (96 or 168) at launch; the last warpgroup gives up what the softmax
+// warpgroups need to hold a row of a step. 4 * 104 + 64 = 5 * 96, 2 * 208 + 88 = 3 * 168.
+constexpr int kRegsSoftmax = kParts == 2 ? 104 : 208, kRegsOther = kParts == 2 ? 64 : 88;
 constexpr int kKeys = 128;             // keys of a block
+constexpr int kStep = kKeys / kParts;  // keys of a step
 constexpr int kBufs = 3;               // S buffers
 constexpr float kRaise = 8.f;          // the reference follows when a block's maximum is 2^8 above it
 constexpr float kFar = 2097152.f;      // 2^21: references that ex2_poly can add 1.5 * 2^23 to
 #ifndef TB_POLY
-#define TB_POLY 2
+#define TB_POLY 0
 #endif
 constexpr int kPoly = TB_POLY;         // of every 8 pairs of exponentials, those by polynomial
 
@@ -58,8 +66,8 @@ template <int D, bool PAIR> struct Geom {
     static constexpr int kBoxes = D / 64;
     static constexpr int kQBytes = kBoxes * 16384;                // 128 rows x D, boxes of 64 columns
     static constexpr int kBytes = kBoxes * 16384 / (PAIR ? 2 : 1);   // a CTA's share of a block's K, of its V
-    static constexpr int kStages = (196608 / 2) / kBytes;         // of K, and of V
-    static constexpr int kBars = 4 * kStages + 1 + 3 * kBufs + 1 + 8 + 4 + 1;
+    static constexpr int kStages = 196608 / (2 * kBytes);         // of a K and a V each
+    static constexpr int kBars = 2 * kStages + 1 + (1 + 2 * kParts) * kBufs + 1 + 4 * kWgs + 4 + 1;
     static constexpr size_t kSmem = (size_t)kQBytes + 2 * kStages * kBytes + 512 + 8 * kBars + 16 + 1024;
 };
 
@@ -73,6 +81,12 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 // columns) contiguous; V is the B operand with N (the head's columns) contiguous, its boxes of 64
 // columns 16384 bytes apart.
 __device__ __forceinline__ uint64_t desc64(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, float* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+                   "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+                 : "r"(taddr));
+}
 __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, float* v) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
                  "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -113,18 +127,18 @@ __device__ __forceinline__ float2 ex2_poly(float s0, float s1, float least, f2 c
                        __int_as_float(__float_as_int(v.y) + (__float_as_int(i.y) << 23)));
 }
 
-// p = 2^(s c + ref) of a row's 128 scores, rounded to T into the TMEM columns from `ts`; returns their
+// p = 2^(s c + ref) of a step's scores of a row, rounded to T into the TMEM columns from `ts`; returns their
 // sum. NPOLY of every 8 pairs go by polynomial, which shares the work between the exponential unit (4
 // lanes a cycle and scheduler: 1024 cycles a block, as long as its products) and the FMA pipes. The
-// sum's additions fill slots that the exponential unit leaves (after the block they took 150 to 500
-// cycles of their own). A hidden score (-inf) has to give exactly 0: masked blocks use NPOLY 0.
+// sum's additions fill slots that the exponential unit leaves. A hidden score (-inf) has to give
+// exactly 0: masked steps use NPOLY 0.
 template <class T, int NPOLY>
-__device__ __forceinline__ float exp_block(const float* s, float c, float ref, uint32_t ts) {
+__device__ __forceinline__ float exp_step(const float* s, float c, float ref, uint32_t ts) {
     const f2 c2 = pack(c, c), ref2 = pack(ref, ref), lifted = add2(ref2, pack(12582912.f, 12582912.f));
     const float least = NPOLY ? __fdividef(-120.f - ref, c) : 0.f;
-    f2 sum[4];
+    f2 sum[2];
 #pragma unroll
-    for (int quarter = 0; quarter < 4; ++quarter) {
+    for (int quarter = 0; quarter < kStep / 32; ++quarter) {
         const float* v = s + quarter * 32;
         uint32_t w[16];
 #pragma unroll
@@ -138,11 +152,11 @@ __device__ __forceinline__ float exp_block(const float* s, float c, float ref, u
                 y.y = ex2(y.y);
             }
             w[q] = pack2(y.x, y.y, T());
-            sum[q & 3] = quarter || q >= 4 ? add2(sum[q & 3], pack(y.x, y.y)) : pack(y.x, y.y);
+            sum[q & 1] = quarter || q >= 2 ? add2(sum[q & 1], pack(y.x, y.y)) : pack(y.x, y.y);
         }
         tmem_st_x16(ts + quarter * 16, w);
     }
-    const float2 all = unpack(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+    const float2 all = unpack(add2(sum[0], sum[1]));
     return all.x + all.y;
 }
 
@@ -174,24 +188,22 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
     __shared__ Item it_s;
     __shared__ uint32_t scan[32];
     uint8_t* smem = smem_align1024(smem_raw);
-    uint8_t* vsm = smem + G::kQBytes + G::kStages * G::kBytes;
-    float* s_ref = reinterpret_cast<float*>(vsm + G::kStages * G::kBytes);       // [128] the rows' reference
+    uint8_t* ring = smem + G::kQBytes;
+    float* s_ref = reinterpret_cast<float*>(ring + 2 * G::kStages * G::kBytes);       // [128] the rows' reference
     uint64_t* bars = reinterpret_cast<uint64_t*>(s_ref + 128);
     uint32_t* s_misc = reinterpret_cast<uint32_t*>(bars + G::kBars);             // [0] tmem, [1] abort
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_misc + 1);
     const uint32_t b0 = smem_u32(bars);
-    auto kfull = [&](uint32_t s) { return b0 + 8u * s; };
-    auto kempty = [&](uint32_t s) { return b0 + 8u * (G::kStages + s); };
-    auto vfull = [&](uint32_t s) { return b0 + 8u * (2 * G::kStages + s); };
-    auto vempty = [&](uint32_t s) { return b0 + 8u * (3 * G::kStages + s); };
-    const uint32_t bq = b0 + 8u * (4 * G::kStages);
+    auto full = [&](uint32_t s) { return b0 + 8u * s; };
+    auto empty = [&](uint32_t s) { return b0 + 8u * (G::kStages + s); };
+    const uint32_t bq = b0 + 8u * (2 * G::kStages);
     auto sfull = [&](uint32_t s) { return bq + 8u * (1 + s); };
-    auto pfull = [&](uint32_t s) { return bq + 8u * (1 + kBufs + s); };
-    auto pvdone = [&](uint32_t s) { return bq + 8u * (1 + 2 * kBufs + s); };
-    const uint32_t ofull = bq + 8u * (1 + 3 * kBufs);
+    auto pfull = [&](uint32_t s, int part) { return bq + 8u * (1 + kBufs + kParts * s + part); };
+    auto pvdone = [&](uint32_t s, int part) { return bq + 8u * (1 + (1 + kParts) * kBufs + kParts * s + part); };
+    const uint32_t ofull = bq + 8u * (1 + (1 + 2 * kParts) * kBufs);
     auto handed = [&](int wg, int q) { return ofull + 8u * (1 + 4 * wg + q); };  // the reference, to a warp
-    auto sums = [&](int q) { return ofull + 8u * (9 + q); };                     // both warpgroups' sums
-    const uint32_t drain = ofull + 8u * 13;
+    auto sums = [&](int q) { return ofull + 8u * (1 + 4 * kWgs + q); };          // the warpgroups' sums
+    const uint32_t drain = ofull + 8u * (5 + 4 * kWgs);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const AttnArgs& a = p.a;
     const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
@@ -214,30 +226,30 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
     const int all = (end + kKeys - 1) / kKeys;
     const int blk0 = (int)((int64_t)all * split / p.nsplit), n = (int)((int64_t)all * (split + 1) / p.nsplit) - blk0;
 
+    if (threadIdx.x < 128) s_ref[threadIdx.x] = -INFINITY;
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < G::kStages; ++s) {
-            mbar_init(kfull(s), PAIR && leader ? 2 : 1);        // its own TMA and the odd CTA's, passed on
-            mbar_init(kempty(s), 1);
-            mbar_init(vfull(s), PAIR && leader ? 2 : 1);
-            mbar_init(vempty(s), 1);
+            mbar_init(full(s), PAIR && leader ? 2 : 1);         // its own TMA and the odd CTA's, passed on
+            mbar_init(empty(s), 1);
         }
         mbar_init(bq, 1);
         for (uint32_t s = 0; s < kBufs; ++s) {
             mbar_init(sfull(s), 1);
-            mbar_init(pfull(s), PAIR ? 8 : 4);                  // the warps of both CTAs, at the even one
-            mbar_init(pvdone(s), 1);
+            for (int part = 0; part < kParts; ++part) {
+                mbar_init(pfull(s, part), PAIR ? 8 : 4);        // the warps of both CTAs, at the even one
+                mbar_init(pvdone(s, part), 1);
+            }
         }
         mbar_init(ofull, 1);
         for (int q = 0; q < 4; ++q) {
-            mbar_init(handed(0, q), 1);
-            mbar_init(handed(1, q), 1);
-            mbar_init(sums(q), 2);
+            for (int wg = 0; wg < kWgs; ++wg) mbar_init(handed(wg, q), 1);
+            mbar_init(sums(q), kWgs);
         }
         mbar_init(drain, 1);
         s_misc[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == kMma) {
         if (PAIR) {
             asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
                          :: "r"(smem_u32(s_misc)), "r"(512u) : "memory");
@@ -253,130 +265,146 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
     if (PAIR) cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = s_misc[0], tmem_o = tmem + kBufs * 128u;
-    const uint32_t sq = smem_u32(smem), sk = sq + G::kQBytes, sv = sk + G::kStages * G::kBytes;
+    const uint32_t sq = smem_u32(smem), skv = sq + G::kQBytes;
+    // The ring's item j holds the K of block j and the V of block j - lag: what the products of one round,
+    // P V of a block and the S three blocks on, read. One barrier to wait for, one to free.
+    const int lag = min(n, kBufs), items = n + lag;
 
-    if (warp >= 8) {
+    if (warp >= kMma) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsOther));
-        bool ok = n > 0;
-        auto wait = [&](uint32_t bar, uint32_t par) {
-            if (ok) ok = __all_sync(0xffffffffu, wait_bar<PAIR>(bar, par, s_abort, a.err));
-            return ok;
-        };
         // The rows of V behind the set's last key belong to others and may hold no numbers, which a p
         // of 0 would not cancel: those of the last 16 that the products read become 0.
-        auto clean = [&](uint32_t st, int keys) {
-            if (keys >= kKeys || (keys & 15) == 0) return;
-            constexpr int per = G::kBytes / kKeys / 16;          // 16-byte words of a key's row
-            for (int w = lane; w < (16 - (keys & 15)) * per; w += 32) {
-                const int row = keys + w / per, x = w % per;
-                *reinterpret_cast<uint4*>(vsm + st * G::kBytes + (x >> 3) * 16384 + row * 128 + (x & 7) * 16) =
-                    make_uint4(0, 0, 0, 0);
+        const int tail = nk - (blk0 + n - 1) * kKeys;          // keys of the last block
+        const bool dirty = n > 0 && tail < kKeys && (tail & 15);
+        auto clean = [&]() {
+            constexpr int per = G::kBytes / kKeys / 16;         // 16-byte words of a key's row
+            uint8_t* v = ring + ((items - 1) % G::kStages) * (2 * G::kBytes) + G::kBytes;
+            for (int w = lane; w < (16 - (tail & 15)) * per; w += 32) {
+                const int row = tail + w / per, x = w % per;
+                *reinterpret_cast<uint4*>(v + (x >> 3) * 16384 + row * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();
             __syncwarp();
         };
-        // Descriptors of tiles in the 128-byte swizzle: low word (address >> 4) | leading offset << 16,
-        // high word 8-row groups 1024 bytes apart. Q and K have their K dimension (the head's columns)
-        // contiguous; V is the B operand with N (the head's columns) contiguous, boxes of 64 columns
-        // 16384 bytes apart.
-        constexpr uint32_t kHi = 64u | (1u << 14) | (2u << 29);
-        if (warp == 10) {
+        if (warp == kTma) {
             // -------------------------------------------------------------- TMA producer
             if (n > 0 && elect_one()) {
                 mbar_arrive_expect_tx(bq, p.q_bytes);
                 for (int b = 0; b < G::kBoxes; ++b)
-                    tma_load_3d(sq + b * 16384, &qmap, b * 64, kvh * a.group, (int)min((int64_t)INT32_MAX, q0 + t0), bq);
+                    tma_load_3d(sq + b * 16384, &qmap, b * 64, kvh * a.group, (int)(q0 + t0), bq);
                 Ring<G::kStages> r;
-                for (int b = 0; b < n; ++b, r.step()) {
-                    const int key = (int)k0 + (blk0 + b) * kKeys;
-                    if (b >= G::kStages && !wait_bar<PAIR>(kempty(r.at), r.round ^ 1, s_abort, a.err)) break;
-                    mbar_arrive_expect_tx(kfull(r.at), G::kBytes);
-                    for (int x = 0; x < G::kBoxes; ++x)
-                        tma_load_3d(sk + r.at * G::kBytes + x * (PAIR ? 8192 : 16384), &kmap, x * 64, kvh,
-                                    key + (PAIR ? (int)rank * 64 : 0), kfull(r.at));
-                    if (b >= G::kStages && !wait_bar<PAIR>(vempty(r.at), r.round ^ 1, s_abort, a.err)) break;
-                    mbar_arrive_expect_tx(vfull(r.at), G::kBytes);
-                    for (int x = 0; x < (PAIR ? 1 : G::kBoxes); ++x)
-                        tma_load_3d(sv + r.at * G::kBytes + x * 16384, &vmap, (PAIR ? (int)rank : x) * 64, kvh, key, vfull(r.at));
+                for (int j = 0; j < items; ++j, r.step()) {
+                    if (j >= G::kStages && !wait_bar<PAIR>(empty(r.at), r.round ^ 1, s_abort, a.err)) break;
+                    const uint32_t k_at = skv + r.at * (2 * G::kBytes), v_at = k_at + G::kBytes;
+                    mbar_arrive_expect_tx(full(r.at), j < n && j >= lag ? 2 * G::kBytes : G::kBytes);
+                    const int key = (int)k0 + (blk0 + j) * kKeys;
+                    if (j < n)
+                        for (int x = 0; x < G::kBoxes; ++x)
+                            tma_load_3d(k_at + x * (PAIR ? 8192 : 16384), &kmap, x * 64, kvh, key + (PAIR ? (int)rank * 64 : 0),
+                                        full(r.at));
+                    if (j >= lag)
+                        for (int x = 0; x < (PAIR ? 1 : G::kBoxes); ++x)
+                            tma_load_3d(v_at + x * 16384, &vmap, (PAIR ? (int)rank : x) * 64, kvh, key - lag * kKeys, full(r.at));
                 }
             }
             __syncwarp();
-        } else if (warp == 8 && leader) {
+        } else if (warp == kMma && leader) {
             // -------------------------------------------------------------- the products
             // One warp issues both: a block's P V and, into the buffer that it frees, the S three blocks on.
-            // MMAs of one thread run in order, so nothing is waited for between the two.
-            const uint32_t qlo = (sq >> 4) | (1u << 16), klo = (sk >> 4) | (1u << 16), vlo = (sv >> 4) | (1024u << 16);
-            Ring<G::kStages> rk, rv;
-            Ring<kBufs> u;
-            auto mma_s = [&](uint32_t buf) {
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint32_t kl = klo + rk.at * (G::kBytes >> 4);
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint64_t qd = (uint64_t)kHi << 32 | (qlo + (k >> 2) * 1024 + (k & 3) * 2);
-                        const uint64_t kd = (uint64_t)kHi << 32 | (kl + (k >> 2) * (PAIR ? 512 : 1024) + (k & 3) * 2);
-                        if (k * 16 < a.dim) {
-                            if (PAIR) tc_mma_ss_pair(tmem + buf * 128, qd, kd, p.idesc_s, k ? 1u : 0u);
-                            else tc_mma(tmem + buf * 128, qd, kd, p.idesc_s, k ? 1u : 0u);
-                        }
-                    }
-                    commit<PAIR>(sfull(buf));
-                    commit<PAIR>(kempty(rk.at));
-                }
-                __syncwarp();
-                rk.step();
+            // MMAs of one thread run in order, so nothing is waited for between the two. Its instructions
+            // are the pace where the softmax keeps up: a wait costs some 150 cycles even when its phase is
+            // over, an MMA issued by a thread on its own 100 instead of 40. Descriptors differ by
+            // constants: low word (address >> 4) | leading offset << 16, high word 8-row groups 1024 bytes
+            // apart in the 128-byte swizzle. Q and K have their K dimension (the head's columns)
+            // contiguous; V is the B operand with N (the head's columns) contiguous, boxes of 64 columns
+            // 16384 bytes apart.
+            constexpr uint32_t kHi = 64u | (1u << 14) | (2u << 29);
+            const uint32_t qlo = (sq >> 4) | (1u << 16), klo = (skv >> 4) | (1u << 16);
+            const uint32_t vlo = ((skv + G::kBytes) >> 4) | (1024u << 16);
+            const int dim = a.dim;
+            bool ok = n > 0;
+            auto wait = [&](uint32_t bar, uint32_t par) {
+                if (ok) ok = __all_sync(0xffffffffu, wait_bar<PAIR>(bar, par, s_abort, a.err));
+                return ok;
             };
-            wait(bq, 0);
-            for (uint32_t b = 0; b < kBufs && (int)b < n; ++b)
-                if (wait(kfull(rk.at), rk.round)) mma_s(b);
-            int keys = nk - blk0 * kKeys;
-            for (int b = 0; b < n && ok; ++b, rv.step(), u.step(), keys -= kKeys) {
-                wait(vfull(rv.at), rv.round);
-                if (ok) clean(rv.at, keys);
-                if (b + kBufs < n) wait(kfull(rk.at), rk.round);
-                if (!wait(pfull(u.at), u.round)) break;
+            Ring<G::kStages> r;
+            Ring<kBufs> u;
+            auto mma_s = [&](uint32_t buf) {         // by the elected thread
+                const uint32_t kl = klo + r.at * (2 * G::kBytes >> 4), td = tmem + buf * 128;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint64_t qd = (uint64_t)kHi << 32 | (qlo + (k >> 2) * 1024 + (k & 3) * 2);
+                    const uint64_t kd = (uint64_t)kHi << 32 | (kl + (k >> 2) * (PAIR ? 512 : 1024) + (k & 3) * 2);
+                    if (k * 16 < dim) {
+                        if (PAIR) tc_mma_ss_pair(td, qd, kd, p.idesc_s, k ? 1u : 0u);
+                        else tc_mma(td, qd, kd, p.idesc_s, k ? 1u : 0u);
+                    }
+                }
+                commit<PAIR>(sfull(buf));
+            };
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bq, 0, s_abort, a.err));
+            for (uint32_t b = 0; (int)b < lag && ok; ++b, r.step()) {
+                if (!wait(full(r.at), r.round)) break;
                 tc_fence_after();
                 if (elect_one()) {
-                    const uint32_t vl = vlo + rv.at * (G::kBytes >> 4);
-#pragma unroll
-                    for (int k = 0; k < kKeys / 16; ++k) {
-                        const uint64_t vd = (uint64_t)kHi << 32 | (vl + k * 128);
-                        if (k * 16 < keys) {
-                            if (PAIR) tc_mma_ts_pair(tmem_o, tmem + u.at * 128 + k * 8, vd, p.idesc_o, b || k ? 1u : 0u);
-                            else tc_mma_ts(tmem_o, tmem + u.at * 128 + k * 8, vd, p.idesc_o, b || k ? 1u : 0u);
-                        }
-                    }
-                    commit<PAIR>(pvdone(u.at));
-                    commit<PAIR>(vempty(rv.at));
-                    if (b == n - 1) commit<PAIR>(ofull);
+                    mma_s(b);
+                    commit<PAIR>(empty(r.at));
                 }
                 __syncwarp();
-                if (b + kBufs < n) mma_s(u.at);
+            }
+            int keys = nk - blk0 * kKeys;
+            for (int b = 0; b < n && ok; ++b, r.step(), u.step(), keys -= kKeys) {
+                if (!wait(full(r.at), r.round)) break;
+                if (b == n - 1 && dirty) clean();
+                const uint32_t vl = vlo + r.at * (2 * G::kBytes >> 4);
+#pragma unroll
+                for (int part = 0; part < kParts; ++part) {
+                    if (!wait(pfull(u.at, part), u.round)) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t pa = tmem + u.at * 128 + part * kStep;
+#pragma unroll
+                        for (int k = part * (kStep / 16); k < (part + 1) * (kStep / 16); ++k) {
+                            const uint64_t vd = (uint64_t)kHi << 32 | (vl + k * 128);
+                            const uint32_t ap = pa + (k % (kStep / 16)) * 8;
+                            if (k * 16 < keys) {
+                                if (PAIR) tc_mma_ts_pair(tmem_o, ap, vd, p.idesc_o, b || k ? 1u : 0u);
+                                else tc_mma_ts(tmem_o, ap, vd, p.idesc_o, b || k ? 1u : 0u);
+                            }
+                        }
+                        commit<PAIR>(pvdone(u.at, part));
+                        if (part == kParts - 1) {
+                            if (b + lag < n) mma_s(u.at);
+                            commit<PAIR>(empty(r.at));
+                            if (b == n - 1) commit<PAIR>(ofull);
+                        }
+                    }
+                    __syncwarp();
+                }
             }
             // every MMA has completed before the TMEM is freed (also after an abort)
             if (elect_one()) PAIR ? tc_commit_pair(drain, 0x1) : tc_commit(drain);
             __syncwarp();
-        } else if (PAIR && !leader && (warp == 8 || warp == 9)) {
+        } else if (PAIR && !leader && warp == kMma) {
             // -------------------------------------------------------------- odd CTA: what has landed, passed on
             Ring<G::kStages> r;
-            int keys = nk - blk0 * kKeys;
-            if (warp == 8 && ok) ok = __all_sync(0xffffffffu, mbar_wait(bq, 0, s_abort, a.err));
-            for (int b = 0; b < n && ok; ++b, r.step(), keys -= kKeys) {
-                const uint32_t bar = warp == 8 ? kfull(r.at) : vfull(r.at);
-                ok = __all_sync(0xffffffffu, mbar_wait(bar, r.round, s_abort, a.err));
+            bool ok = n > 0 && __all_sync(0xffffffffu, mbar_wait(bq, 0, s_abort, a.err));
+            for (int j = 0; j < items && ok; ++j, r.step()) {
+                ok = __all_sync(0xffffffffu, mbar_wait(full(r.at), r.round, s_abort, a.err));
                 if (!ok) break;
-                if (warp == 9) clean(r.at, keys);
+                const bool last = j == items - 1 && dirty;
+                if (last) clean();
                 if (lane == 0) {
-                    if (warp == 9 && keys < kKeys) mbar_arrive_cluster(bar, 0);     // its zeros before the products
-                    else mbar_arrive_cluster_relaxed(bar, 0);
+                    if (last) mbar_arrive_cluster(full(r.at), 0);               // its zeros before the products
+                    else mbar_arrive_cluster_relaxed(full(r.at), 0);
                 }
             }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kRegsSoftmax));
         // ------------------------------------------------------------------ softmax and output
-        const int wg = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
+        // Warpgroup wg takes part wg % kParts of every other block.
+        const int wg = warp >> 2, quad = warp & 3, r = quad * 32 + lane, part = wg % kParts;
         const int t = t0 + r / a.group, h = kvh * a.group + r % a.group;
         const bool valid = r < p.tile_tokens * a.group && t < nq;
         const int lim = !valid ? nk : a.causal ? max(0, min(nk, t + 1 + nk - nq)) : nk;     // keys the row sees
@@ -385,50 +413,51 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
         const float c = a.scale_log2;
         // p in f16 starts at 2^7 instead of 1 (2^15 after the largest rise): small p keep their digits
         constexpr float lift = std::is_same<T, __half>::value ? 7.f : 0.f;
-        float ref = -INFINITY, l = 0.f;              // of the warpgroup's own blocks; -inf: no key so far
+        float ref = -INFINITY, l = 0.f;              // of the warpgroup's own steps; -inf: no key so far
         float shift = lift;                          // what scores are shifted by: lift - ref
         bool ok = true, far = false;
         Ring<kBufs> u;
-        if (wg == 1) u.step();
-        for (int b = wg; b < n; b += 2) {
-            const uint32_t ts = tmem + u.at * 128u + lane_base;
+        if (wg >= kParts) u.step();
+        uint32_t mine = wg == 0 ? 1 : 0;             // parity of the reference's next hand-off
+        for (int b = wg / kParts; b < n; b += 2, mine ^= 1) {
+            const uint32_t ts = tmem + u.at * 128u + part * kStep + lane_base;
             if (!__all_sync(0xffffffffu, wait_bar<PAIR>(sfull(u.at), u.round, s_abort, a.err))) { ok = false; break; }
             tc_fence_after();
-            float s[128];
+            float s[kStep];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) tmem_ld_x32(ts + q * 32, s + q * 32);
-            // meanwhile: the reference after the block before, from the other warpgroup
-            float now = -INFINITY;
-            if (b > 0) {
-                const uint32_t par = (uint32_t)((wg ? b - 1 : b - 2) >> 1 & 1);
-                if (!__all_sync(0xffffffffu, mbar_wait(handed(wg, quad), par, s_abort, a.err))) { ok = false; break; }
-                now = s_ref[r];
-            }
+            for (int q = 0; q < kStep; q += 32) tmem_ld_x32(ts + q, s + q);
             tmem_wait_ld();
-            const int key0 = (blk0 + b) * kKeys;
-            const bool masked = wlim < key0 + kKeys;
+            const int key0 = (blk0 + b) * kKeys + part * kStep;
+            const bool masked = wlim < key0 + kStep;
             if (masked) {
                 const int left = lim - key0;
 #pragma unroll
-                for (int q = 0; q < 128; ++q) s[q] = q < left ? s[q] : -INFINITY;
+                for (int q = 0; q < kStep; ++q) s[q] = q < left ? s[q] : -INFINITY;
             }
             float mx[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) mx[e] = max3(s[e], s[e + 4], s[e + 8]);
 #pragma unroll
-            for (int q = 12; q < 124; q += 8) {
+            for (int q = 12; q < kStep - 4; q += 8) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[q + e], s[q + 4 + e]);
             }
-            const float top = max3(max3(mx[0], mx[1], s[124]), max3(mx[2], mx[3], s[125]), max2(s[126], s[127])) * c;
+            const float top = max3(max3(mx[0], mx[1], s[kStep - 4]), max3(mx[2], mx[3], s[kStep - 3]), max2(s[kStep - 2], s[kStep - 1])) * c;
+            // The reference after the step before, from the warpgroup before. Only the comparison stands between
+            // two hand-offs: with the loads and the maximum in between they came 1000 cycles apart.
+            float now = -INFINITY;
+            if (b > 0 || wg > 0) {
+                if (!__all_sync(0xffffffffu, mbar_wait(handed(wg, quad), mine, s_abort, a.err))) { ok = false; break; }
+                now = s_ref[r];
+            }
             const bool raise = !(top - now <= kRaise) && !(top == -INFINITY && now == -INFINITY);
             if (far || __any_sync(0xffffffffu, raise || now != ref)) {
                 const float next = raise ? rintf(top) : now;
                 s_ref[r] = next;
-                if (b > 0 && __any_sync(0xffffffffu, raise)) {
-                    // O is at rest once the block before has been added
-                    const uint32_t before = u.at ? u.at - 1 : kBufs - 1, par = u.at ? u.round : u.round ^ 1;
-                    if (!__all_sync(0xffffffffu, wait_bar<PAIR>(pvdone(before), par, s_abort, a.err))) { ok = false; break; }
+                if ((b > 0 || part) && __any_sync(0xffffffffu, raise)) {
+                    // O is at rest once the step before has been added
+                    const uint32_t before = part ? u.at : u.at ? u.at - 1 : kBufs - 1, par = part || u.at ? u.round : u.round ^ 1;
+                    if (!__all_sync(0xffffffffu, wait_bar<PAIR>(pvdone(before, part ? part - 1 : kParts - 1), par, s_abort, a.err))) { ok = false; break; }
                     tc_fence_after();
                     const float al = raise ? ex2(now - next) : 1.f;
 #pragma unroll 1
@@ -441,19 +470,20 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                         tmem_st_x32(to + q, reinterpret_cast<const uint32_t*>(o));
                     }
                 }
+                __syncwarp();                        // s_ref before the hand-off
                 l = next == ref ? l : l * ex2(ref - next);
                 ref = next;
                 shift = lift - (ref == -INFINITY ? 0.f : ref);
                 far = __any_sync(0xffffffffu, !(fabsf(ref) < kFar) && ref != -INFINITY);
             }
-            if (lane == 0) mbar_arrive(handed(1 - wg, quad));
-            l += masked || far ? exp_block<T, 0>(s, c, shift, ts) : exp_block<T, kPoly>(s, c, shift, ts);
+            if (lane == 0) mbar_arrive(handed((wg + 1) % kWgs, quad));
+            l += masked || far ? exp_step<T, 0>(s, c, shift, ts) : exp_step<T, kPoly>(s, c, shift, ts);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                if (PAIR) mbar_arrive_cluster_relaxed(pfull(u.at), 0);
-                else mbar_arrive(pfull(u.at));
+                if (PAIR) mbar_arrive_cluster_relaxed(pfull(u.at, part), 0);
+                else mbar_arrive(pfull(u.at, part));
             }
             u.step();
             u.step();
@@ -464,16 +494,18 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
         }
         float total = 0.f;
         if (n > 0 && ok) {
-            // both warpgroups' sums against the last reference, through Q's place (its products are done)
+            // all warpgroups' sums against the last reference, through Q's place (its products are done)
             float2* s_sum = reinterpret_cast<float2*>(smem);
             s_sum[wg * 128 + r] = make_float2(l, ref);
             __syncwarp();
             if (lane == 0) mbar_arrive(sums(quad));
             ok = __all_sync(0xffffffffu, mbar_wait(sums(quad), 0, s_abort, a.err));
-            const float2 x = s_sum[r], y = s_sum[128 + r];
             ref = s_ref[r];
-            total = (x.y == ref ? x.x : x.y == -INFINITY ? 0.f : x.x * ex2(x.y - ref)) +
-                    (y.y == ref ? y.x : y.y == -INFINITY ? 0.f : y.x * ex2(y.y - ref));
+#pragma unroll
+            for (int w = 0; w < kWgs; ++w) {
+                const float2 x = s_sum[w * 128 + r];
+                total += x.y == ref ? x.x : x.y == -INFINITY ? 0.f : x.x * ex2(x.y - ref);
+            }
         }
         if (ok) {
             const bool none = n == 0 || lim <= blk0 * kKeys;       // the row sees no key here
@@ -485,35 +517,34 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 if (p.part) p.part_lse[at] = lg;
                 else if (a.lse) a.lse[row * a.heads + h] = lg * 0.69314718055994530942f;
             }
-            float* part = p.part + at * a.dim;
+            float* part_row = p.part + at * a.dim;
             O* out = reinterpret_cast<O*>(a.out) + row * a.out_row + (int64_t)h * a.out_head;
-            // each warpgroup writes half of the head's columns
-#pragma unroll 1
-            for (int q = wg * (D / 2); q < (wg + 1) * (D / 2); q += 32) {
-                float o[32];
+            // each warpgroup writes its share of the head's columns
+            constexpr int W = D / kWgs;
+#pragma unroll
+            for (int w = 0; w < W; w += 16) {
+                const int q = wg * W + w;
+                float o[16];
                 __syncwarp();
                 if (n > 0) {
-                    tmem_ld_x32(to + q, o);
+                    tmem_ld_x16(to + q, o);
                     tmem_wait_ld();
                 }
                 if (!valid || (p.part && none)) continue;
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = none ? 0.f : o[e] * inv;
-                if (p.part) {
+                for (int e = 0; e < 16; ++e) o[e] = none ? 0.f : o[e] * inv;
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8)
-                        if (q + e < a.dim) store8<float>(part + q + e, o + e);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8)
-                        if (q + e < a.dim) store8<O>(out + q + e, o + e);
-                }
+                for (int e = 0; e < 16; e += 8)
+                    if (q + e < a.dim) {
+                        if (p.part) store8<float>(part_row + q + e, o + e);
+                        else store8<O>(out + q + e, o + e);
+                    }
             }
         }
         tc_fence_before();
     }
     __syncthreads();
-    if (warp == 8 && leader) {
+    if (warp == kMma && leader) {
         const long long w0 = clock64();
         while (!mbar_try_wait(drain, 0) && clock64() - w0 < kWaitCycles) { }
     }
@@ -524,7 +555,7 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
     }
     __syncthreads();
     if (PAIR) cluster_sync_all();
-    if (warp == 8) {
+    if (warp == kMma) {
         tc_fence_after();
         if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
         else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
