@@ -19,6 +19,10 @@
 // The warpgroups hand it on from block to block through shared memory; the one that raises it waits
 // until the block before has been added and scales O.
 //
+// The grid is what fits the GPU; each CTA (pair) works through its share of the list of tiles, so the next
+// tile's loads and first products run while the last one's softmax and output finish (a launch of
+// one CTA a tile paid some 4 us a tile for them). One warp finds the tiles in the tables of sets.
+//
 // With few CTAs the keys are cut into `nsplit` ranges, which leave partial rows (32 bits, normalised,
 // with their log sums) that k_attn_join adds up in a fixed order.
 #include "tb_packed.cuh"
@@ -33,19 +37,13 @@ namespace {
 using namespace tbtc;
 using namespace tbpk;
 
-#ifndef TB_PARTS
-#define TB_PARTS 1
-#endif
-constexpr int kParts = TB_PARTS;       // parts of a block, each a warpgroup's step
-constexpr int kWgs = 2 * kParts;       // softmax warpgroups
-constexpr int kThreads = kWgs * 128 + 128;
-constexpr int kMma = kWgs * 4;         // warps: softmax, then products (odd CTA of a pair: passes on), TMA, two idle
-constexpr int kTma = kMma + 1;
-// Registers: 65536 / kThreads (96 or 168) at launch; the last warpgroup gives up what the softmax
-// warpgroups need to hold a row of a step. 4 * 104 + 64 = 5 * 96, 2 * 208 + 88 = 3 * 168.
-constexpr int kRegsSoftmax = kParts == 2 ? 104 : 208, kRegsOther = kParts == 2 ? 64 : 88;
+constexpr int kThreads = 384;
+constexpr int kMma = 8, kTma = 9, kList = 10;      // warps 0-3 and 4-7 softmax, products (odd CTA of a pair: passes on), TMA, list
+// Registers: 65536 / 384 threads allows 168 at launch; the third warpgroup gives up what the two
+// softmax warpgroups need to hold a row of S. 2 * 208 + 88 = 3 * 168.
+constexpr int kRegsSoftmax = 208, kRegsOther = 88;
 constexpr int kKeys = 128;             // keys of a block
-constexpr int kStep = kKeys / kParts;  // keys of a step
+constexpr int kJobs = 3;               // tiles that the list warp is ahead
 constexpr int kBufs = 3;               // S buffers
 constexpr float kRaise = 8.f;          // the reference follows when a block's maximum is 2^8 above it
 constexpr float kFar = 2097152.f;      // 2^21: references that ex2_poly can add 1.5 * 2^23 to
@@ -67,8 +65,10 @@ template <int D, bool PAIR> struct Geom {
     static constexpr int kQBytes = kBoxes * 16384;                // 128 rows x D, boxes of 64 columns
     static constexpr int kBytes = kBoxes * 16384 / (PAIR ? 2 : 1);   // a CTA's share of a block's K, of its V
     static constexpr int kStages = 196608 / (2 * kBytes);         // of a K and a V each
-    static constexpr int kBars = 2 * kStages + 1 + (1 + 2 * kParts) * kBufs + 1 + 4 * kWgs + 4 + 1;
-    static constexpr size_t kSmem = (size_t)kQBytes + 2 * kStages * kBytes + 512 + 8 * kBars + 16 + 1024;
+    static constexpr int kBars = 2 * kStages + 2 + 3 * kBufs + 2 + 8 + 4 + 2 * kJobs + 1;
+    static constexpr size_t kUsed = (size_t)kQBytes + 2 * kStages * kBytes + 2048 + 8 * kBars + kJobs * 48 + 16;
+    static constexpr size_t kSlack = 512;                         // for a base that is no multiple of 1024
+    static constexpr size_t kSmem = kUsed + kSlack;
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -127,18 +127,18 @@ __device__ __forceinline__ float2 ex2_poly(float s0, float s1, float least, f2 c
                        __int_as_float(__float_as_int(v.y) + (__float_as_int(i.y) << 23)));
 }
 
-// p = 2^(s c + ref) of a step's scores of a row, rounded to T into the TMEM columns from `ts`; returns their
+// p = 2^(s c + ref) of 128 scores of a row, rounded to T into the TMEM columns from `ts`; returns their
 // sum. NPOLY of every 8 pairs go by polynomial, which shares the work between the exponential unit (4
 // lanes a cycle and scheduler: 1024 cycles a block, as long as its products) and the FMA pipes. The
 // sum's additions fill slots that the exponential unit leaves. A hidden score (-inf) has to give
 // exactly 0: masked steps use NPOLY 0.
 template <class T, int NPOLY>
-__device__ __forceinline__ float exp_step(const float* s, float c, float ref, uint32_t ts) {
+__device__ __forceinline__ float exp_block(const float* s, float c, float ref, uint32_t ts) {
     const f2 c2 = pack(c, c), ref2 = pack(ref, ref), lifted = add2(ref2, pack(12582912.f, 12582912.f));
     const float least = NPOLY ? __fdividef(-120.f - ref, c) : 0.f;
     f2 sum[2];
 #pragma unroll
-    for (int quarter = 0; quarter < kStep / 32; ++quarter) {
+    for (int quarter = 0; quarter < 4; ++quarter) {
         const float* v = s + quarter * 32;
         uint32_t w[16];
 #pragma unroll
@@ -180,70 +180,72 @@ template <int N> struct Ring {
     }
 };
 
+// A tile of the list: query rows of a set, a key head, a range of its key blocks. 12 words.
+struct Job {
+    int q0, nq, k0, nk;    // the set's rows
+    int first;             // the tile's first token, in the set
+    int blk0, n;           // key blocks
+    int kvh, split, end;   // end: the list is done
+    int pad[2];
+};
+
 template <class T, class O, int D, bool PAIR>
 __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorMap& kmap, const CUtensorMap& vmap,
                                         const TcArgs& p) {
     using G = Geom<D, PAIR>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ Item it_s;
-    __shared__ uint32_t scan[32];
     uint8_t* smem = smem_align1024(smem_raw);
     uint8_t* ring = smem + G::kQBytes;
-    float* s_ref = reinterpret_cast<float*>(ring + 2 * G::kStages * G::kBytes);       // [128] the rows' reference
-    uint64_t* bars = reinterpret_cast<uint64_t*>(s_ref + 128);
-    uint32_t* s_misc = reinterpret_cast<uint32_t*>(bars + G::kBars);             // [0] tmem, [1] abort
+    float* s_ref = reinterpret_cast<float*>(ring + 2 * G::kStages * G::kBytes);   // [2][128] the rows' reference, by tile
+    float* s_sum = s_ref + 256;                                                   // [2][128] the warpgroups' sums
+    uint64_t* bars = reinterpret_cast<uint64_t*>(s_sum + 256);
+    Job* s_job = reinterpret_cast<Job*>(bars + G::kBars);
+    uint32_t* s_misc = reinterpret_cast<uint32_t*>(s_job + kJobs);                // [0] tmem, [1] abort
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_misc + 1);
     const uint32_t b0 = smem_u32(bars);
     auto full = [&](uint32_t s) { return b0 + 8u * s; };
     auto empty = [&](uint32_t s) { return b0 + 8u * (G::kStages + s); };
-    const uint32_t bq = b0 + 8u * (2 * G::kStages);
-    auto sfull = [&](uint32_t s) { return bq + 8u * (1 + s); };
-    auto pfull = [&](uint32_t s, int part) { return bq + 8u * (1 + kBufs + kParts * s + part); };
-    auto pvdone = [&](uint32_t s, int part) { return bq + 8u * (1 + (1 + kParts) * kBufs + kParts * s + part); };
-    const uint32_t ofull = bq + 8u * (1 + (1 + 2 * kParts) * kBufs);
-    auto handed = [&](int wg, int q) { return ofull + 8u * (1 + 4 * wg + q); };  // the reference, to a warp
-    auto sums = [&](int q) { return ofull + 8u * (1 + 4 * kWgs + q); };          // the warpgroups' sums
-    const uint32_t drain = ofull + 8u * (5 + 4 * kWgs);
+    const uint32_t bq = b0 + 8u * (2 * G::kStages), qempty = bq + 8u;
+    auto sfull = [&](uint32_t s) { return bq + 8u * (2 + s); };
+    auto pfull = [&](uint32_t s) { return bq + 8u * (2 + kBufs + s); };
+    auto pvdone = [&](uint32_t s) { return bq + 8u * (2 + 2 * kBufs + s); };
+    const uint32_t ofull = bq + 8u * (2 + 3 * kBufs), oempty = ofull + 8u;
+    auto handed = [&](int wg, int q) { return ofull + 8u * (2 + 4 * wg + q); };   // the reference, to a warp
+    auto sums = [&](int q) { return ofull + 8u * (10 + q); };
+    auto jfull = [&](uint32_t s) { return ofull + 8u * (14 + s); };
+    auto jempty = [&](uint32_t s) { return ofull + 8u * (14 + kJobs + s); };
+    const uint32_t drain = ofull + 8u * (14 + 2 * kJobs);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const AttnArgs& a = p.a;
     const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
     const bool leader = rank == 0;
+    if ((size_t)(smem - smem_raw) > G::kSlack) {
+        if (threadIdx.x == 0) atomicCAS(a.err, 0, TB_DEVERR_WAIT_TIMEOUT);
+        return;                            // both CTAs of a pair
+    }
 
-    uint32_t idx = PAIR ? cluster_id_x() : blockIdx.x;
-    const int split = idx % p.nsplit;
-    idx /= p.nsplit;
-    const int kvh = idx % a.kv_heads;
-    find_item(a.q_off, a.nset, a.nq, a.unit, idx / a.kv_heads, a.err, &it_s, scan);
-    if (it_s.set < 0) return;              // both CTAs of a pair
-    int64_t k0, k1;
-    set_range(a.k_off, it_s.set, a.nk, k0, k1, a.err);
-    const int64_t q0 = it_s.lo;
-    const int nq = (int)(it_s.hi - it_s.lo), nk = (int)(k1 - k0);
-    // causal: the last rows of a set see the most keys; they go first
-    const int first = (a.causal ? (int)(it_s.items - 1 - it_s.item) : (int)it_s.item) * a.unit;
-    const int t0 = first + (int)rank * p.tile_tokens;                            // the CTA's first token, in the set
-    const int end = a.causal ? max(0, min(nk, min(first + a.unit, nq) + nk - nq)) : nk;
-    const int all = (end + kKeys - 1) / kKeys;
-    const int blk0 = (int)((int64_t)all * split / p.nsplit), n = (int)((int64_t)all * (split + 1) / p.nsplit) - blk0;
-
-    if (threadIdx.x < 128) s_ref[threadIdx.x] = -INFINITY;
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < G::kStages; ++s) {
             mbar_init(full(s), PAIR && leader ? 2 : 1);         // its own TMA and the odd CTA's, passed on
             mbar_init(empty(s), 1);
         }
         mbar_init(bq, 1);
+        mbar_init(qempty, 1);
         for (uint32_t s = 0; s < kBufs; ++s) {
             mbar_init(sfull(s), 1);
-            for (int part = 0; part < kParts; ++part) {
-                mbar_init(pfull(s, part), PAIR ? 8 : 4);        // the warps of both CTAs, at the even one
-                mbar_init(pvdone(s, part), 1);
-            }
+            mbar_init(pfull(s), PAIR ? 8 : 4);                  // the warps of both CTAs, at the even one
+            mbar_init(pvdone(s), 1);
         }
         mbar_init(ofull, 1);
+        mbar_init(oempty, PAIR ? 16 : 8);
         for (int q = 0; q < 4; ++q) {
-            for (int wg = 0; wg < kWgs; ++wg) mbar_init(handed(wg, q), 1);
-            mbar_init(sums(q), kWgs);
+            mbar_init(handed(0, q), 1);
+            mbar_init(handed(1, q), 1);
+            mbar_init(sums(q), 2);
+        }
+        for (uint32_t s = 0; s < kJobs; ++s) {
+            mbar_init(jfull(s), 1);
+            mbar_init(jempty(s), 10);                           // softmax warps, products, TMA
         }
         mbar_init(drain, 1);
         s_misc[1] = 0;
@@ -266,48 +268,136 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
     tc_fence_after();
     const uint32_t tmem = s_misc[0], tmem_o = tmem + kBufs * 128u;
     const uint32_t sq = smem_u32(smem), skv = sq + G::kQBytes;
-    // The ring's item j holds the K of block j and the V of block j - lag: what the products of one round,
-    // P V of a block and the S three blocks on, read. One barrier to wait for, one to free.
-    const int lag = min(n, kBufs), items = n + lag;
 
-    if (warp >= kMma) {
+    Ring<kJobs> jr;
+    // the next tile of the list; false at its end
+    auto next_job = [&](Job& j) {
+        if (!__all_sync(0xffffffffu, mbar_wait(jfull(jr.at), jr.round, s_abort, a.err))) return false;
+        const int4* src = reinterpret_cast<const int4*>(s_job + jr.at);
+        const int4 x = src[0], y = src[1], z = src[2];
+        j.q0 = x.x; j.nq = x.y; j.k0 = x.z; j.nk = x.w;
+        j.first = y.x; j.blk0 = y.y; j.n = y.z; j.kvh = y.w;
+        j.split = z.x; j.end = z.y;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(jempty(jr.at));
+        jr.step();
+        return j.end == 0;
+    };
+
+    if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsOther));
+        bool ok = true;
+        auto wait = [&](uint32_t bar, uint32_t par) {
+            if (ok) ok = __all_sync(0xffffffffu, wait_bar<PAIR>(bar, par, s_abort, a.err));
+            return ok;
+        };
         // The rows of V behind the set's last key belong to others and may hold no numbers, which a p
         // of 0 would not cancel: those of the last 16 that the products read become 0.
-        const int tail = nk - (blk0 + n - 1) * kKeys;          // keys of the last block
-        const bool dirty = n > 0 && tail < kKeys && (tail & 15);
-        auto clean = [&]() {
+        auto clean = [&](uint32_t st, int keys) {
             constexpr int per = G::kBytes / kKeys / 16;         // 16-byte words of a key's row
-            uint8_t* v = ring + ((items - 1) % G::kStages) * (2 * G::kBytes) + G::kBytes;
-            for (int w = lane; w < (16 - (tail & 15)) * per; w += 32) {
-                const int row = tail + w / per, x = w % per;
+            uint8_t* v = ring + st * (2 * G::kBytes) + G::kBytes;
+            for (int w = lane; w < (16 - (keys & 15)) * per; w += 32) {
+                const int row = keys + w / per, x = w % per;
                 *reinterpret_cast<uint4*>(v + (x >> 3) * 16384 + row * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();
             __syncwarp();
         };
-        if (warp == kTma) {
-            // -------------------------------------------------------------- TMA producer
-            if (n > 0 && elect_one()) {
-                mbar_arrive_expect_tx(bq, p.q_bytes);
-                for (int b = 0; b < G::kBoxes; ++b)
-                    tma_load_3d(sq + b * 16384, &qmap, b * 64, kvh * a.group, (int)(q0 + t0), bq);
-                Ring<G::kStages> r;
-                for (int j = 0; j < items; ++j, r.step()) {
-                    if (j >= G::kStages && !wait_bar<PAIR>(empty(r.at), r.round ^ 1, s_abort, a.err)) break;
-                    const uint32_t k_at = skv + r.at * (2 * G::kBytes), v_at = k_at + G::kBytes;
-                    mbar_arrive_expect_tx(full(r.at), j < n && j >= lag ? 2 * G::kBytes : G::kBytes);
-                    const int key = (int)k0 + (blk0 + j) * kKeys;
-                    if (j < n)
-                        for (int x = 0; x < G::kBoxes; ++x)
-                            tma_load_3d(k_at + x * (PAIR ? 8192 : 16384), &kmap, x * 64, kvh, key + (PAIR ? (int)rank * 64 : 0),
-                                        full(r.at));
-                    if (j >= lag)
-                        for (int x = 0; x < (PAIR ? 1 : G::kBoxes); ++x)
-                            tma_load_3d(v_at + x * 16384, &vmap, (PAIR ? (int)rank : x) * 64, kvh, key - lag * kKeys, full(r.at));
+        // A tile's items of the ring: item j holds the K of its block j and the V of block j - lag, what the
+        // products of one round read. One barrier to wait for, one to free.
+        Job j;
+        if (warp == kList) {
+            // -------------------------------------------------------------- the list
+            // Tiles in the order set, piece of the set, key head, range of keys; CTA c of N takes c, 2N-1-c,
+            // 2N+c, ...: there and back, so that none has the longer ones (causal: a set's last pieces,
+            // which see the most keys, come first) every time. A lane holds one of 32 sets.
+            const uint32_t c = PAIR ? cluster_id_x() : blockIdx.x, nc = PAIR ? nclusters_x() : gridDim.x;
+            int set0 = -32;
+            uint32_t base = 0, total = 0, inc = 0, cnt = 0;
+            int64_t qlo = 0, qhi = 0, klo = 0, khi = 0;
+            for (uint32_t k = 0;; ++k) {
+                uint32_t idx = k * nc + (k & 1 ? nc - 1 - c : c);
+                const int split = idx % p.nsplit;
+                idx /= p.nsplit;
+                const int kvh = idx % a.kv_heads;
+                const uint32_t piece = idx / a.kv_heads;
+                while (piece >= base + total && set0 + 32 < a.nset) {
+                    base += total;
+                    set0 += 32;
+                    cnt = 0;
+                    if (set0 + lane < a.nset) {
+                        set_range(a.q_off, set0 + lane, a.nq, qlo, qhi, a.err);
+                        set_range(a.k_off, set0 + lane, a.nk, klo, khi, a.err);
+                        cnt = (uint32_t)((qhi - qlo + a.unit - 1) / a.unit);
+                    }
+                    inc = cnt;
+#pragma unroll
+                    for (int d = 1; d < 32; d *= 2) {
+                        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, d);
+                        if (lane >= d) inc += v;
+                    }
+                    total = __shfl_sync(0xffffffffu, inc, 31);
                 }
+                const bool found = piece < base + total;
+                const int src = found ? __ffs(__ballot_sync(0xffffffffu, base + inc > piece)) - 1 : 0;
+                const uint32_t cs = __shfl_sync(0xffffffffu, cnt, src), at = piece - base - (__shfl_sync(0xffffffffu, inc, src) - cs);
+                Job o;
+                o.q0 = (int)__shfl_sync(0xffffffffu, qlo, src);
+                o.nq = (int)__shfl_sync(0xffffffffu, qhi, src) - o.q0;
+                o.k0 = (int)__shfl_sync(0xffffffffu, klo, src);
+                o.nk = (int)__shfl_sync(0xffffffffu, khi, src) - o.k0;
+                o.first = (int)(a.causal ? cs - 1 - at : at) * a.unit;
+                const int end = a.causal ? max(0, min(o.nk, min(o.first + a.unit, o.nq) + o.nk - o.nq)) : o.nk;
+                const int all = (end + kKeys - 1) / kKeys;
+                o.blk0 = (int)((int64_t)all * split / p.nsplit);
+                o.n = (int)((int64_t)all * (split + 1) / p.nsplit) - o.blk0;
+                o.kvh = kvh;
+                o.split = split;
+                o.end = found ? 0 : 1;
+                if (k >= kJobs && !__all_sync(0xffffffffu, mbar_wait(jempty(jr.at), jr.round ^ 1, s_abort, a.err))) break;
+                if (lane == 0) {
+                    int4* dst = reinterpret_cast<int4*>(s_job + jr.at);
+                    dst[0] = make_int4(o.q0, o.nq, o.k0, o.nk);
+                    dst[1] = make_int4(o.first, o.blk0, o.n, o.kvh);
+                    dst[2] = make_int4(o.split, o.end, 0, 0);
+                    mbar_arrive(jfull(jr.at));
+                }
+                __syncwarp();
+                jr.step();
+                if (!found) break;
             }
-            __syncwarp();
+        } else if (warp == kTma) {
+            // -------------------------------------------------------------- TMA producer
+            Ring<G::kStages> r;
+            uint32_t used = 0, tiles = 0;
+            while (ok && next_job(j)) {
+                if (j.n == 0) continue;
+                const int lag = min(j.n, kBufs), items = j.n + lag;
+                if (tiles && !wait(qempty, (tiles - 1) & 1)) break;
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(bq, p.q_bytes);
+                    for (int b = 0; b < G::kBoxes; ++b)
+                        tma_load_3d(sq + b * 16384, &qmap, b * 64, j.kvh * a.group, j.q0 + j.first + (int)rank * p.tile_tokens, bq);
+                }
+                __syncwarp();
+                for (int i = 0; i < items; ++i, r.step(), ++used) {
+                    if (used >= G::kStages && !wait(empty(r.at), r.round ^ 1)) break;
+                    if (elect_one()) {
+                        const uint32_t k_at = skv + r.at * (2 * G::kBytes), v_at = k_at + G::kBytes;
+                        mbar_arrive_expect_tx(full(r.at), i < j.n && i >= lag ? 2 * G::kBytes : G::kBytes);
+                        const int key = j.k0 + (j.blk0 + i) * kKeys;
+                        if (i < j.n)
+                            for (int x = 0; x < G::kBoxes; ++x)
+                                tma_load_3d(k_at + x * (PAIR ? 8192 : 16384), &kmap, x * 64, j.kvh,
+                                            key + (PAIR ? (int)rank * 64 : 0), full(r.at));
+                        if (i >= lag)
+                            for (int x = 0; x < (PAIR ? 1 : G::kBoxes); ++x)
+                                tma_load_3d(v_at + x * 16384, &vmap, (PAIR ? (int)rank : x) * 64, j.kvh, key - lag * kKeys, full(r.at));
+                    }
+                    __syncwarp();
+                }
+                ++tiles;
+            }
         } else if (warp == kMma && leader) {
             // -------------------------------------------------------------- the products
             // One warp issues both: a block's P V and, into the buffer that it frees, the S three blocks on.
@@ -322,15 +412,11 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
             const uint32_t qlo = (sq >> 4) | (1u << 16), klo = (skv >> 4) | (1u << 16);
             const uint32_t vlo = ((skv + G::kBytes) >> 4) | (1024u << 16);
             const int dim = a.dim;
-            bool ok = n > 0;
-            auto wait = [&](uint32_t bar, uint32_t par) {
-                if (ok) ok = __all_sync(0xffffffffu, wait_bar<PAIR>(bar, par, s_abort, a.err));
-                return ok;
-            };
             Ring<G::kStages> r;
-            Ring<kBufs> u;
-            auto mma_s = [&](uint32_t buf) {         // by the elected thread
-                const uint32_t kl = klo + r.at * (2 * G::kBytes >> 4), td = tmem + buf * 128;
+            Ring<kBufs> u, us;                       // P V's and S's buffers
+            uint32_t tiles = 0;
+            auto mma_s = [&](bool last) {            // by the elected thread
+                const uint32_t kl = klo + r.at * (2 * G::kBytes >> 4), td = tmem + us.at * 128;
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     const uint64_t qd = (uint64_t)kHi << 32 | (qlo + (k >> 2) * 1024 + (k & 3) * 2);
@@ -340,47 +426,51 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                         else tc_mma(td, qd, kd, p.idesc_s, k ? 1u : 0u);
                     }
                 }
-                commit<PAIR>(sfull(buf));
+                commit<PAIR>(sfull(us.at));
+                if (last) commit<PAIR>(qempty);
             };
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bq, 0, s_abort, a.err));
-            for (uint32_t b = 0; (int)b < lag && ok; ++b, r.step()) {
-                if (!wait(full(r.at), r.round)) break;
-                tc_fence_after();
-                if (elect_one()) {
-                    mma_s(b);
-                    commit<PAIR>(empty(r.at));
-                }
-                __syncwarp();
-            }
-            int keys = nk - blk0 * kKeys;
-            for (int b = 0; b < n && ok; ++b, r.step(), u.step(), keys -= kKeys) {
-                if (!wait(full(r.at), r.round)) break;
-                if (b == n - 1 && dirty) clean();
-                const uint32_t vl = vlo + r.at * (2 * G::kBytes >> 4);
-#pragma unroll
-                for (int part = 0; part < kParts; ++part) {
-                    if (!wait(pfull(u.at, part), u.round)) break;
+            while (ok && next_job(j)) {
+                const int n = j.n;
+                if (n == 0) continue;
+                const int lag = min(n, kBufs);
+                ok = __all_sync(0xffffffffu, mbar_wait(bq, tiles & 1, s_abort, a.err));
+                for (int b = 0; b < lag && ok; ++b, r.step(), us.step()) {
+                    if (!wait(full(r.at), r.round)) break;
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint32_t pa = tmem + u.at * 128 + part * kStep;
-#pragma unroll
-                        for (int k = part * (kStep / 16); k < (part + 1) * (kStep / 16); ++k) {
-                            const uint64_t vd = (uint64_t)kHi << 32 | (vl + k * 128);
-                            const uint32_t ap = pa + (k % (kStep / 16)) * 8;
-                            if (k * 16 < keys) {
-                                if (PAIR) tc_mma_ts_pair(tmem_o, ap, vd, p.idesc_o, b || k ? 1u : 0u);
-                                else tc_mma_ts(tmem_o, ap, vd, p.idesc_o, b || k ? 1u : 0u);
-                            }
-                        }
-                        commit<PAIR>(pvdone(u.at, part));
-                        if (part == kParts - 1) {
-                            if (b + lag < n) mma_s(u.at);
-                            commit<PAIR>(empty(r.at));
-                            if (b == n - 1) commit<PAIR>(ofull);
-                        }
+                        mma_s(b == n - 1);
+                        commit<PAIR>(empty(r.at));
                     }
                     __syncwarp();
                 }
+                int keys = j.nk - j.blk0 * kKeys;
+                for (int b = 0; b < n && ok; ++b, r.step(), u.step(), keys -= kKeys) {
+                    if (!wait(full(r.at), r.round)) break;
+                    if (keys < kKeys && (keys & 15)) clean(r.at, keys);
+                    // the last tile's O has been read
+                    if (b == 0 && tiles && !wait(oempty, (tiles - 1) & 1)) break;
+                    if (!wait(pfull(u.at), u.round)) break;
+                    tc_fence_after();
+                    const bool more = b + lag < n;
+                    if (elect_one()) {
+                        const uint32_t vl = vlo + r.at * (2 * G::kBytes >> 4), pa = tmem + u.at * 128;
+#pragma unroll
+                        for (int k = 0; k < kKeys / 16; ++k) {
+                            const uint64_t vd = (uint64_t)kHi << 32 | (vl + k * 128);
+                            if (k * 16 < keys) {
+                                if (PAIR) tc_mma_ts_pair(tmem_o, pa + k * 8, vd, p.idesc_o, b || k ? 1u : 0u);
+                                else tc_mma_ts(tmem_o, pa + k * 8, vd, p.idesc_o, b || k ? 1u : 0u);
+                            }
+                        }
+                        commit<PAIR>(pvdone(u.at));
+                        if (more) mma_s(b + lag == n - 1);
+                        commit<PAIR>(empty(r.at));
+                        if (b == n - 1) commit<PAIR>(ofull);
+                    }
+                    __syncwarp();
+                    if (more) us.step();
+                }
+                ++tiles;
             }
             // every MMA has completed before the TMEM is freed (also after an abort)
             if (elect_one()) PAIR ? tc_commit_pair(drain, 0x1) : tc_commit(drain);
@@ -388,158 +478,170 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
         } else if (PAIR && !leader && warp == kMma) {
             // -------------------------------------------------------------- odd CTA: what has landed, passed on
             Ring<G::kStages> r;
-            bool ok = n > 0 && __all_sync(0xffffffffu, mbar_wait(bq, 0, s_abort, a.err));
-            for (int j = 0; j < items && ok; ++j, r.step()) {
-                ok = __all_sync(0xffffffffu, mbar_wait(full(r.at), r.round, s_abort, a.err));
-                if (!ok) break;
-                const bool last = j == items - 1 && dirty;
-                if (last) clean();
-                if (lane == 0) {
-                    if (last) mbar_arrive_cluster(full(r.at), 0);               // its zeros before the products
-                    else mbar_arrive_cluster_relaxed(full(r.at), 0);
+            uint32_t tiles = 0;
+            while (ok && next_job(j)) {
+                if (j.n == 0) continue;
+                const int lag = min(j.n, kBufs), items = j.n + lag, tail = j.nk - (j.blk0 + j.n - 1) * kKeys;
+                ok = __all_sync(0xffffffffu, mbar_wait(bq, tiles & 1, s_abort, a.err));
+                for (int i = 0; i < items && ok; ++i, r.step()) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(full(r.at), r.round, s_abort, a.err));
+                    if (!ok) break;
+                    const bool dirty = i == items - 1 && tail < kKeys && (tail & 15);
+                    if (dirty) clean(r.at, tail);
+                    if (lane == 0) {
+                        if (dirty) mbar_arrive_cluster(full(r.at), 0);          // its zeros before the products
+                        else mbar_arrive_cluster_relaxed(full(r.at), 0);
+                    }
                 }
+                ++tiles;
             }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kRegsSoftmax));
         // ------------------------------------------------------------------ softmax and output
-        // Warpgroup wg takes part wg % kParts of every other block.
-        const int wg = warp >> 2, quad = warp & 3, r = quad * 32 + lane, part = wg % kParts;
-        const int t = t0 + r / a.group, h = kvh * a.group + r % a.group;
-        const bool valid = r < p.tile_tokens * a.group && t < nq;
-        const int lim = !valid ? nk : a.causal ? max(0, min(nk, t + 1 + nk - nq)) : nk;     // keys the row sees
-        const int wlim = __reduce_min_sync(0xffffffffu, lim);
+        // The warpgroups take turns over the blocks of all tiles.
+        const int wg = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
         const uint32_t lane_base = (uint32_t)(quad * 32) << 16, to = tmem_o + lane_base;
         const float c = a.scale_log2;
         // p in f16 starts at 2^7 instead of 1 (2^15 after the largest rise): small p keep their digits
         constexpr float lift = std::is_same<T, __half>::value ? 7.f : 0.f;
-        float ref = -INFINITY, l = 0.f;              // of the warpgroup's own steps; -inf: no key so far
-        float shift = lift;                          // what scores are shifted by: lift - ref
-        bool ok = true, far = false;
         Ring<kBufs> u;
-        if (wg >= kParts) u.step();
-        uint32_t mine = wg == 0 ? 1 : 0;             // parity of the reference's next hand-off
-        for (int b = wg / kParts; b < n; b += 2, mine ^= 1) {
-            const uint32_t ts = tmem + u.at * 128u + part * kStep + lane_base;
-            if (!__all_sync(0xffffffffu, wait_bar<PAIR>(sfull(u.at), u.round, s_abort, a.err))) { ok = false; break; }
-            tc_fence_after();
-            float s[kStep];
+        uint32_t tiles = 0, blocks = 0, turns = 0;   // tiles with keys, blocks of all tiles, hand-offs received
+        bool ok = true;
+        Job j;
+        while (ok && next_job(j)) {
+            const int t = j.first + (int)rank * p.tile_tokens + r / a.group, h = j.kvh * a.group + r % a.group;
+            const bool valid = r < p.tile_tokens * a.group && t < j.nq;
+            const int lim = !valid ? j.nk : a.causal ? max(0, min(j.nk, t + 1 + j.nk - j.nq)) : j.nk;  // keys the row sees
+            const int wlim = __reduce_min_sync(0xffffffffu, lim), n = j.n;
+            float* refs = s_ref + (tiles & 1) * 128;
+            float ref = -INFINITY, l = 0.f;          // of the warpgroup's own blocks; -inf: no key so far
+            float shift = lift;                      // what scores are shifted by: lift - ref
+            bool far = false;
+            for (int b = 0; b < n; ++b, ++blocks, u.step()) {
+                if ((int)(blocks & 1) != wg) continue;
+                const uint32_t ts = tmem + u.at * 128u + lane_base;
+                if (!__all_sync(0xffffffffu, wait_bar<PAIR>(sfull(u.at), u.round, s_abort, a.err))) { ok = false; break; }
+                tc_fence_after();
+                float s[kKeys];
 #pragma unroll
-            for (int q = 0; q < kStep; q += 32) tmem_ld_x32(ts + q, s + q);
-            tmem_wait_ld();
-            const int key0 = (blk0 + b) * kKeys + part * kStep;
-            const bool masked = wlim < key0 + kStep;
-            if (masked) {
-                const int left = lim - key0;
-#pragma unroll
-                for (int q = 0; q < kStep; ++q) s[q] = q < left ? s[q] : -INFINITY;
-            }
-            float mx[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = max3(s[e], s[e + 4], s[e + 8]);
-#pragma unroll
-            for (int q = 12; q < kStep - 4; q += 8) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[q + e], s[q + 4 + e]);
-            }
-            const float top = max3(max3(mx[0], mx[1], s[kStep - 4]), max3(mx[2], mx[3], s[kStep - 3]), max2(s[kStep - 2], s[kStep - 1])) * c;
-            // The reference after the step before, from the warpgroup before. Only the comparison stands between
-            // two hand-offs: with the loads and the maximum in between they came 1000 cycles apart.
-            float now = -INFINITY;
-            if (b > 0 || wg > 0) {
-                if (!__all_sync(0xffffffffu, mbar_wait(handed(wg, quad), mine, s_abort, a.err))) { ok = false; break; }
-                now = s_ref[r];
-            }
-            const bool raise = !(top - now <= kRaise) && !(top == -INFINITY && now == -INFINITY);
-            if (far || __any_sync(0xffffffffu, raise || now != ref)) {
-                const float next = raise ? rintf(top) : now;
-                s_ref[r] = next;
-                if ((b > 0 || part) && __any_sync(0xffffffffu, raise)) {
-                    // O is at rest once the step before has been added
-                    const uint32_t before = part ? u.at : u.at ? u.at - 1 : kBufs - 1, par = part || u.at ? u.round : u.round ^ 1;
-                    if (!__all_sync(0xffffffffu, wait_bar<PAIR>(pvdone(before, part ? part - 1 : kParts - 1), par, s_abort, a.err))) { ok = false; break; }
-                    tc_fence_after();
-                    const float al = raise ? ex2(now - next) : 1.f;
-#pragma unroll 1
-                    for (int q = 0; q < D; q += 32) {
-                        float o[32];
-                        tmem_ld_x32(to + q, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] *= al;
-                        tmem_st_x32(to + q, reinterpret_cast<const uint32_t*>(o));
-                    }
+                for (int q = 0; q < kKeys; q += 32) tmem_ld_x32(ts + q, s + q);
+                // meanwhile: the reference after the block before, from the other warpgroup
+                float now = -INFINITY;
+                if (blocks > 0) {
+                    if (!__all_sync(0xffffffffu, mbar_wait(handed(wg, quad), turns & 1, s_abort, a.err))) { ok = false; break; }
+                    ++turns;
+                    if (b > 0) now = refs[r];
                 }
-                __syncwarp();                        // s_ref before the hand-off
-                l = next == ref ? l : l * ex2(ref - next);
-                ref = next;
-                shift = lift - (ref == -INFINITY ? 0.f : ref);
-                far = __any_sync(0xffffffffu, !(fabsf(ref) < kFar) && ref != -INFINITY);
-            }
-            if (lane == 0) mbar_arrive(handed((wg + 1) % kWgs, quad));
-            l += masked || far ? exp_step<T, 0>(s, c, shift, ts) : exp_step<T, kPoly>(s, c, shift, ts);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if (PAIR) mbar_arrive_cluster_relaxed(pfull(u.at, part), 0);
-                else mbar_arrive(pfull(u.at, part));
-            }
-            u.step();
-            u.step();
-        }
-        if (n > 0 && ok) {
-            ok = __all_sync(0xffffffffu, wait_bar<PAIR>(ofull, 0, s_abort, a.err));
-            tc_fence_after();
-        }
-        float total = 0.f;
-        if (n > 0 && ok) {
-            // all warpgroups' sums against the last reference, through Q's place (its products are done)
-            float2* s_sum = reinterpret_cast<float2*>(smem);
-            s_sum[wg * 128 + r] = make_float2(l, ref);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(sums(quad));
-            ok = __all_sync(0xffffffffu, mbar_wait(sums(quad), 0, s_abort, a.err));
-            ref = s_ref[r];
+                tmem_wait_ld();
+                const int key0 = (j.blk0 + b) * kKeys;
+                const bool masked = wlim < key0 + kKeys;
+                if (masked) {
+                    const int left = lim - key0;
 #pragma unroll
-            for (int w = 0; w < kWgs; ++w) {
-                const float2 x = s_sum[w * 128 + r];
-                total += x.y == ref ? x.x : x.y == -INFINITY ? 0.f : x.x * ex2(x.y - ref);
+                    for (int q = 0; q < kKeys; ++q) s[q] = q < left ? s[q] : -INFINITY;
+                }
+                float mx[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx[e] = max3(s[e], s[e + 4], s[e + 8]);
+#pragma unroll
+                for (int q = 12; q < kKeys - 4; q += 8) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[q + e], s[q + 4 + e]);
+                }
+                const float top = max3(max3(mx[0], mx[1], s[kKeys - 4]), max3(mx[2], mx[3], s[kKeys - 3]),
+                                       max2(s[kKeys - 2], s[kKeys - 1])) * c;
+                const bool raise = !(top - now <= kRaise) && !(top == -INFINITY && now == -INFINITY);
+                if (b == 0 || far || __any_sync(0xffffffffu, raise || now != ref)) {
+                    const float next = raise ? rintf(top) : now;
+                    refs[r] = next;
+                    if (b > 0 && __any_sync(0xffffffffu, raise)) {
+                        // O is at rest once the block before has been added
+                        const uint32_t before = u.at ? u.at - 1 : kBufs - 1, par = u.at ? u.round : u.round ^ 1;
+                        if (!__all_sync(0xffffffffu, wait_bar<PAIR>(pvdone(before), par, s_abort, a.err))) { ok = false; break; }
+                        tc_fence_after();
+                        const float al = raise ? ex2(now - next) : 1.f;
+#pragma unroll 1
+                        for (int q = 0; q < D; q += 32) {
+                            float o[32];
+                            tmem_ld_x32(to + q, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] *= al;
+                            tmem_st_x32(to + q, reinterpret_cast<const uint32_t*>(o));
+                        }
+                    }
+                    __syncwarp();                    // the references before the hand-off
+                    l = next == ref ? l : l * ex2(ref - next);
+                    ref = next;
+                    shift = lift - (ref == -INFINITY ? 0.f : ref);
+                    far = __any_sync(0xffffffffu, !(fabsf(ref) < kFar) && ref != -INFINITY);
+                }
+                if (lane == 0) mbar_arrive(handed(1 - wg, quad));
+                l += masked || far ? exp_block<T, 0>(s, c, shift, ts) : exp_block<T, kPoly>(s, c, shift, ts);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (PAIR) mbar_arrive_cluster_relaxed(pfull(u.at), 0);
+                    else mbar_arrive(pfull(u.at));
+                }
             }
-        }
-        if (ok) {
-            const bool none = n == 0 || lim <= blk0 * kKeys;       // the row sees no key here
+            float total = 0.f;
+            if (n > 0 && ok) {
+                ok = __all_sync(0xffffffffu, wait_bar<PAIR>(ofull, tiles & 1, s_abort, a.err));
+                tc_fence_after();
+                // both warpgroups' sums against the last reference
+                const float last = refs[r];
+                s_sum[wg * 128 + r] = ref == last ? l : ref == -INFINITY ? 0.f : l * ex2(ref - last);
+                ref = last;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sums(quad));
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(sums(quad), tiles & 1, s_abort, a.err));
+                total = s_sum[r] + s_sum[128 + r];
+            }
+            if (!ok) break;
+            const bool none = n == 0 || lim <= j.blk0 * kKeys;     // the row sees no key here
             const float inv = none ? 0.f : 1.f / total;
             const float lg = none ? -INFINITY : ref - lift + log2f(total);
-            const int64_t row = q0 + t;
-            const int64_t at = ((int64_t)split * a.nq + row) * a.heads + h;
+            const int64_t row = (int64_t)j.q0 + t;
+            const int64_t at = ((int64_t)j.split * a.nq + row) * a.heads + h;
             if (valid && wg == 0) {
                 if (p.part) p.part_lse[at] = lg;
                 else if (a.lse) a.lse[row * a.heads + h] = lg * 0.69314718055994530942f;
             }
-            float* part_row = p.part + at * a.dim;
+            float* part = p.part + at * a.dim;
             O* out = reinterpret_cast<O*>(a.out) + row * a.out_row + (int64_t)h * a.out_head;
-            // each warpgroup writes its share of the head's columns
-            constexpr int W = D / kWgs;
-#pragma unroll
-            for (int w = 0; w < W; w += 16) {
+            // each warpgroup writes half of the head's columns
+            constexpr int W = D / 2;
+#pragma unroll 1
+            for (int w = 0; w < W; w += 32) {
                 const int q = wg * W + w;
-                float o[16];
+                float o[32];
                 __syncwarp();
                 if (n > 0) {
-                    tmem_ld_x16(to + q, o);
+                    tmem_ld_x32(to + q, o);
                     tmem_wait_ld();
+                    if (w + 32 >= W) {               // O may be written again
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (PAIR) mbar_arrive_cluster_relaxed(oempty, 0);
+                            else mbar_arrive(oempty);
+                        }
+                    }
                 }
                 if (!valid || (p.part && none)) continue;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = none ? 0.f : o[e] * inv;
+                for (int e = 0; e < 32; ++e) o[e] = none ? 0.f : o[e] * inv;
 #pragma unroll
-                for (int e = 0; e < 16; e += 8)
+                for (int e = 0; e < 32; e += 8)
                     if (q + e < a.dim) {
-                        if (p.part) store8<float>(part_row + q + e, o + e);
+                        if (p.part) store8<float>(part + q + e, o + e);
                         else store8<O>(out + q + e, o + e);
                     }
             }
+            if (n > 0) ++tiles;
         }
         tc_fence_before();
     }
@@ -548,7 +650,7 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
         const long long w0 = clock64();
         while (!mbar_try_wait(drain, 0) && clock64() - w0 < kWaitCycles) { }
     }
-    if (*s_abort && threadIdx.x == 0 && n > 0) {
+    if (*s_abort && threadIdx.x == 0) {
         // after an abort: wait out the loads that may still be in flight
         const long long w0 = clock64();
         while (clock64() - w0 < 20000000) { }
@@ -626,7 +728,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ TcArg
 struct Plan {
     bool pair;
     int tile_tokens, unit, nsplit;
-    int64_t items;                     // CTAs, or pairs of them
+    int64_t items;                     // tiles, at most
 };
 
 // Pairs for wide heads where an average set's rows fill more than one CTA. Keys are cut where the CTAs
@@ -674,9 +776,11 @@ tb_status launch(tb_ctx* ctx, const TcArgs& p, const Plan& l, const CUtensorMap&
                                 : wide ? (const void*)k_attn_tc<T, O, 128> : (const void*)k_attn_tc<T, O, 64>;
     if (sm > (size_t)ctx->max_smem_optin) return tb_fail(ctx, TB_ERR_UNSUPPORTED, "tb_attention: shared memory too small");
     TB_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
-    if (l.pair) k_attn_pair<T, O><<<(unsigned)(2 * l.items), kThreads, sm, ctx->stream>>>(qm, km, vm, p);
-    else if (wide) k_attn_tc<T, O, 128><<<(unsigned)l.items, kThreads, sm, ctx->stream>>>(qm, km, vm, p);
-    else k_attn_tc<T, O, 64><<<(unsigned)l.items, kThreads, sm, ctx->stream>>>(qm, km, vm, p);
+    const unsigned grid = l.pair ? 2u * (unsigned)std::min<int64_t>(l.items, ctx->num_sms / 2)
+                                 : (unsigned)std::min<int64_t>(l.items, ctx->num_sms);
+    if (l.pair) k_attn_pair<T, O><<<grid, kThreads, sm, ctx->stream>>>(qm, km, vm, p);
+    else if (wide) k_attn_tc<T, O, 128><<<grid, kThreads, sm, ctx->stream>>>(qm, km, vm, p);
+    else k_attn_tc<T, O, 64><<<grid, kThreads, sm, ctx->stream>>>(qm, km, vm, p);
     TB_LAUNCH_CHECK(ctx, "k_attn_tc");
     if (p.part) {
         k_attn_join<O><<<(unsigned)((p.a.nq * p.a.heads + 7) / 8), 256, 0, ctx->stream>>>(p, l.nsplit);
