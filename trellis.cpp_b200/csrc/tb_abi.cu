@@ -126,6 +126,7 @@ tb_status tb_ctx_check_device(tb_ctx* ctx) {
         const char* what = h == TB_DEVERR_HASH_PROBE ? "hash probe bound exceeded"
                          : h == TB_DEVERR_WAIT_TIMEOUT ? "bounded mbarrier wait timed out in the conv kernel"
                          : h == TB_DEVERR_TMEM_ALLOC ? "TMEM allocation failed"
+                         : h == TB_DEVERR_SMEM_BASE ? "shared memory is not aligned for the attention kernel"
                          : h == TB_DEVERR_BAD_OFFSETS ? "an offset table of packed sets descends or leaves the array"
                          : "unknown device error";
         return tb_fail(ctx, TB_ERR_DEVICE, what);

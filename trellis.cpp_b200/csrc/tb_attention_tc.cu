@@ -19,9 +19,10 @@
 // The warpgroups hand it on from block to block through shared memory; the one that raises it waits
 // until the block before has been added and scales O.
 //
-// The grid is what fits the GPU; each CTA (pair) works through its share of the list of tiles, so the next
-// tile's loads and first products run while the last one's softmax and output finish (a launch of
-// one CTA a tile paid some 4 us a tile for them). One warp finds the tiles in the tables of sets.
+// The launch has a CTA (pair) for each tile, but those that run take over tiles that have not started
+// (clusterlaunchcontrol), so the next tile's loads and first products run while the last one's softmax
+// and output finish (a CTA a tile paid some 4 us for them) and no SM idles while others have work
+// left. One warp finds the tiles in the tables of sets.
 //
 // With few CTAs the keys are cut into `nsplit` ranges, which leave partial rows (32 bits, normalised,
 // with their log sums) that k_attn_join adds up in a fixed order.
@@ -40,23 +41,18 @@ using namespace tbpk;
 constexpr int kThreads = 384;
 constexpr int kMma = 8, kTma = 9, kList = 10;      // warps 0-3 and 4-7 softmax, products (odd CTA of a pair: passes on), TMA, list
 // Registers: 65536 / 384 threads allows 168 at launch; the third warpgroup gives up what the two
-// softmax warpgroups need to hold a row of S. 2 * 208 + 88 = 3 * 168.
-constexpr int kRegsSoftmax = 208, kRegsOther = 88;
+// softmax warpgroups need to hold a row of S. 2 * 216 + 72 = 3 * 168.
+constexpr int kRegsSoftmax = 216, kRegsOther = 72;
 constexpr int kKeys = 128;             // keys of a block
-constexpr int kJobs = 3;               // tiles that the list warp is ahead
+constexpr int kJobs = 2;               // tiles read ahead of the one in work, and it
 constexpr int kBufs = 3;               // S buffers
 constexpr float kRaise = 8.f;          // the reference follows when a block's maximum is 2^8 above it
-constexpr float kFar = 2097152.f;      // 2^21: references that ex2_poly can add 1.5 * 2^23 to
-#ifndef TB_POLY
-#define TB_POLY 0
-#endif
-constexpr int kPoly = TB_POLY;         // of every 8 pairs of exponentials, those by polynomial
-
 struct TcArgs {
     AttnArgs a;
     float* part;                       // [nsp][nq][heads][dim] partial rows, null without splits
     float* part_lse;                   // [nsp][nq][heads], base 2
     int nsplit, tile_tokens;           // key ranges; tokens of a 128-row tile
+    int wide;                          // output rows (or partial rows) start at multiples of 32 bytes
     uint32_t idesc_s, idesc_o, q_bytes;   // q_bytes: what one tile's boxes deliver
 };
 
@@ -65,9 +61,9 @@ template <int D, bool PAIR> struct Geom {
     static constexpr int kQBytes = kBoxes * 16384;                // 128 rows x D, boxes of 64 columns
     static constexpr int kBytes = kBoxes * 16384 / (PAIR ? 2 : 1);   // a CTA's share of a block's K, of its V
     static constexpr int kStages = 196608 / (2 * kBytes);         // of a K and a V each
-    static constexpr int kBars = 2 * kStages + 2 + 3 * kBufs + 2 + 8 + 4 + 2 * kJobs + 1;
-    static constexpr size_t kUsed = (size_t)kQBytes + 2 * kStages * kBytes + 2048 + 8 * kBars + kJobs * 48 + 16;
-    static constexpr size_t kSlack = 512;                         // for a base that is no multiple of 1024
+    static constexpr int kBars = (2 * kStages + 2 + 3 * kBufs + 2 + 8 + 4 + 2 * kJobs + 1 + 9 + 1) / 2 * 2;
+    static constexpr size_t kUsed = (size_t)kQBytes + 2 * kStages * kBytes + 2048 + 8 * kBars + kJobs * 48 + 48;
+    static constexpr size_t kSlack = 448;                         // for a base that is no multiple of 1024
     static constexpr size_t kSmem = kUsed + kSlack;
 };
 
@@ -110,32 +106,13 @@ __device__ __forceinline__ float max2(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
-// 2^(s c + ref) of two scores on the FMA pipes, beside the exponential unit. ref is a whole number,
-// so one fused product with ref + 1.5 * 2^23 (`lifted`) rounds the exponent to the nearest whole i in
-// its low bits, a second leaves the rest f = s c - (i - ref) without another rounding; 2^f by the
-// cubic of least relative error on [-1/2, 1/2] (exchange method, 7.5e-5: an eighth of a half step of
-// f16), and i is added to its exponent bits. Scores are taken at `least` (2^-120) at least.
-__device__ __forceinline__ float2 ex2_poly(float s0, float s1, float least, f2 c, f2 lifted) {
-    const f2 s = pack(max2(s0, least), max2(s1, least));
-    const f2 r = fma2(s, c, lifted);
-    const f2 f = fma2(s, c, sub2(lifted, r));
-    f2 y = fma2(pack(0.0551716685f, 0.0551716685f), f, pack(0.242611125f, 0.242611125f));
-    y = fma2(y, f, pack(0.693260968f, 0.693260968f));
-    y = fma2(y, f, pack(0.999928057f, 0.999928057f));
-    const float2 i = unpack(r), v = unpack(y);
-    return make_float2(__int_as_float(__float_as_int(v.x) + (__float_as_int(i.x) << 23)),
-                       __int_as_float(__float_as_int(v.y) + (__float_as_int(i.y) << 23)));
-}
-
-// p = 2^(s c + ref) of 128 scores of a row, rounded to T into the TMEM columns from `ts`; returns their
-// sum. NPOLY of every 8 pairs go by polynomial, which shares the work between the exponential unit (4
-// lanes a cycle and scheduler: 1024 cycles a block, as long as its products) and the FMA pipes. The
-// sum's additions fill slots that the exponential unit leaves. A hidden score (-inf) has to give
-// exactly 0: masked steps use NPOLY 0.
-template <class T, int NPOLY>
-__device__ __forceinline__ float exp_block(const float* s, float c, float ref, uint32_t ts) {
-    const f2 c2 = pack(c, c), ref2 = pack(ref, ref), lifted = add2(ref2, pack(12582912.f, 12582912.f));
-    const float least = NPOLY ? __fdividef(-120.f - ref, c) : 0.f;
+// p = 2^(s c + ref) of a row's 128 scores, rounded to T into the TMEM columns from `ts`; returns their
+// sum. The exponential unit (4 lanes a cycle and scheduler: 1024 cycles a block, as long as the block's
+// products) sets the pace and the sum's additions fill slots that it leaves. (A share of the
+// exponentials by a cubic on the FMA pipes, 1 or 2 of 8, cost as many cycles in issue as it saved
+// there: 1507 -> 1559 and 1659 us at 16384 x 12 x 128.)
+template <class T> __device__ __forceinline__ float exp_block(const float* s, float c, float ref, uint32_t ts) {
+    const f2 c2 = pack(c, c), ref2 = pack(ref, ref);
     f2 sum[2];
 #pragma unroll
     for (int quarter = 0; quarter < 4; ++quarter) {
@@ -143,14 +120,9 @@ __device__ __forceinline__ float exp_block(const float* s, float c, float ref, u
         uint32_t w[16];
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
-            float2 y;
-            if ((q & 7) * NPOLY / 8 != ((q & 7) + 1) * NPOLY / 8) {
-                y = ex2_poly(v[2 * q], v[2 * q + 1], least, c2, lifted);
-            } else {
-                y = unpack(fma2(pack(v[2 * q], v[2 * q + 1]), c2, ref2));
-                y.x = ex2(y.x);
-                y.y = ex2(y.y);
-            }
+            float2 y = unpack(fma2(pack(v[2 * q], v[2 * q + 1]), c2, ref2));
+            y.x = ex2(y.x);
+            y.y = ex2(y.y);
             w[q] = pack2(y.x, y.y, T());
             sum[q & 1] = quarter || q >= 2 ? add2(sum[q & 1], pack(y.x, y.y)) : pack(y.x, y.y);
         }
@@ -189,6 +161,34 @@ struct Job {
     int pad[2];
 };
 
+// 32 values of a row at p, as far as `left` says (a multiple of 8). Lanes are rows, so each store is a
+// sector or two of its own: 32 bytes at once where the rows allow it.
+template <class O> __device__ __forceinline__ void store_row(O* p, const float* v, int left, bool wide) {
+    constexpr int n = 32 / (int)sizeof(O);               // values of 32 bytes
+    if (wide && left >= 32) {
+#pragma unroll
+        for (int e = 0; e < 32; e += n) {
+            uint32_t w[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                if (sizeof(O) == 4) {
+                    w[q] = __float_as_uint(v[e + q]);
+                } else {
+                    using H = typename std::conditional<sizeof(O) == 4, __half, O>::type;
+                    w[q] = pack2(v[(e + 2 * q) % 32], v[(e + 2 * q + 1) % 32], H());
+                }
+            }
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                         :: "l"(p + e), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                         : "memory");
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 32; e += 8)
+            if (e < left) store8<O>(p + e, v + e);
+    }
+}
+
 template <class T, class O, int D, bool PAIR>
 __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorMap& kmap, const CUtensorMap& vmap,
                                         const TcArgs& p) {
@@ -200,7 +200,9 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
     float* s_sum = s_ref + 256;                                                   // [2][128] the warpgroups' sums
     uint64_t* bars = reinterpret_cast<uint64_t*>(s_sum + 256);
     Job* s_job = reinterpret_cast<Job*>(bars + G::kBars);
-    uint32_t* s_misc = reinterpret_cast<uint32_t*>(s_job + kJobs);                // [0] tmem, [1] abort
+    uint32_t* s_take = reinterpret_cast<uint32_t*>(s_job + kJobs);                // [4] the tile taken over, as answered
+    uint32_t* s_next = s_take + 4;                                                // [4] its number, for the odd CTA
+    uint32_t* s_misc = s_next + 4;                                                // [0] tmem, [1] abort
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_misc + 1);
     const uint32_t b0 = smem_u32(bars);
     auto full = [&](uint32_t s) { return b0 + 8u * s; };
@@ -214,13 +216,15 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
     auto sums = [&](int q) { return ofull + 8u * (10 + q); };
     auto jfull = [&](uint32_t s) { return ofull + 8u * (14 + s); };
     auto jempty = [&](uint32_t s) { return ofull + 8u * (14 + kJobs + s); };
-    const uint32_t drain = ofull + 8u * (14 + 2 * kJobs);
+    const uint32_t drain = ofull + 8u * (14 + 2 * kJobs), taken = drain + 8u;
+    auto told = [&](uint32_t s) { return taken + 8u * (1 + s); };
+    auto heard = [&](uint32_t s) { return taken + 8u * (5 + s); };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const AttnArgs& a = p.a;
     const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
     const bool leader = rank == 0;
     if ((size_t)(smem - smem_raw) > G::kSlack) {
-        if (threadIdx.x == 0) atomicCAS(a.err, 0, TB_DEVERR_WAIT_TIMEOUT);
+        if (threadIdx.x == 0) atomicCAS(a.err, 0, TB_DEVERR_SMEM_BASE);
         return;                            // both CTAs of a pair
     }
 
@@ -248,6 +252,11 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
             mbar_init(jempty(s), 10);                           // softmax warps, products, TMA
         }
         mbar_init(drain, 1);
+        mbar_init(taken, 1);
+        for (uint32_t s = 0; s < 4; ++s) {
+            mbar_init(told(s), 1);
+            mbar_init(heard(s), 1);
+        }
         s_misc[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -270,18 +279,16 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
     const uint32_t sq = smem_u32(smem), skv = sq + G::kQBytes;
 
     Ring<kJobs> jr;
-    // the next tile of the list; false at its end
-    auto next_job = [&](Job& j) {
-        if (!__all_sync(0xffffffffu, mbar_wait(jfull(jr.at), jr.round, s_abort, a.err))) return false;
-        const int4* src = reinterpret_cast<const int4*>(s_job + jr.at);
-        const int4 x = src[0], y = src[1], z = src[2];
-        j.q0 = x.x; j.nq = x.y; j.k0 = x.z; j.nk = x.w;
-        j.first = y.x; j.blk0 = y.y; j.n = y.z; j.kvh = y.w;
-        j.split = z.x; j.end = z.y;
+    // The next tile of the list, in place until it is released; null at the list's end.
+    auto next_job = [&]() -> const Job* {
+        if (!__all_sync(0xffffffffu, mbar_wait(jfull(jr.at), jr.round, s_abort, a.err))) return nullptr;
+        const Job* j = s_job + jr.at;
+        return j->end ? nullptr : j;
+    };
+    auto release_job = [&]() {
         __syncwarp();
         if (lane == 0) mbar_arrive(jempty(jr.at));
         jr.step();
-        return j.end == 0;
     };
 
     if (warp >= 8) {
@@ -308,20 +315,20 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
         Job j;
         if (warp == kList) {
             // -------------------------------------------------------------- the list
-            // Tiles in the order set, piece of the set, key head, range of keys; CTA c of N takes c, 2N-1-c,
-            // 2N+c, ...: there and back, so that none has the longer ones (causal: a set's last pieces,
-            // which see the most keys, come first) every time. A lane holds one of 32 sets.
-            const uint32_t c = PAIR ? cluster_id_x() : blockIdx.x, nc = PAIR ? nclusters_x() : gridDim.x;
+            // Tiles in the order set, piece of the set (causal: the last ones, which see the most keys, come
+            // first), key head, range of keys. A lane holds one of 32 sets; numbers only grow.
             int set0 = -32;
             uint32_t base = 0, total = 0, inc = 0, cnt = 0;
             int64_t qlo = 0, qhi = 0, klo = 0, khi = 0;
+            uint32_t number = PAIR ? cluster_id_x() : blockIdx.x, jobs = 0;
             for (uint32_t k = 0;; ++k) {
-                uint32_t idx = k * nc + (k & 1 ? nc - 1 - c : c);
+                const bool over = number == 0xffffffffu;         // none left to take over
+                uint32_t idx = over ? 0 : number;
                 const int split = idx % p.nsplit;
                 idx /= p.nsplit;
                 const int kvh = idx % a.kv_heads;
                 const uint32_t piece = idx / a.kv_heads;
-                while (piece >= base + total && set0 + 32 < a.nset) {
+                while (!over && piece >= base + total && set0 + 32 < a.nset) {
                     base += total;
                     set0 += 32;
                     cnt = 0;
@@ -338,7 +345,7 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                     }
                     total = __shfl_sync(0xffffffffu, inc, 31);
                 }
-                const bool found = piece < base + total;
+                const bool found = !over && piece < base + total;       // the launch has some more than there are
                 const int src = found ? __ffs(__ballot_sync(0xffffffffu, base + inc > piece)) - 1 : 0;
                 const uint32_t cs = __shfl_sync(0xffffffffu, cnt, src), at = piece - base - (__shfl_sync(0xffffffffu, inc, src) - cs);
                 Job o;
@@ -353,24 +360,62 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 o.n = (int)((int64_t)all * (split + 1) / p.nsplit) - o.blk0;
                 o.kvh = kvh;
                 o.split = split;
-                o.end = found ? 0 : 1;
-                if (k >= kJobs && !__all_sync(0xffffffffu, mbar_wait(jempty(jr.at), jr.round ^ 1, s_abort, a.err))) break;
-                if (lane == 0) {
-                    int4* dst = reinterpret_cast<int4*>(s_job + jr.at);
-                    dst[0] = make_int4(o.q0, o.nq, o.k0, o.nk);
-                    dst[1] = make_int4(o.first, o.blk0, o.n, o.kvh);
-                    dst[2] = make_int4(o.split, o.end, 0, 0);
-                    mbar_arrive(jfull(jr.at));
+                o.end = over ? 1 : 0;
+                if (found || over) {
+                    if (jobs >= kJobs && !__all_sync(0xffffffffu, mbar_wait(jempty(jr.at), jr.round ^ 1, s_abort, a.err))) break;
+                    if (lane == 0) {
+                        int4* dst = reinterpret_cast<int4*>(s_job + jr.at);
+                        dst[0] = make_int4(o.q0, o.nq, o.k0, o.nk);
+                        dst[1] = make_int4(o.first, o.blk0, o.n, o.kvh);
+                        dst[2] = make_int4(o.split, o.end, 0, 0);
+                        mbar_arrive(jfull(jr.at));
+                    }
+                    __syncwarp();
+                    jr.step();
+                    ++jobs;
+                    if (over) break;
                 }
-                __syncwarp();
-                jr.step();
-                if (!found) break;
+                if (leader) {
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(taken, 16);
+                        asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                                     :: "r"(smem_u32(s_take)), "r"(taken) : "memory");
+                    }
+                    __syncwarp();
+                    if (!__all_sync(0xffffffffu, mbar_wait(taken, k & 1, s_abort, a.err))) break;
+                    uint32_t x, got;
+                    asm volatile("{\n\t.reg .pred p;\n\t.reg .b128 h;\n\t"
+                                 "ld.shared.b128 h, [%2];\n\t"
+                                 "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+                                 "selp.u32 %1, 1, 0, p;\n\tmov.u32 %0, 0;\n\t"
+                                 "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n\t}"
+                                 : "=r"(x), "=r"(got) : "r"(smem_u32(s_take)) : "memory");
+                    number = got ? (PAIR ? x / 2 : x) : 0xffffffffu;
+                    fence_proxy_async_smem();                    // read before the next answer is written
+                    __syncwarp();
+                    // one of four places for the odd CTA, once it has read what was there
+                    if (PAIR && k >= 4 && !__all_sync(0xffffffffu, mbar_wait_cluster(heard(k & 3), ((k >> 2) - 1) & 1, s_abort, a.err)))
+                        break;
+                    if (PAIR && lane == 0) {
+                        asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, 1;\n\t"
+                                     "st.shared::cluster.u32 [ra], %1;\n\t}"
+                                     :: "r"(smem_u32(s_next + (k & 3))), "r"(number) : "memory");
+                        mbar_arrive_cluster(told(k & 3), 1);
+                    }
+                } else {
+                    if (!__all_sync(0xffffffffu, mbar_wait_cluster(told(k & 3), k >> 2 & 1, s_abort, a.err))) break;
+                    number = *reinterpret_cast<volatile uint32_t*>(s_next + (k & 3));
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(heard(k & 3), 0);
+                }
             }
         } else if (warp == kTma) {
             // -------------------------------------------------------------- TMA producer
             Ring<G::kStages> r;
             uint32_t used = 0, tiles = 0;
-            while (ok && next_job(j)) {
+            while (const Job* from = next_job()) {
+                j = *from;
+                release_job();
                 if (j.n == 0) continue;
                 const int lag = min(j.n, kBufs), items = j.n + lag;
                 if (tiles && !wait(qempty, (tiles - 1) & 1)) break;
@@ -396,6 +441,7 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                     }
                     __syncwarp();
                 }
+                if (!ok) break;
                 ++tiles;
             }
         } else if (warp == kMma && leader) {
@@ -429,8 +475,10 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 commit<PAIR>(sfull(us.at));
                 if (last) commit<PAIR>(qempty);
             };
-            while (ok && next_job(j)) {
-                const int n = j.n;
+            while (const Job* from = ok ? next_job() : nullptr) {
+                const int n = from->n;
+                int keys = from->nk - from->blk0 * kKeys;
+                release_job();
                 if (n == 0) continue;
                 const int lag = min(n, kBufs);
                 ok = __all_sync(0xffffffffu, mbar_wait(bq, tiles & 1, s_abort, a.err));
@@ -443,7 +491,6 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                     }
                     __syncwarp();
                 }
-                int keys = j.nk - j.blk0 * kKeys;
                 for (int b = 0; b < n && ok; ++b, r.step(), u.step(), keys -= kKeys) {
                     if (!wait(full(r.at), r.round)) break;
                     if (keys < kKeys && (keys & 15)) clean(r.at, keys);
@@ -479,7 +526,9 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
             // -------------------------------------------------------------- odd CTA: what has landed, passed on
             Ring<G::kStages> r;
             uint32_t tiles = 0;
-            while (ok && next_job(j)) {
+            while (const Job* from = ok ? next_job() : nullptr) {
+                j = *from;
+                release_job();
                 if (j.n == 0) continue;
                 const int lag = min(j.n, kBufs), items = j.n + lag, tail = j.nk - (j.blk0 + j.n - 1) * kKeys;
                 ok = __all_sync(0xffffffffu, mbar_wait(bq, tiles & 1, s_abort, a.err));
@@ -508,16 +557,25 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
         Ring<kBufs> u;
         uint32_t tiles = 0, blocks = 0, turns = 0;   // tiles with keys, blocks of all tiles, hand-offs received
         bool ok = true;
-        Job j;
-        while (ok && next_job(j)) {
-            const int t = j.first + (int)rank * p.tile_tokens + r / a.group, h = j.kvh * a.group + r % a.group;
-            const bool valid = r < p.tile_tokens * a.group && t < j.nq;
-            const int lim = !valid ? j.nk : a.causal ? max(0, min(j.nk, t + 1 + j.nk - j.nq)) : j.nk;  // keys the row sees
-            const int wlim = __reduce_min_sync(0xffffffffu, lim), n = j.n;
+        while (const Job* job = ok ? next_job() : nullptr) {
+            const int n = job->n;
+            // the keys from the tile's first block on that the row sees; rows past the set see all
+            auto rows = [&](int& t, int& h) {
+                t = job->first + (int)rank * p.tile_tokens + r / a.group;
+                h = job->kvh * a.group + r % a.group;
+                return r < p.tile_tokens * a.group && t < job->nq;
+            };
+            int lim, wlim;
+            {
+                int t, h;
+                const int nk = job->nk;
+                lim = !rows(t, h) ? nk : a.causal ? max(0, min(nk, t + 1 + nk - job->nq)) : nk;
+                lim -= job->blk0 * kKeys;
+                wlim = __reduce_min_sync(0xffffffffu, lim);
+            }
             float* refs = s_ref + (tiles & 1) * 128;
             float ref = -INFINITY, l = 0.f;          // of the warpgroup's own blocks; -inf: no key so far
             float shift = lift;                      // what scores are shifted by: lift - ref
-            bool far = false;
             for (int b = 0; b < n; ++b, ++blocks, u.step()) {
                 if ((int)(blocks & 1) != wg) continue;
                 const uint32_t ts = tmem + u.at * 128u + lane_base;
@@ -534,10 +592,9 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                     if (b > 0) now = refs[r];
                 }
                 tmem_wait_ld();
-                const int key0 = (j.blk0 + b) * kKeys;
-                const bool masked = wlim < key0 + kKeys;
+                const bool masked = wlim < (b + 1) * kKeys;
                 if (masked) {
-                    const int left = lim - key0;
+                    const int left = lim - b * kKeys;
 #pragma unroll
                     for (int q = 0; q < kKeys; ++q) s[q] = q < left ? s[q] : -INFINITY;
                 }
@@ -552,7 +609,7 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 const float top = max3(max3(mx[0], mx[1], s[kKeys - 4]), max3(mx[2], mx[3], s[kKeys - 3]),
                                        max2(s[kKeys - 2], s[kKeys - 1])) * c;
                 const bool raise = !(top - now <= kRaise) && !(top == -INFINITY && now == -INFINITY);
-                if (b == 0 || far || __any_sync(0xffffffffu, raise || now != ref)) {
+                if (b == 0 || __any_sync(0xffffffffu, raise || now != ref)) {
                     const float next = raise ? rintf(top) : now;
                     refs[r] = next;
                     if (b > 0 && __any_sync(0xffffffffu, raise)) {
@@ -575,10 +632,10 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                     l = next == ref ? l : l * ex2(ref - next);
                     ref = next;
                     shift = lift - (ref == -INFINITY ? 0.f : ref);
-                    far = __any_sync(0xffffffffu, !(fabsf(ref) < kFar) && ref != -INFINITY);
                 }
                 if (lane == 0) mbar_arrive(handed(1 - wg, quad));
-                l += masked || far ? exp_block<T, 0>(s, c, shift, ts) : exp_block<T, kPoly>(s, c, shift, ts);
+                __syncwarp();                        // the hand-off first: the exponentials are not moved ahead of it
+                l += exp_block<T>(s, c, shift, ts);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -601,11 +658,12 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 total = s_sum[r] + s_sum[128 + r];
             }
             if (!ok) break;
-            const bool none = n == 0 || lim <= j.blk0 * kKeys;     // the row sees no key here
+            int t, h;
+            const bool valid = rows(t, h), none = n == 0 || lim <= 0;      // none: the row sees no key here
             const float inv = none ? 0.f : 1.f / total;
             const float lg = none ? -INFINITY : ref - lift + log2f(total);
-            const int64_t row = (int64_t)j.q0 + t;
-            const int64_t at = ((int64_t)j.split * a.nq + row) * a.heads + h;
+            const int64_t row = (int64_t)job->q0 + t;
+            const int64_t at = ((int64_t)job->split * a.nq + row) * a.heads + h;
             if (valid && wg == 0) {
                 if (p.part) p.part_lse[at] = lg;
                 else if (a.lse) a.lse[row * a.heads + h] = lg * 0.69314718055994530942f;
@@ -634,14 +692,11 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 if (!valid || (p.part && none)) continue;
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = none ? 0.f : o[e] * inv;
-#pragma unroll
-                for (int e = 0; e < 32; e += 8)
-                    if (q + e < a.dim) {
-                        if (p.part) store8<float>(part + q + e, o + e);
-                        else store8<O>(out + q + e, o + e);
-                    }
+                if (p.part) store_row<float>(part + q, o, a.dim - q, p.wide);
+                else store_row<O>(out + q, o, a.dim - q, p.wide);
             }
             if (n > 0) ++tiles;
+            release_job();
         }
         tc_fence_before();
     }
@@ -776,8 +831,7 @@ tb_status launch(tb_ctx* ctx, const TcArgs& p, const Plan& l, const CUtensorMap&
                                 : wide ? (const void*)k_attn_tc<T, O, 128> : (const void*)k_attn_tc<T, O, 64>;
     if (sm > (size_t)ctx->max_smem_optin) return tb_fail(ctx, TB_ERR_UNSUPPORTED, "tb_attention: shared memory too small");
     TB_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
-    const unsigned grid = l.pair ? 2u * (unsigned)std::min<int64_t>(l.items, ctx->num_sms / 2)
-                                 : (unsigned)std::min<int64_t>(l.items, ctx->num_sms);
+    const unsigned grid = (unsigned)(l.pair ? 2 * l.items : l.items);
     if (l.pair) k_attn_pair<T, O><<<grid, kThreads, sm, ctx->stream>>>(qm, km, vm, p);
     else if (wide) k_attn_tc<T, O, 128><<<grid, kThreads, sm, ctx->stream>>>(qm, km, vm, p);
     else k_attn_tc<T, O, 64><<<grid, kThreads, sm, ctx->stream>>>(qm, km, vm, p);
@@ -810,6 +864,11 @@ tb_status tb_attn_tc_launch(tb_ctx* ctx, const AttnArgs& args, tb_dtype dtype, t
     if (l.nsplit > 1) {
         p.part = reinterpret_cast<float*>(workspace);
         p.part_lse = p.part + (size_t)l.nsplit * a.nq * a.heads * a.dim;
+    }
+    {
+        const int64_t size = (int64_t)tb_dtype_size(out_dtype);
+        const bool rows = (reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.out_row * size) | (uintptr_t)(a.out_head * size)) % 32 == 0;
+        p.wide = l.nsplit > 1 ? a.dim % 8 == 0 && reinterpret_cast<uintptr_t>(workspace) % 32 == 0 : rows;
     }
     const uint32_t fmt = dtype == TB_BF16 ? 1u : 0u;
     const uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((l.pair ? 16u : 8u) << 24);

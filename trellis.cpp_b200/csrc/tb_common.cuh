@@ -15,6 +15,7 @@ enum tb_device_error : int {
     TB_DEVERR_HASH_PROBE = 1,     // hash insert/lookup exceeded its probe bound
     TB_DEVERR_WAIT_TIMEOUT = 2,   // a bounded mbarrier wait in the conv kernel ran out
     TB_DEVERR_TMEM_ALLOC = 3,     // TMEM allocation returned an unusable address
+    TB_DEVERR_SMEM_BASE = 5,      // dynamic shared memory starts too far from a multiple of 1024
     TB_DEVERR_BAD_OFFSETS = 4,    // an offset table of packed sets descends or leaves the array
 };
 
