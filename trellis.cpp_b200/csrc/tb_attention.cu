@@ -7,9 +7,13 @@
 // sum and output so far are scaled by exp(old - new).
 //
 // k_attn_cc: one block takes 64 rows (a row is a query token and one of the heads that share a key
-// head, so a group's heads read the keys once) and walks the keys 64 at a time: scores by 4 x 4
-// register tiles from shared memory, softmax over 16 lanes a row, output by 4 x (dim / 16) tiles.
-// Bound by the FFMA rate and the shared-memory reads that feed it.
+// head, so a group's heads read the keys once) and walks the keys 64 at a time. Scores and output are
+// the same product of two tiles in shared memory, 8 x 4 values a thread: the values are laid in the
+// tile, so 16 bytes are two pairs of neighbours of the summed axis for packed FMAs, and the two halves
+// of a pair's sum meet at the end. Bound by what feeds the FMAs: a warp's step is 12 16-byte loads, 4
+// cycles of the SM's shared-memory path each, and 64 packed FMAs, 2 cycles of its scheduler each, so
+// the path is busy 192 cycles for 128 of the four schedulers' FMAs. 800 and 600 rows, 8 heads of 64:
+// 92 us, 22 TFLOP/s (4 x 4 values a thread, 256 threads, unpacked: 107 us).
 #include "tb_packed.cuh"
 
 #include <algorithm>
@@ -21,25 +25,59 @@ namespace {
 
 using namespace tbpk;
 
-constexpr int kCcThreads = 256, kCcRows = 64, kCcKeys = 64;
+constexpr int kCcThreads = 128, kCcRows = 64, kCcKeys = 64, kCcLd = 68;
 
 template <class T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <class T, class O, int D>
-__global__ void __launch_bounds__(kCcThreads) k_attn_cc(const __grid_constant__ AttnArgs a) {
-    constexpr int LD = D + 4;                       // row stride of q and k tiles: no bank is hit twice
+// x[i][j] = sum over n < N of a[i * 8 rows][n] b[j * 16 rows][n]. Row strides of 4 modulo 32 words: the
+// 16 rows of b and the two of a that a warp reads at once lie in different banks.
+template <int N, int LDA, int LDB>
+__device__ __forceinline__ void tile_product(const float* a, const float* b, float (&x)[8][4]) {
+    f2 acc[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0;
+#pragma unroll 2
+    for (int n = 0; n < N; n += 4) {
+        ulonglong2 bv[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bv[j] = *reinterpret_cast<const ulonglong2*>(b + 16 * j * LDB + n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const ulonglong2 av = *reinterpret_cast<const ulonglong2*>(a + 8 * i * LDA + n);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = fma2(av.y, bv[j].y, fma2(av.x, bv[j].x, acc[i][j]));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack(acc[i][j]);
+            x[i][j] = f.x + f.y;
+        }
+}
+
+// Operands are 32-bit; without keys nothing is read, and O alone counts.
+template <class O, int D>
+__global__ void __launch_bounds__(kCcThreads, 2) k_attn_cc(const __grid_constant__ AttnArgs a) {
+    constexpr int LD = D + 4, V4 = D / 64;
     extern __shared__ float sm[];
     float* sq = sm;                                 // [64][LD]
-    float* sk = sq + kCcRows * LD;                  // [64][LD]
-    float* sv = sk + kCcKeys * LD;                  // [64][D]
-    float* sp = sv + kCcKeys * D;                   // [64][68]
+    float* sk = sq + kCcRows * LD;                  // [64][LD], then the weights [64][68]
+    float* sv = sk + kCcKeys * LD;                  // [D][68]: values of a column side by side
+    float* sp = sk;
     __shared__ Item it;
     __shared__ uint32_t scan[32];
-    const int kvh = blockIdx.x % a.kv_heads;
-    find_item(a.q_off, a.nset, a.nq, a.unit, blockIdx.x / a.kv_heads, a.err, &it, scan);
+    uint32_t idx = blockIdx.x;
+    const int split = idx % a.nsplit;
+    idx /= a.nsplit;
+    const int kvh = idx % a.kv_heads;
+    find_item(a.q_off, a.nset, a.nq, a.unit, idx / a.kv_heads, a.err, &it, scan);
     if (it.set < 0) return;
     // causal: the last rows of a set see the most keys; they go first
     const int piece = a.causal ? (int)(it.items - 1 - it.item) : (int)it.item;
@@ -47,70 +85,58 @@ __global__ void __launch_bounds__(kCcThreads) k_attn_cc(const __grid_constant__ 
     set_range(a.k_off, it.set, a.nk, k0, k1, a.err);
     const int nq = (int)(it.hi - it.lo), nk = (int)(k1 - k0), g = a.group;
     const int t0 = piece * a.unit, rows = min(a.unit, nq - t0) * g;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;     // rows ty + 8 i
 
-    for (int i = threadIdx.x; i < kCcRows * (D / 8); i += kCcThreads) {
-        const int r = i / (D / 8), d = i % (D / 8) * 8;
-        float v[8];
+    int lim[8];                                     // keys that the thread's rows see
+    float m[8], l[8], o[8][4 * V4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.f;
-        if (r < rows && d < a.dim)
-            load8<T>(reinterpret_cast<const T*>(a.q) + (it.lo + t0 + r / g) * a.q_row + (int64_t)(kvh * g + r % g) * a.q_head + d, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sq[r * LD + d + j] = v[j] * a.scale_log2;
-    }
-    int lim[4];                                     // keys that the thread's rows see
-    float m[4], l[4], o[4][D / 16];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = ty * 4 + i;
+    for (int i = 0; i < 8; ++i) {
+        const int r = ty + 8 * i;
         lim[i] = r >= rows ? 0 : (a.causal ? max(0, min(nk, t0 + r / g + nk - nq + 1)) : nk);
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j) o[i][j] = 0.f;
+        for (int j = 0; j < 4 * V4; ++j) o[i][j] = 0.f;
     }
     const int last_t = t0 + (rows - 1) / g;
     const int end = a.causal ? max(0, min(nk, last_t + nk - nq + 1)) : nk;
-    for (int kb = 0; kb < end; kb += kCcKeys) {
+    const int all = (end + kCcKeys - 1) / kCcKeys;
+    const int first = (int)((int64_t)all * split / a.nsplit) * kCcKeys;
+    const int stop = min(end, (int)((int64_t)all * (split + 1) / a.nsplit) * kCcKeys);
+    if (first < stop)
+        for (int i = threadIdx.x; i < kCcRows * (D / 8); i += kCcThreads) {
+            const int r = i / (D / 8), d = i % (D / 8) * 8;
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = 0.f;
+            if (r < rows && d < a.dim)
+                load8<float>(reinterpret_cast<const float*>(a.q) + (it.lo + t0 + r / g) * a.q_row + (int64_t)(kvh * g + r % g) * a.q_head + d, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= a.scale_log2;
+            store8<float>(sq + r * LD + d, v);
+        }
+    for (int kb = first; kb < stop; kb += kCcKeys) {
         __syncthreads();
         for (int i = threadIdx.x; i < kCcKeys * (D / 8); i += kCcThreads) {
-            const int r = i / (D / 8), d = i % (D / 8) * 8;
+            const int r = i / (D / 8), d = i % (D / 8) * 8;     // a row's columns on neighbouring lanes
+            const int vr = i % kCcKeys, vd = i / kCcKeys * 8;   // rows on neighbouring lanes: turned without conflicts
             float kv[8], vv[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) kv[j] = vv[j] = 0.f;
-            if (kb + r < nk && d < a.dim) {         // keys past the set stay zero
-                load8<T>(reinterpret_cast<const T*>(a.k) + (k0 + kb + r) * a.k_row + (int64_t)kvh * a.k_head + d, kv);
-                load8<T>(reinterpret_cast<const T*>(a.v) + (k0 + kb + r) * a.v_row + (int64_t)kvh * a.v_head + d, vv);
-            }
+            for (int j = 0; j < 8; ++j) kv[j] = vv[j] = 0.f;    // keys past the set stay zero
+            if (kb + r < nk && d < a.dim)
+                load8<float>(reinterpret_cast<const float*>(a.k) + (k0 + kb + r) * a.k_row + (int64_t)kvh * a.k_head + d, kv);
+            if (kb + vr < nk && vd < a.dim)
+                load8<float>(reinterpret_cast<const float*>(a.v) + (k0 + kb + vr) * a.v_row + (int64_t)kvh * a.v_head + vd, vv);
             store8<float>(sk + r * LD + d, kv);
-            store8<float>(sv + r * D + d, vv);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sv[(vd + j) * kCcLd + vr] = vv[j];
         }
         __syncthreads();
-        float s[4][4];
+        float s[8][4];
+        tile_product<D, LD, LD>(sq + ty * LD, sk + tx * LD, s);
+        __syncthreads();                            // every warp is through with the keys
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-#pragma unroll 4
-        for (int d = 0; d < D; d += 4) {
-            float4 qv[4], kv[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(sq + (ty * 4 + i) * LD + d);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * LD + d);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s[i][j] = fmaf(qv[i].x, kv[j].x, s[i][j]);
-                    s[i][j] = fmaf(qv[i].y, kv[j].y, s[i][j]);
-                    s[i][j] = fmaf(qv[i].z, kv[j].z, s[i][j]);
-                    s[i][j] = fmaf(qv[i].w, kv[j].w, s[i][j]);
-                }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 8; ++i) {
             float mx = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -128,74 +154,120 @@ __global__ void __launch_bounds__(kCcThreads) k_attn_cc(const __grid_constant__ 
             for (int j = 0; j < 4; ++j) {
                 const float p = exp2f(s[i][j] - ref);
                 sum += p;
-                sp[(ty * 4 + i) * 68 + tx + 16 * j] = p;
+                sp[(ty + 8 * i) * kCcLd + tx + 16 * j] = p;
             }
             l[i] = fmaf(l[i], al, sum);                          // the lane's own keys; joined at the end
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j) o[i][j] *= al;
+            for (int j = 0; j < 4 * V4; ++j) o[i][j] *= al;
         }
         __syncwarp();                               // a row's 16 lanes are one half of a warp
-#pragma unroll 2
-        for (int kk = 0; kk < kCcKeys; kk += 4) {
-            float4 p[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const float4*>(sp + (ty * 4 + i) * 68 + kk);
+        for (int c = 0; c < V4; ++c) {
+            tile_product<kCcKeys, kCcLd, kCcLd>(sp + ty * kCcLd, sv + (c * 64 + tx) * kCcLd, s);
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int c = 0; c < D / 64; ++c) {
-                    const float4 v = *reinterpret_cast<const float4*>(sv + (kk + q) * D + c * 64 + tx * 4);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float pq = q == 0 ? p[i].x : q == 1 ? p[i].y : q == 2 ? p[i].z : p[i].w;
-                        o[i][4 * c] = fmaf(pq, v.x, o[i][4 * c]);
-                        o[i][4 * c + 1] = fmaf(pq, v.y, o[i][4 * c + 1]);
-                        o[i][4 * c + 2] = fmaf(pq, v.z, o[i][4 * c + 2]);
-                        o[i][4 * c + 3] = fmaf(pq, v.w, o[i][4 * c + 3]);
-                    }
-                }
+                for (int j = 0; j < 4; ++j) o[i][4 * c + j] += s[i][j];
         }
-        __syncwarp();
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = ty * 4 + i;
+    for (int i = 0; i < 8; ++i) {
+        const int r = ty + 8 * i;
         float sum = l[i];
 #pragma unroll
         for (int d = 8; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (r >= rows) continue;
         const int64_t t = it.lo + t0 + r / g;
         const int h = kvh * g + r % g;
-        const bool none = lim[i] == 0;              // a row without a key: out 0, lse -inf
+        const bool none = min(lim[i], stop) <= first;       // a row without a key: out 0, lse -inf
+        const float lg = none ? -INFINITY : m[i] + log2f(sum);
         const float inv = none ? 0.f : 1.f / sum;
+        if (a.part) {
+            const int64_t at = ((int64_t)split * a.nq + t) * a.heads + h;
+            if (tx == 0) a.part_lse[at] = lg;
+            if (none) continue;
+#pragma unroll
+            for (int j = 0; j < 4 * V4; ++j)
+                if (tx + 16 * j < a.dim) a.part[at * a.dim + tx + 16 * j] = o[i][j] * inv;
+            continue;
+        }
         O* out = reinterpret_cast<O*>(a.out) + t * a.out_row + (int64_t)h * a.out_head;
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int d = c * 64 + tx * 4 + j;
-                if (d < a.dim) out[d] = from_f32<O>(none ? 0.f : o[i][4 * c + j] * inv);
-            }
-        if (a.lse && tx == 0)
-            a.lse[t * a.heads + h] = none ? -INFINITY : (m[i] + log2f(sum)) * 0.69314718055994530942f;
+        for (int j = 0; j < 4 * V4; ++j)
+            if (tx + 16 * j < a.dim) out[tx + 16 * j] = from_f32<O>(none ? 0.f : o[i][j] * inv);
+        if (a.lse && tx == 0) a.lse[t * a.heads + h] = lg * 0.69314718055994530942f;
     }
 }
 
-template <class T, class O, int D>
+// Blocks of the CUDA-core kernel before the keys are cut.
+int64_t cc_items(int64_t nq, int nset, int kv_heads, int group) {
+    const int unit = kCcRows / group;
+    return ((nq + unit - 1) / unit + nset) * kv_heads;
+}
+// Fewer blocks than three an SM are cut into ranges of at least two blocks of keys (800 and 600 rows,
+// 8 heads of 64, 192 blocks: 104 us whole, 92 us with the keys cut in two and joined).
+int cc_nsplit(const tb_ctx* ctx, int64_t nq, int64_t nk, int nset, int kv_heads, int group) {
+    const int64_t items = cc_items(nq, nset, kv_heads, group), blocks = (nk / nset + kCcKeys - 1) / kCcKeys;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({3ll * ctx->num_sms / items, blocks / 2, 32}));
+}
+
+template <class O, int D>
 tb_status launch_cc(tb_ctx* ctx, AttnArgs a) {
-    constexpr size_t sm = sizeof(float) * (2 * 64 * (D + 4) + 64 * D + 64 * 68);
-    a.unit = std::max(1, kCcRows / a.group);
-    const int64_t items = ((a.nq + a.unit - 1) / a.unit + a.nset) * a.kv_heads;
+    constexpr size_t sm = sizeof(float) * (2 * 64 * (D + 4) + D * kCcLd);
+    a.unit = kCcRows / a.group;
+    const int64_t items = cc_items(a.nq, a.nset, a.kv_heads, a.group) * a.nsplit;
     if (items > INT32_MAX) return tb_fail(ctx, TB_ERR_TOO_LARGE, "tb_attention: too many rows times heads");
-    TB_CUDA_TRY(ctx, cudaFuncSetAttribute(k_attn_cc<T, O, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
-    k_attn_cc<T, O, D><<<(unsigned)items, kCcThreads, sm, ctx->stream>>>(a);
+    TB_CUDA_TRY(ctx, cudaFuncSetAttribute(k_attn_cc<O, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
+    k_attn_cc<O, D><<<(unsigned)items, kCcThreads, sm, ctx->stream>>>(a);
     TB_LAUNCH_CHECK(ctx, "k_attn_cc");
     return TB_OK;
 }
 
-template <class T, class O>
-tb_status launch_cc_dim(tb_ctx* ctx, const AttnArgs& a) {
-    return a.dim <= 64 ? launch_cc<T, O, 64>(ctx, a) : launch_cc<T, O, 128>(ctx, a);
+// Joins the partial rows: with lg_s the base-2 log sum of part s and M their maximum,
+//   out = sum_s 2^(lg_s - M) out_s / sum_s 2^(lg_s - M),  lse = (M + log2(that sum)) / log2(e).
+// A warp a row and head: a lane takes one part's weight (at most 32), then four values of the row.
+template <class O>
+__global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ AttnArgs a) {
+    const int lane = threadIdx.x & 31;
+    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int64_t row = at / a.heads, h = at % a.heads, step = a.nq * a.heads;
+    int64_t lo = 0, hi = a.nq;
+    if (a.q_off) {
+        lo = min(max((int64_t)a.q_off[0], (int64_t)0), a.nq);
+        hi = min((int64_t)a.q_off[a.nset], a.nq);
+    }
+    if (row < lo || row >= hi) return;
+    const float lg = lane < a.nsplit ? a.part_lse[lane * step + at] : -INFINITY;
+    float mx = lg;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    // a log sum that is no number does not show in the maximum: it goes by its weight
+    const float w = lg == -INFINITY ? 0.f : exp2f(lg - mx);
+    const int c0 = lane * 4;
+    float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < a.nsplit; ++s) {
+        const float ws = __shfl_sync(0xffffffffu, w, s), ls = __shfl_sync(0xffffffffu, lg, s);
+        sum += ws;
+        if (ls == -INFINITY || c0 >= a.dim) continue;        // no key here, nothing was written
+        const float4 v = *reinterpret_cast<const float4*>(a.part + (s * step + at) * a.dim + c0);
+        o[0] = fmaf(ws, v.x, o[0]);
+        o[1] = fmaf(ws, v.y, o[1]);
+        o[2] = fmaf(ws, v.z, o[2]);
+        o[3] = fmaf(ws, v.w, o[3]);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (lane == 0 && a.lse) a.lse[at] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994530942f;
+    if (c0 >= a.dim) return;
+    O* out = reinterpret_cast<O*>(a.out) + row * a.out_row + h * a.out_head + c0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= inv;
+    if (sizeof(O) == 4) {
+        *reinterpret_cast<float4*>(out) = make_float4(o[0], o[1], o[2], o[3]);
+    } else {
+        using H = typename std::conditional<sizeof(O) == 4, __half, O>::type;
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack2(o[0], o[1], H()), pack2(o[2], o[3], H()));
+    }
 }
 
 bool bad_stride(int64_t count, int64_t stride, int64_t unit) { return count > 1 && (stride <= 0 || stride % unit != 0); }
@@ -264,29 +336,48 @@ tb_status attn_args(tb_ctx* ctx, const tb_attention_params* p, AttnArgs& a) {
 
 }  // namespace
 
+// Ranges that the kernel for these arguments cuts the keys into; 1 without keys.
+static int attn_nsplit(const tb_ctx* ctx, tb_dtype dtype, int64_t nq, int64_t nk, int nset, int heads, int kv_heads, int dim) {
+    if (nq <= 0 || nk <= 0 || nset <= 0) return 1;
+    if (dtype == TB_F32) return cc_nsplit(ctx, nq, nk, nset, kv_heads, heads / kv_heads);
+    return tb_attn_tc_nsplit(ctx, nq, nk, nset, heads, kv_heads, dim);
+}
+
 extern "C" size_t tb_attention_workspace_bytes(const tb_ctx* ctx, const tb_attention_params* p) {
-    if (!ctx || !p || (p->dtype != TB_F16 && p->dtype != TB_BF16) || p->heads < 1 || p->kv_heads < 1 ||
-        p->heads % p->kv_heads != 0 || p->heads / p->kv_heads > 64 || p->head_dim < 1)
+    if (!ctx || !p || p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads != 0 || p->heads / p->kv_heads > 64 ||
+        p->head_dim < 1)
         return 0;
-    return tb_attn_tc_workspace(ctx, p->nq, p->nk, p->nset, p->heads, p->kv_heads, p->head_dim);
+    const int n = attn_nsplit(ctx, p->dtype, p->nq, p->nk, p->nset, p->heads, p->kv_heads, p->head_dim);
+    return n > 1 ? (size_t)n * p->nq * p->heads * (p->head_dim + 1) * sizeof(float) : 0;
 }
 
 extern "C" tb_status tb_attention(tb_ctx* ctx, const tb_attention_params* p) {
     if (!ctx) return TB_ERR_INVALID_ARG;
     AttnArgs a{};
-    const tb_status s = attn_args(ctx, p, a);
+    tb_status s = attn_args(ctx, p, a);
     if (s != TB_OK) return s;
     if (a.nq == 0 || a.nset == 0) return TB_OK;
-    const size_t need = tb_attention_workspace_bytes(ctx, p);
-    if (need && (!p->workspace || p->workspace_bytes < need || !tb_aligned16(p->workspace)))
-        return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_attention: workspace too small or not 16-byte aligned");
+    a.nsplit = attn_nsplit(ctx, p->dtype, a.nq, a.nk, a.nset, a.heads, a.kv_heads, a.dim);
+    if (a.nsplit > 1) {
+        const size_t rows = (size_t)a.nsplit * a.nq * a.heads;
+        if (!p->workspace || p->workspace_bytes < rows * (a.dim + 1) * sizeof(float) || !tb_aligned16(p->workspace))
+            return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_attention: workspace too small or not 16-byte aligned");
+        if ((a.nq * a.heads + 3) / 4 > INT32_MAX) return tb_fail(ctx, TB_ERR_TOO_LARGE, "tb_attention: too many rows times heads");
+        a.part = reinterpret_cast<float*>(p->workspace);
+        a.part_lse = a.part + rows * a.dim;
+    }
     tb_device_guard guard;
     TB_CUDA_TRY(ctx, guard.enter(ctx->device));
-    if (p->dtype == TB_F32) return launch_cc_dim<float, float>(ctx, a);
-    if (a.nk > 0) return tb_attn_tc_launch(ctx, a, p->dtype, p->out_dtype, p->workspace);
-    // no key rows to describe to the tensor cores' loads: every row is 0
-    if (p->dtype == TB_F16)
-        return p->out_dtype == TB_F32 ? launch_cc_dim<__half, float>(ctx, a) : launch_cc_dim<__half, __half>(ctx, a);
-    return p->out_dtype == TB_F32 ? launch_cc_dim<__nv_bfloat16, float>(ctx, a)
-                                  : launch_cc_dim<__nv_bfloat16, __nv_bfloat16>(ctx, a);
+    // without key rows there is nothing to describe to the tensor cores' loads: every row is 0
+    if (p->dtype != TB_F32 && a.nk > 0) s = tb_attn_tc_launch(ctx, a, p->dtype, p->out_dtype);
+    else if (p->out_dtype == TB_F16) s = launch_cc<__half, 128>(ctx, a);
+    else if (p->out_dtype == TB_BF16) s = launch_cc<__nv_bfloat16, 128>(ctx, a);
+    else s = a.dim <= 64 ? launch_cc<float, 64>(ctx, a) : launch_cc<float, 128>(ctx, a);
+    if (s != TB_OK || !a.part) return s;
+    const unsigned blocks = (unsigned)((a.nq * a.heads + 3) / 4);
+    if (p->out_dtype == TB_F32) k_attn_join<float><<<blocks, 128, 0, ctx->stream>>>(a);
+    else if (p->out_dtype == TB_F16) k_attn_join<__half><<<blocks, 128, 0, ctx->stream>>>(a);
+    else k_attn_join<__nv_bfloat16><<<blocks, 128, 0, ctx->stream>>>(a);
+    TB_LAUNCH_CHECK(ctx, "k_attn_join");
+    return TB_OK;
 }

@@ -16,9 +16,13 @@ struct AttnArgs {
     int nset, heads, kv_heads, group, dim, causal;
     int unit;                        // query tokens of a block
     float scale_log2;                // scale * log2(e): scores in powers of two
+    int nsplit;                      // ranges the keys are cut into
+    float* part;                     // [nsplit][nq][heads][dim] partial rows (normalised), null with one range
+    float* part_lse;                 // [nsplit][nq][heads] their log sums, base 2; -inf: no key, row not written
     int* err;
 };
 
-// 16-bit operands on tensor cores; nq, nk, nset > 0.
-size_t tb_attn_tc_workspace(const tb_ctx* ctx, int64_t nq, int64_t nk, int nset, int heads, int kv_heads, int dim);
-tb_status tb_attn_tc_launch(tb_ctx* ctx, const AttnArgs& args, tb_dtype dtype, tb_dtype out_dtype, void* workspace);
+// The plan of a kernel that may cut the keys: how many ranges.
+int tb_attn_tc_nsplit(const tb_ctx* ctx, int64_t nq, int64_t nk, int nset, int heads, int kv_heads, int dim);
+// 16-bit operands on tensor cores; nq, nk, nset > 0. args.nsplit as planned, part and part_lse set.
+tb_status tb_attn_tc_launch(tb_ctx* ctx, const AttnArgs& args, tb_dtype dtype, tb_dtype out_dtype);

@@ -25,7 +25,7 @@
 // left. One warp finds the tiles in the tables of sets.
 //
 // With few CTAs the keys are cut into `nsplit` ranges, which leave partial rows (32 bits, normalised,
-// with their log sums) that k_attn_join adds up in a fixed order.
+// with their log sums) that are added up in a fixed order (k_attn_join in tb_attention.cu).
 #include "tb_packed.cuh"
 #include "tb_tc_ptx.cuh"
 
@@ -49,9 +49,7 @@ constexpr int kBufs = 3;               // S buffers
 constexpr float kRaise = 8.f;          // the reference follows when a block's maximum is 2^8 above it
 struct TcArgs {
     AttnArgs a;
-    float* part;                       // [nsp][nq][heads][dim] partial rows, null without splits
-    float* part_lse;                   // [nsp][nq][heads], base 2
-    int nsplit, tile_tokens;           // key ranges; tokens of a 128-row tile
+    int tile_tokens;                   // tokens of a 128-row tile
     int wide;                          // output rows (or partial rows) start at multiples of 32 bytes
     uint32_t idesc_s, idesc_o, q_bytes;   // q_bytes: what one tile's boxes deliver
 };
@@ -71,17 +69,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
                  " [%0], [%1, {%2, %3, %4}], [%5];"
                  :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
-}
-// Shared-memory descriptors of tiles in the 128-byte swizzle: low word (address >> 4) | leading
-// offset << 16, high word 8-row groups 1024 bytes apart. Q and K have their K dimension (the head's
-// columns) contiguous; V is the B operand with N (the head's columns) contiguous, its boxes of 64
-// columns 16384 bytes apart.
-__device__ __forceinline__ uint64_t desc64(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
-__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, float* v) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
-                   "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
-                 : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, float* v) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -324,8 +311,8 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
             for (uint32_t k = 0;; ++k) {
                 const bool over = number == 0xffffffffu;         // none left to take over
                 uint32_t idx = over ? 0 : number;
-                const int split = idx % p.nsplit;
-                idx /= p.nsplit;
+                const int split = idx % a.nsplit;
+                idx /= a.nsplit;
                 const int kvh = idx % a.kv_heads;
                 const uint32_t piece = idx / a.kv_heads;
                 while (!over && piece >= base + total && set0 + 32 < a.nset) {
@@ -356,8 +343,8 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 o.first = (int)(a.causal ? cs - 1 - at : at) * a.unit;
                 const int end = a.causal ? max(0, min(o.nk, min(o.first + a.unit, o.nq) + o.nk - o.nq)) : o.nk;
                 const int all = (end + kKeys - 1) / kKeys;
-                o.blk0 = (int)((int64_t)all * split / p.nsplit);
-                o.n = (int)((int64_t)all * (split + 1) / p.nsplit) - o.blk0;
+                o.blk0 = (int)((int64_t)all * split / a.nsplit);
+                o.n = (int)((int64_t)all * (split + 1) / a.nsplit) - o.blk0;
                 o.kvh = kvh;
                 o.split = split;
                 o.end = over ? 1 : 0;
@@ -665,10 +652,10 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
             const int64_t row = (int64_t)job->q0 + t;
             const int64_t at = ((int64_t)job->split * a.nq + row) * a.heads + h;
             if (valid && wg == 0) {
-                if (p.part) p.part_lse[at] = lg;
+                if (a.part) a.part_lse[at] = lg;
                 else if (a.lse) a.lse[row * a.heads + h] = lg * 0.69314718055994530942f;
             }
-            float* part = p.part + at * a.dim;
+            float* part = a.part + at * a.dim;
             O* out = reinterpret_cast<O*>(a.out) + row * a.out_row + (int64_t)h * a.out_head;
             // each warpgroup writes half of the head's columns
             constexpr int W = D / 2;
@@ -689,10 +676,10 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                         }
                     }
                 }
-                if (!valid || (p.part && none)) continue;
+                if (!valid || (a.part && none)) continue;
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = none ? 0.f : o[e] * inv;
-                if (p.part) store_row<float>(part + q, o, a.dim - q, p.wide);
+                if (a.part) store_row<float>(part + q, o, a.dim - q, p.wide);
                 else store_row<O>(out + q, o, a.dim - q, p.wide);
             }
             if (n > 0) ++tiles;
@@ -730,54 +717,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 k_attn_pair(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
             const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TcArgs p) {
     attn_tc<T, O, 128, true>(qmap, kmap, vmap, p);
-}
-
-// Joins the partial rows: with lg_s the base-2 log sum of part s and M their maximum,
-//   out = sum_s 2^(lg_s - M) out_s / sum_s 2^(lg_s - M),  lse = (M + log2(that sum)) / log2(e).
-// A warp a row and head, parts in order.
-template <class O>
-__global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ TcArgs p, int nsp) {
-    const AttnArgs& a = p.a;
-    const int lane = threadIdx.x & 31;
-    int64_t lo = 0, hi = a.nq;
-    if (a.q_off) {
-        lo = min(max((int64_t)a.q_off[0], (int64_t)0), a.nq);
-        hi = min((int64_t)a.q_off[a.nset], a.nq);
-    }
-    const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int64_t row = at / a.heads, h = at % a.heads;
-    if (row < lo || row >= hi) return;
-    const int64_t step = a.nq * a.heads;
-    float mx = -INFINITY;
-    for (int s = lane; s < nsp; s += 32) mx = fmaxf(mx, p.part_lse[s * step + at]);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-    float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    const int c0 = lane * 4;
-    // a log sum that is no number does not show in the maximum: it goes by its weight
-    for (int s = 0; s < nsp; ++s) {
-        const float lg = p.part_lse[s * step + at];
-        if (lg == -INFINITY) continue;              // no key here, nothing was written
-        const float w = exp2f(lg - mx);
-        sum += w;
-        if (c0 < a.dim) {
-            const float4 v = *reinterpret_cast<const float4*>(p.part + (s * step + at) * a.dim + c0);
-            o[0] = fmaf(w, v.x, o[0]);
-            o[1] = fmaf(w, v.y, o[1]);
-            o[2] = fmaf(w, v.z, o[2]);
-            o[3] = fmaf(w, v.w, o[3]);
-        }
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (lane == 0 && a.lse) a.lse[at] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994530942f;
-    if (c0 >= a.dim) return;
-    O* out = reinterpret_cast<O*>(a.out) + row * a.out_row + h * a.out_head + c0;
-    if (sizeof(O) == 4) {
-        *reinterpret_cast<float4*>(out) = make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-    } else {
-        using H = typename std::conditional<sizeof(O) == 4, __half, O>::type;
-        *reinterpret_cast<uint2*>(out) = make_uint2(pack2(o[0] * inv, o[1] * inv, H()), pack2(o[2] * inv, o[3] * inv, H()));
-    }
 }
 
 struct Plan {
@@ -836,39 +775,27 @@ tb_status launch(tb_ctx* ctx, const TcArgs& p, const Plan& l, const CUtensorMap&
     else if (wide) k_attn_tc<T, O, 128><<<grid, kThreads, sm, ctx->stream>>>(qm, km, vm, p);
     else k_attn_tc<T, O, 64><<<grid, kThreads, sm, ctx->stream>>>(qm, km, vm, p);
     TB_LAUNCH_CHECK(ctx, "k_attn_tc");
-    if (p.part) {
-        k_attn_join<O><<<(unsigned)((p.a.nq * p.a.heads + 7) / 8), 256, 0, ctx->stream>>>(p, l.nsplit);
-        TB_LAUNCH_CHECK(ctx, "k_attn_join");
-    }
     return TB_OK;
 }
 
 }  // namespace
 
-size_t tb_attn_tc_workspace(const tb_ctx* ctx, int64_t nq, int64_t nk, int nset, int heads, int kv_heads, int dim) {
-    if (nq <= 0 || nk <= 0 || nset <= 0) return 0;
-    const Plan l = attn_plan(ctx->num_sms, nq, nk, nset, kv_heads, heads / kv_heads, dim);
-    return l.nsplit > 1 ? (size_t)l.nsplit * nq * heads * (dim + 1) * sizeof(float) : 0;
+int tb_attn_tc_nsplit(const tb_ctx* ctx, int64_t nq, int64_t nk, int nset, int heads, int kv_heads, int dim) {
+    return attn_plan(ctx->num_sms, nq, nk, nset, kv_heads, heads / kv_heads, dim).nsplit;
 }
 
-tb_status tb_attn_tc_launch(tb_ctx* ctx, const AttnArgs& args, tb_dtype dtype, tb_dtype out_dtype, void* workspace) {
+tb_status tb_attn_tc_launch(tb_ctx* ctx, const AttnArgs& args, tb_dtype dtype, tb_dtype out_dtype) {
     TcArgs p{};
     p.a = args;
     const AttnArgs& a = p.a;
     const Plan l = attn_plan(ctx->num_sms, a.nq, a.nk, a.nset, a.kv_heads, a.group, a.dim);
-    if (2 * l.items > INT32_MAX || (l.nsplit > 1 && (a.nq * a.heads + 7) / 8 > INT32_MAX))
-        return tb_fail(ctx, TB_ERR_TOO_LARGE, "tb_attention: too many rows times heads");
+    if (2 * l.items > INT32_MAX) return tb_fail(ctx, TB_ERR_TOO_LARGE, "tb_attention: too many rows times heads");
     p.a.unit = l.unit;
     p.tile_tokens = l.tile_tokens;
-    p.nsplit = l.nsplit;
-    if (l.nsplit > 1) {
-        p.part = reinterpret_cast<float*>(workspace);
-        p.part_lse = p.part + (size_t)l.nsplit * a.nq * a.heads * a.dim;
-    }
     {
         const int64_t size = (int64_t)tb_dtype_size(out_dtype);
         const bool rows = (reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.out_row * size) | (uintptr_t)(a.out_head * size)) % 32 == 0;
-        p.wide = l.nsplit > 1 ? a.dim % 8 == 0 && reinterpret_cast<uintptr_t>(workspace) % 32 == 0 : rows;
+        p.wide = a.part ? reinterpret_cast<uintptr_t>(a.part) % 32 == 0 : rows;
     }
     const uint32_t fmt = dtype == TB_BF16 ? 1u : 0u;
     const uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((l.pair ? 16u : 8u) << 24);
