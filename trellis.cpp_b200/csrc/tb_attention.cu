@@ -340,6 +340,7 @@ tb_status attn_args(tb_ctx* ctx, const tb_attention_params* p, AttnArgs& a) {
 static int attn_nsplit(const tb_ctx* ctx, tb_dtype dtype, int64_t nq, int64_t nk, int nset, int heads, int kv_heads, int dim) {
     if (nq <= 0 || nk <= 0 || nset <= 0) return 1;
     if (dtype == TB_F32) return cc_nsplit(ctx, nq, nk, nset, kv_heads, heads / kv_heads);
+    if (tb_attn_few(nq, nset, heads / kv_heads)) return tb_attn_few_nsplit(ctx, nq, nk, nset, kv_heads, heads / kv_heads);
     return tb_attn_tc_nsplit(ctx, nq, nk, nset, heads, kv_heads, dim);
 }
 
@@ -368,8 +369,10 @@ extern "C" tb_status tb_attention(tb_ctx* ctx, const tb_attention_params* p) {
     }
     tb_device_guard guard;
     TB_CUDA_TRY(ctx, guard.enter(ctx->device));
-    // without key rows there is nothing to describe to the tensor cores' loads: every row is 0
-    if (p->dtype != TB_F32 && a.nk > 0) s = tb_attn_tc_launch(ctx, a, p->dtype, p->out_dtype);
+    // without key rows there is nothing to describe to the TMA loads: every row is 0
+    if (p->dtype != TB_F32 && a.nk > 0)
+        s = tb_attn_few(a.nq, a.nset, a.group) ? tb_attn_few_launch(ctx, a, p->dtype, p->out_dtype)
+                                               : tb_attn_tc_launch(ctx, a, p->dtype, p->out_dtype);
     else if (p->out_dtype == TB_F16) s = launch_cc<__half, 128>(ctx, a);
     else if (p->out_dtype == TB_BF16) s = launch_cc<__nv_bfloat16, 128>(ctx, a);
     else s = a.dim <= 64 ? launch_cc<float, 64>(ctx, a) : launch_cc<float, 128>(ctx, a);

@@ -65,11 +65,6 @@ template <int D, bool PAIR> struct Geom {
     static constexpr size_t kSmem = kUsed + kSlack;
 };
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-                 " [%0], [%1, {%2, %3, %4}], [%5];"
-                 :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
-}
 __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, float* v) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
                  "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -741,26 +736,6 @@ Plan attn_plan(int num_sms, int64_t nq, int64_t nk, int nset, int kv_heads, int 
     return l;
 }
 
-tb_status encode(tb_ctx* ctx, CUtensorMap* map, tb_dtype dtype, const void* base, int dim, int64_t heads, int64_t head,
-                 int64_t rows, int64_t row, uint32_t box_heads, uint32_t box_rows) {
-    if (!ctx->encode_tiled) {
-        void* fn = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        TB_CUDA_TRY(ctx, cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
-        if (!fn || q != cudaDriverEntryPointSuccess)
-            return tb_fail(ctx, TB_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
-        ctx->encode_tiled = fn;
-    }
-    const cuuint64_t gdim[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)rows};
-    const cuuint64_t stride[2] = {(cuuint64_t)(heads > 1 ? head : dim) * 2, (cuuint64_t)(rows > 1 ? row : dim) * 2};
-    const cuuint32_t box[3] = {64, box_heads, box_rows}, es[3] = {1, 1, 1};
-    const CUresult cr = reinterpret_cast<EncodeTiledFn>(ctx->encode_tiled)(
-        map, dtype == TB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
-        gdim, stride, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return cr == CUDA_SUCCESS ? TB_OK : tb_fail(ctx, TB_ERR_CUDA, "cuTensorMapEncodeTiled failed for tb_attention");
-}
-
 template <class T, class O>
 tb_status launch(tb_ctx* ctx, const TcArgs& p, const Plan& l, const CUtensorMap& qm, const CUtensorMap& km,
                  const CUtensorMap& vm) {
@@ -779,6 +754,26 @@ tb_status launch(tb_ctx* ctx, const TcArgs& p, const Plan& l, const CUtensorMap&
 }
 
 }  // namespace
+
+tb_status tb_attn_encode(tb_ctx* ctx, CUtensorMap* map, tb_dtype dtype, const void* base, int dim, int64_t heads, int64_t head,
+                         int64_t rows, int64_t row, uint32_t box_heads, uint32_t box_rows) {
+    if (!ctx->encode_tiled) {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        TB_CUDA_TRY(ctx, cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
+        if (!fn || q != cudaDriverEntryPointSuccess)
+            return tb_fail(ctx, TB_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
+        ctx->encode_tiled = fn;
+    }
+    const cuuint64_t gdim[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t stride[2] = {(cuuint64_t)(heads > 1 ? head : dim) * 2, (cuuint64_t)(rows > 1 ? row : dim) * 2};
+    const cuuint32_t box[3] = {64, box_heads, box_rows}, es[3] = {1, 1, 1};
+    const CUresult cr = reinterpret_cast<EncodeTiledFn>(ctx->encode_tiled)(
+        map, dtype == TB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
+        gdim, stride, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return cr == CUDA_SUCCESS ? TB_OK : tb_fail(ctx, TB_ERR_CUDA, "cuTensorMapEncodeTiled failed for tb_attention");
+}
 
 int tb_attn_tc_nsplit(const tb_ctx* ctx, int64_t nq, int64_t nk, int nset, int heads, int kv_heads, int dim) {
     return attn_plan(ctx->num_sms, nq, nk, nset, kv_heads, heads / kv_heads, dim).nsplit;
@@ -804,9 +799,9 @@ tb_status tb_attn_tc_launch(tb_ctx* ctx, const AttnArgs& args, tb_dtype dtype, t
     p.idesc_o = base | (1u << 16) | ((l.pair ? 16u : (uint32_t)((a.dim + 15) / 16 * 2)) << 17);
     p.q_bytes = (uint32_t)((a.dim <= 64 ? 1 : 2) * 128 * a.group * l.tile_tokens);
     CUtensorMap qm, km, vm;
-    tb_status s = encode(ctx, &qm, dtype, a.q, a.dim, a.heads, a.q_head, a.nq, a.q_row, (uint32_t)a.group, (uint32_t)l.tile_tokens);
-    if (s == TB_OK) s = encode(ctx, &km, dtype, a.k, a.dim, a.kv_heads, a.k_head, a.nk, a.k_row, 1, l.pair ? 64 : kKeys);
-    if (s == TB_OK) s = encode(ctx, &vm, dtype, a.v, a.dim, a.kv_heads, a.v_head, a.nk, a.v_row, 1, kKeys);
+    tb_status s = tb_attn_encode(ctx, &qm, dtype, a.q, a.dim, a.heads, a.q_head, a.nq, a.q_row, (uint32_t)a.group, (uint32_t)l.tile_tokens);
+    if (s == TB_OK) s = tb_attn_encode(ctx, &km, dtype, a.k, a.dim, a.kv_heads, a.k_head, a.nk, a.k_row, 1, l.pair ? 64 : kKeys);
+    if (s == TB_OK) s = tb_attn_encode(ctx, &vm, dtype, a.v, a.dim, a.kv_heads, a.v_head, a.nk, a.v_row, 1, kKeys);
     if (s != TB_OK) return s;
     if (dtype == TB_F16)
         return out_dtype == TB_F32 ? launch<__half, float>(ctx, p, l, qm, km, vm) : launch<__half, __half>(ctx, p, l, qm, km, vm);
