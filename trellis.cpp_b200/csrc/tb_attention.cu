@@ -245,16 +245,17 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ AttnA
     const float w = lg == -INFINITY ? 0.f : exp2f(lg - mx);
     const int c0 = lane * 4;
     float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+    const float* part = a.part + at * a.dim + (c0 < a.dim ? c0 : 0);
+#pragma unroll 8
     for (int s = 0; s < a.nsplit; ++s) {
-        const float ws = __shfl_sync(0xffffffffu, w, s), ls = __shfl_sync(0xffffffffu, lg, s);
+        const float4 v = *reinterpret_cast<const float4*>(part + s * step * a.dim);
+        const float ws = __shfl_sync(0xffffffffu, w, s);
+        const bool written = __shfl_sync(0xffffffffu, lg, s) != -INFINITY;     // else whatever was there
         sum += ws;
-        if (ls == -INFINITY || c0 >= a.dim) continue;        // no key here, nothing was written
-        const float4 v = *reinterpret_cast<const float4*>(a.part + (s * step + at) * a.dim + c0);
-        o[0] = fmaf(ws, v.x, o[0]);
-        o[1] = fmaf(ws, v.y, o[1]);
-        o[2] = fmaf(ws, v.z, o[2]);
-        o[3] = fmaf(ws, v.w, o[3]);
+        o[0] = written ? fmaf(ws, v.x, o[0]) : o[0];
+        o[1] = written ? fmaf(ws, v.y, o[1]) : o[1];
+        o[2] = written ? fmaf(ws, v.z, o[2]) : o[2];
+        o[3] = written ? fmaf(ws, v.w, o[3]) : o[3];
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     if (lane == 0 && a.lse) a.lse[at] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994530942f;

@@ -291,7 +291,7 @@ bool tb_attn_few(int64_t nq, int nset, int group) { return group <= kFewRows && 
 int tb_attn_few_nsplit(const tb_ctx* ctx, int64_t nq, int64_t nk, int nset, int kv_heads, int group) {
     const int unit = kFewRows / group;
     const int64_t ctas = std::max<int64_t>((nq + unit - 1) / unit, std::min<int64_t>(nset, nq)) * kv_heads;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({8ll * ctx->num_sms / ctas, nk / nset / 256, 32}));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({4ll * ctx->num_sms / ctas, nk / nset / 256, 32}));
 }
 
 tb_status tb_attn_few_launch(tb_ctx* ctx, const AttnArgs& args, tb_dtype dtype, tb_dtype out_dtype) {

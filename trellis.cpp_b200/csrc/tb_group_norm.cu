@@ -65,7 +65,7 @@ struct Running {
 // 8 values of 16-bit or 32-bit type as they come from memory: 16-byte words, unpacked when used, so
 // that a batch of rows in flight takes few registers.
 template <class T> struct Raw8 {
-    static constexpr int kRows = 4;      // rows of a batch, in flight together
+    static constexpr int kRows = 8;      // rows of a batch, in flight together
     uint4 w;
     __device__ void load(const T* p) { w = *reinterpret_cast<const uint4*>(p); }
     __device__ void load_last(const T* p) { w = __ldcs(reinterpret_cast<const uint4*>(p)); }
@@ -264,7 +264,7 @@ __device__ __forceinline__ void gn_write(const GnArgs& a, const f2* mean, const 
 }
 
 template <class T>
-__global__ void __launch_bounds__(kGnThreads, sizeof(T) == 4 ? 3 : 4) k_gn_stats(const __grid_constant__ GnArgs a) {
+__global__ void __launch_bounds__(kGnThreads, 2) k_gn_stats(const __grid_constant__ GnArgs a) {
     __shared__ Item it;
     __shared__ uint32_t scan[32];
     extern __shared__ float4 ent[];
@@ -396,15 +396,16 @@ int gn_slab(int c, int cg, int size) {
     return slab;
 }
 
-constexpr int kGnSmall = 4096;
+constexpr int kGnSmall = 4096, kGnPieces = 8;
 
-// Rows of a piece: about eight pieces an SM over the whole array, 16 rows at least.
-int gn_unit(int num_sms, int64_t n) {
-    const int64_t pieces = 8ll * num_sms;
+// Rows of a piece: eight pieces an SM over the whole array, those that the sets' ends add included, so
+// that the last wave of blocks is a full one; 16 rows at least.
+int gn_unit(int num_sms, int64_t n, int nset) {
+    const int64_t pieces = kGnPieces * num_sms - std::min(nset, 4 * num_sms);
     return (int)std::max<int64_t>(16, (n + pieces - 1) / pieces);
 }
 int64_t gn_pieces(int num_sms, int64_t n, int nset) {
-    const int unit = gn_unit(num_sms, n);
+    const int unit = gn_unit(num_sms, n, nset);
     return (n + unit - 1) / unit + nset;
 }
 
@@ -471,7 +472,7 @@ extern "C" tb_status tb_group_norm(tb_ctx* ctx, const void* x, tb_dtype x_dtype,
     a.nset = nset;
     a.c = c;
     a.groups = groups;
-    a.unit = gn_unit(ctx->num_sms, n);
+    a.unit = gn_unit(ctx->num_sms, n, nset);
     a.slab = n <= kGnSmall ? gn_slab(c, c / groups, (int)tb_dtype_size(x_dtype)) : 0;
     a.eps = eps;
     a.act = act == TB_EPI_SILU;
