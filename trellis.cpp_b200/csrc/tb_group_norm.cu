@@ -13,7 +13,8 @@
 // squared deviations with its running ones (no difference of large sums, so a mean far from zero
 // costs no digits); entries are joined as
 //   mean = sum n_i mean_i / N,  M2 = sum M2_i + sum n_i (mean_i - mean)^2
-// always in the same order, so results repeat to the bit. Bound by memory.
+// always in the same order, so results repeat to the bit. Bound by memory: 262144 x 512 of bf16 in
+// 8 sets take 148 us, 58 of them for the statistics (4.6 TB/s).
 #include "tb_packed.cuh"
 
 #include <algorithm>
@@ -24,6 +25,9 @@ using namespace tbpk;
 
 constexpr int kGnThreads = 256;
 constexpr int kGnMaxC = 2048;
+// The bytes at the array's end that k_gn_stats leaves in L2 for k_gn_apply, which begins with them; the
+// others go first. (262144 x 512 of bf16: 150 us with 60 MB, 152 with 90 MB, 156 without hints.)
+constexpr int64_t kGnKeep = 60 << 20;
 
 struct GnArgs {
     const void* x;
@@ -32,7 +36,8 @@ struct GnArgs {
     const float* w;
     const float* b;
     int64_t n;
-    int nset, c, groups, unit, slab;
+    int nset, c, groups, slab;
+    int unit, unit_out;   // rows of a piece of k_gn_stats, of k_gn_apply
     float eps;
     int act;
     float2* part;     // [pieces][groups] mean, M2
@@ -62,12 +67,26 @@ struct Running {
     }
 };
 
+// 16 bytes with a policy for their stay in L2.
+__device__ __forceinline__ uint4 load16(const void* p, uint64_t policy) {
+    uint4 v;
+    asm volatile("ld.global.L2::cache_hint.v4.b32 {%0,%1,%2,%3}, [%4], %5;"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p), "l"(policy) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint64_t l2_policy(bool keep) {
+    uint64_t normal, first;
+    asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(normal));
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(first));
+    return keep ? normal : first;
+}
+
 // 8 values of 16-bit or 32-bit type as they come from memory: 16-byte words, unpacked when used, so
 // that a batch of rows in flight takes few registers.
 template <class T> struct Raw8 {
     static constexpr int kRows = 8;      // rows of a batch, in flight together
     uint4 w;
-    __device__ void load(const T* p) { w = *reinterpret_cast<const uint4*>(p); }
+    __device__ void load(const T* p, uint64_t policy) { w = load16(p, policy); }
     __device__ void load_last(const T* p) { w = __ldcs(reinterpret_cast<const uint4*>(p)); }
     __device__ void get(f2* v) const {
         float x[8];
@@ -79,9 +98,10 @@ template <class T> struct Raw8 {
 template <> struct Raw8<float> {
     static constexpr int kRows = 4;
     float4 a, b;
-    __device__ void load(const float* p) {
-        a = reinterpret_cast<const float4*>(p)[0];
-        b = reinterpret_cast<const float4*>(p)[1];
+    __device__ void load(const float* p, uint64_t policy) {
+        const uint4 u = load16(p, policy), v = load16(p + 4, policy);
+        a = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+        b = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
     }
     __device__ void load_last(const float* p) {
         a = __ldcs(reinterpret_cast<const float4*>(p));
@@ -97,7 +117,8 @@ template <> struct Raw8<float> {
 
 // Rows r, r + step, ... below r1 of the thread's 8 channels (x: of row 0).
 template <class T>
-__device__ __forceinline__ void gn_read(Running& s, const T* x, int64_t c, int64_t r, int64_t r1, int64_t step) {
+__device__ __forceinline__ void gn_read(Running& s, const T* x, int64_t c, int64_t r, int64_t r1, int64_t step,
+                                        uint64_t policy) {
     constexpr int R = Raw8<T>::kRows;
     const f2 zero = pack(0.f, 0.f);
     for (; r < r1; r += R * step) {
@@ -106,7 +127,7 @@ __device__ __forceinline__ void gn_read(Running& s, const T* x, int64_t c, int64
         f2 m[4] = {zero, zero, zero, zero}, d2[4] = {zero, zero, zero, zero}, v[4];
         if (k == R) {
 #pragma unroll
-            for (int q = 0; q < R; ++q) raw[q].load(x + (r + q * step) * c);
+            for (int q = 0; q < R; ++q) raw[q].load(x + (r + q * step) * c, policy);
 #pragma unroll
             for (int q = 0; q < R; ++q) {
                 raw[q].get(v);
@@ -127,7 +148,7 @@ __device__ __forceinline__ void gn_read(Running& s, const T* x, int64_t c, int64
         } else {                         // the last rows, fewer than a batch, in flight together as well
 #pragma unroll
             for (int q = 0; q < R; ++q)
-                if (q < k) raw[q].load(x + (r + q * step) * c);
+                if (q < k) raw[q].load(x + (r + q * step) * c, policy);
             // the share of a third or so is not exact: it multiplies differences from the first row
             f2 first[4];
             raw[0].get(first);
@@ -158,8 +179,7 @@ __device__ __forceinline__ void gn_read(Running& s, const T* x, int64_t c, int64
 
 // A mean of entries (mean_i, M2_i, n_i) in two rounds: m from the plain sum, a few steps off, then
 // d = sum n_i (mean_i - m), which is near 0 and so keeps its digits, and q = sum M2_i + n_i (mean_i - m)^2;
-// the mean is m + d / N, rounded once, and M2 = q - d^2 / N. (The same in 64 bits took 6 us longer for
-// 1024 entries a group.)
+// the mean is m + d / N, rounded once, and M2 = q - d^2 / N.
 __device__ __forceinline__ void gn_add(float off, float m2, float n, float& d, float& q) {
     d = fmaf(n, off, d);
     q += fmaf(n, off * off, m2);
@@ -172,8 +192,7 @@ __device__ __forceinline__ void gn_settle(float& m, float& m2, float d, float q,
 
 // Joins the block's threads: `lanes` row lanes of tc threads, 8 channels a thread. Where groups are
 // whole threads (cg % 8 == 0) a thread joins its channels first. A group's entries lie together and a
-// team of up to 32 threads adds them up; put(g, mean, M2) by its first thread. (With whole-number
-// divisions for each entry's place the join took 27 of 72 us of a pass over 262144 x 512.)
+// team of up to 32 threads adds them up; put(g, mean, M2) by its first thread.
 template <class F>
 __device__ __forceinline__ void gn_join(const Running& s, int ry, int tx, int lanes, int groups, int cg, float rows,
                                         float4* ent, F put) {
@@ -275,7 +294,8 @@ __global__ void __launch_bounds__(kGnThreads, 2) k_gn_stats(const __grid_constan
     const int64_t r0 = it.lo + (int64_t)it.item * a.unit, r1 = min(it.hi, r0 + a.unit);
     Running s;
     s.clear();
-    if (ry < lanes) gn_read<T>(s, reinterpret_cast<const T*>(a.x) + tx * 8, a.c, r0 + ry, r1, lanes);
+    const uint64_t policy = l2_policy((a.n - r0) * a.c * (int64_t)sizeof(T) < kGnKeep);
+    if (ry < lanes) gn_read<T>(s, reinterpret_cast<const T*>(a.x) + tx * 8, a.c, r0 + ry, r1, lanes, policy);
     float2* part = a.part + (int64_t)blockIdx.x * a.groups;
     gn_join(s, ry, tx, lanes, a.groups, a.c / a.groups, (float)(r1 - r0), ent,
             [&](int g, float m, float q) { part[g] = make_float2(m, q); });
@@ -353,12 +373,12 @@ template <class T, class O>
 __global__ void __launch_bounds__(kGnThreads, sizeof(T) == 4 ? 3 : 4) k_gn_apply(const __grid_constant__ GnArgs a) {
     __shared__ Item it;
     __shared__ uint32_t scan[32];
-    find_item(a.off, a.nset, a.n, a.unit, gridDim.x - 1 - blockIdx.x, a.err, &it, scan);
+    find_item(a.off, a.nset, a.n, a.unit_out, gridDim.x - 1 - blockIdx.x, a.err, &it, scan);
     if (it.set < 0) return;
     const int tc = a.c / 8, lanes = kGnThreads / tc;
     const int ry = threadIdx.x / tc, ch = (threadIdx.x % tc) * 8;
     if (ry >= lanes) return;
-    const int64_t r0 = it.lo + (int64_t)it.item * a.unit, r1 = min(it.hi, r0 + a.unit);
+    const int64_t r0 = it.lo + (int64_t)it.item * a.unit_out, r1 = min(it.hi, r0 + a.unit_out);
     f2 mean[4], f[4], b[4];
     gn_factors(a, a.stat + (int64_t)it.set * a.groups, ch, 0, mean, f, b);
     gn_write<T, O>(a, mean, f, b, ch, r0 + ry, r1, lanes);
@@ -376,7 +396,7 @@ __global__ void __launch_bounds__(kGnThreads) k_gn_small(const __grid_constant__
     const int ry = threadIdx.x / tc, tx = threadIdx.x % tc, ch0 = blockIdx.y * a.slab, ch = ch0 + tx * 8;
     Running s;
     s.clear();
-    if (ry < lanes) gn_read<T>(s, reinterpret_cast<const T*>(a.x) + ch, a.c, lo + ry, hi, lanes);
+    if (ry < lanes) gn_read<T>(s, reinterpret_cast<const T*>(a.x) + ch, a.c, lo + ry, hi, lanes, l2_policy(true));
     const float count = (float)(hi - lo) * cg;
     gn_join(s, ry, tx, lanes, a.slab / cg, cg, (float)(hi - lo), ent,
             [&](int g, float m, float q) { stat[g] = make_float2(m, 1.f / sqrtf(q / count + a.eps)); });
@@ -396,21 +416,25 @@ int gn_slab(int c, int cg, int size) {
     return slab;
 }
 
-constexpr int kGnSmall = 4096, kGnPieces = 8;
+// One launch where three would take longer than a second reading by few blocks (800 x 128: 7 us in one,
+// 12 in three; 8192 x 512: 24 and 17).
+constexpr int kGnSmall = 4096;
+// Pieces an SM: one wave of k_gn_stats's blocks, whose join costs as much as some rows (16384 x 512:
+// 22 us with two, 32 with eight); one of k_gn_apply's, or two smaller ones where the array is larger
+// than L2 and the pass long enough to have a tail (65536 x 512: 47 us with four, 49 with eight;
+// 262144 x 512: 151 and 148).
+constexpr int kGnPieces = 2;
+int gn_pieces_out(int64_t n, int c, tb_dtype t) { return n * c * (int64_t)tb_dtype_size(t) > 2 * kGnKeep ? 8 : 4; }
 
-// Rows of a piece: eight pieces an SM over the whole array, those that the sets' ends add included, so
-// that the last wave of blocks is a full one; 16 rows at least.
-int gn_unit(int num_sms, int64_t n, int nset) {
-    const int64_t pieces = kGnPieces * num_sms - std::min(nset, 4 * num_sms);
+// Rows of a piece, so that the sets' ends included there are `per` pieces an SM, and 16 rows at least.
+int gn_unit(int num_sms, int64_t n, int nset, int per) {
+    const int64_t pieces = (int64_t)per * num_sms - std::min(nset, per * num_sms / 2);
     return (int)std::max<int64_t>(16, (n + pieces - 1) / pieces);
 }
-int64_t gn_pieces(int num_sms, int64_t n, int nset) {
-    const int unit = gn_unit(num_sms, n, nset);
-    return (n + unit - 1) / unit + nset;
-}
+int64_t gn_pieces(int64_t n, int nset, int unit) { return (n + unit - 1) / unit + nset; }
 
 template <class T>
-void launch_gn(const GnArgs& a, bool f32_out, int64_t pieces, cudaStream_t st) {
+void launch_gn(const GnArgs& a, bool f32_out, cudaStream_t st) {
     if (a.slab) {
         const int cg = a.c / a.groups;
         const size_t sm = (size_t)(kGnThreads / (a.slab / 8)) * a.slab / (cg % 8 == 0 ? 8 : 1) * sizeof(float4);
@@ -420,18 +444,19 @@ void launch_gn(const GnArgs& a, bool f32_out, int64_t pieces, cudaStream_t st) {
         return;
     }
     const size_t sm = (size_t)(kGnThreads / (a.c / 8)) * a.c / (a.c / a.groups % 8 == 0 ? 8 : 1) * sizeof(float4);
-    k_gn_stats<T><<<(unsigned)pieces, kGnThreads, sm, st>>>(a);
+    k_gn_stats<T><<<(unsigned)gn_pieces(a.n, a.nset, a.unit), kGnThreads, sm, st>>>(a);
     const unsigned gy = (unsigned)std::min(a.groups, std::max(1, 4096 / a.nset));
     k_gn_merge<<<dim3((unsigned)a.nset, gy), 128, 0, st>>>(a);
-    if (f32_out) k_gn_apply<T, float><<<(unsigned)pieces, kGnThreads, 0, st>>>(a);
-    else k_gn_apply<T, T><<<(unsigned)pieces, kGnThreads, 0, st>>>(a);
+    const unsigned blocks = (unsigned)gn_pieces(a.n, a.nset, a.unit_out);
+    if (f32_out) k_gn_apply<T, float><<<blocks, kGnThreads, 0, st>>>(a);
+    else k_gn_apply<T, T><<<blocks, kGnThreads, 0, st>>>(a);
 }
 
 }  // namespace
 
 extern "C" size_t tb_group_norm_workspace_bytes(const tb_ctx* ctx, int64_t n, int c, int groups, int nset) {
     if (!ctx || n <= 0 || c < 1 || groups < 1 || c % groups != 0 || nset < 1 || n <= kGnSmall) return 0;
-    return (size_t)(gn_pieces(ctx->num_sms, n, nset) + nset) * groups * sizeof(float2);
+    return (size_t)(gn_pieces(n, nset, gn_unit(ctx->num_sms, n, nset, kGnPieces)) + nset) * groups * sizeof(float2);
 }
 
 extern "C" tb_status tb_group_norm(tb_ctx* ctx, const void* x, tb_dtype x_dtype, const int32_t* offsets, int nset,
@@ -461,7 +486,6 @@ extern "C" tb_status tb_group_norm(tb_ctx* ctx, const void* x, tb_dtype x_dtype,
     const size_t need = tb_group_norm_workspace_bytes(ctx, n, c, groups, nset);
     if (need && (!workspace || workspace_bytes < need || !tb_aligned16(workspace)))
         return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_group_norm: workspace too small or not 16-byte aligned");
-    const int64_t pieces = gn_pieces(ctx->num_sms, n, nset);
     GnArgs a{};
     a.x = x;
     a.out = out;
@@ -472,18 +496,19 @@ extern "C" tb_status tb_group_norm(tb_ctx* ctx, const void* x, tb_dtype x_dtype,
     a.nset = nset;
     a.c = c;
     a.groups = groups;
-    a.unit = gn_unit(ctx->num_sms, n, nset);
+    a.unit = gn_unit(ctx->num_sms, n, nset, kGnPieces);
+    a.unit_out = gn_unit(ctx->num_sms, n, nset, gn_pieces_out(n, c, x_dtype));
     a.slab = n <= kGnSmall ? gn_slab(c, c / groups, (int)tb_dtype_size(x_dtype)) : 0;
     a.eps = eps;
     a.act = act == TB_EPI_SILU;
     a.part = reinterpret_cast<float2*>(workspace);
-    a.stat = a.part + pieces * groups;
+    a.stat = a.part + gn_pieces(n, nset, a.unit) * groups;
     a.err = ctx->d_err;
     tb_device_guard guard;
     TB_CUDA_TRY(ctx, guard.enter(ctx->device));
-    if (x_dtype == TB_F32) launch_gn<float>(a, true, pieces, ctx->stream);
-    else if (x_dtype == TB_F16) launch_gn<__half>(a, out_dtype == TB_F32, pieces, ctx->stream);
-    else launch_gn<__nv_bfloat16>(a, out_dtype == TB_F32, pieces, ctx->stream);
+    if (x_dtype == TB_F32) launch_gn<float>(a, true, ctx->stream);
+    else if (x_dtype == TB_F16) launch_gn<__half>(a, out_dtype == TB_F32, ctx->stream);
+    else launch_gn<__nv_bfloat16>(a, out_dtype == TB_F32, ctx->stream);
     TB_LAUNCH_CHECK(ctx, "tb_group_norm");
     return TB_OK;
 }
