@@ -97,6 +97,72 @@ def test_few_queries_many_keys(tb, ql, kl, dtype):
         _check(ops, q, k, v, ref.offsets(ql), ref.offsets(kl), causal)
 
 
+FEW = [      # sets of 16 rows or fewer on average, with heads that share a key head counted as rows
+    ([1], [1], 1, 1),
+    ([1], [15], 16, 1),
+    ([3], [17], 4, 1),
+    ([2, 5, 1], [16, 63, 64], 6, 2),
+    ([1] * 5, [0, 65, 127, 3, 1000], 8, 2),
+    ([16, 16], [40, 700], 2, 2),
+    ([0, 0, 40, 0, 1], [9, 0, 500, 70, 2049], 3, 3),      # one set of more rows than a tile
+    ([7], [4099], 2, 1),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d", [8, 40, 64, 72, 128])
+@pytest.mark.parametrize("ql,kl,h,hk", FEW)
+def test_sets_of_few_rows(tb, ql, kl, h, hk, d, causal, dtype):
+    from trellis_cpp_b200 import ops
+    q, k, v = _inputs(d + len(ql), sum(ql), sum(kl), h, hk, d, dtype)
+    _check(ops, q, k, v, ref.offsets(ql), ref.offsets(kl), causal)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_rows_strides_and_float32_output(tb, dtype):
+    # new tokens as the views of one product, keys and values as the halves of a cache's rows, head-major
+    from trellis_cpp_b200 import ops
+    h, hk, d, kl = 8, 2, 128, [300, 1, 2000]
+    x, _, _ = _inputs(20, 3, 1, h + 2 * hk, 1, d, dtype)
+    cache, _, _ = _inputs(21, 2 * hk, 1, sum(kl), 1, d, dtype)
+    k, v = cache[:hk].transpose(0, 1), cache[hk:].transpose(0, 1)
+    qo, ko = [0, 1, 2, 3], ref.offsets(kl)
+    got = _check(ops, x[:, :h], k, v, qo, ko, True)
+    wide = _check(ops, x[:, :h], k, v, qo, ko, True, out_dtype=torch.float32)
+    assert torch.equal(wide.to(dtype), got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale,spread", [(1e-4, 1.0), (0.125, 20.0), (2.0, 3.0)])
+def test_few_rows_flat_steep_and_rising_scores(tb, scale, spread, dtype):
+    from trellis_cpp_b200 import ops
+    q, k, v = _inputs(22, 4, 3000, 2, 2, 64, dtype, spread)
+    _check(ops, q, k, v, [0, 1, 4], [0, 900, 3000], True, scale=scale)
+    k = (k.abs() * torch.linspace(0.1, 4, 3000, device="cuda")[:, None, None]).to(dtype)
+    _check(ops, q.abs(), k, v, [0, 1, 4], [0, 900, 3000], False, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_rows_where_the_next_set_holds_no_numbers(tb, dtype):
+    from trellis_cpp_b200 import ops
+    q, k, v = _inputs(23, 2, 2000, 4, 1, 128, dtype)
+    k[1003:] = math.nan
+    v[1003:] = math.inf
+    out = ops.attention(q, k, v, ref.table([0, 1, 2]), ref.table([0, 1003, 2000]))
+    want, _, wgt, reach = ref.attention(q[:1], k[:1003], v[:1003], [0, 1], [0, 1003], False, 128 ** -0.5)
+    tol = ref.attention_tolerance(want, wgt, reach, 128, 1003, dtype, dtype)
+    assert ref.close(out[:1], want, tol) <= 1.0
+    assert bool(torch.isnan(out[1:]).all())
+    k[1003:] = 0
+    k[5, 0, 3] = math.nan                          # in the first range of the keys, then in the last
+    assert bool(torch.isnan(ops.attention(q[:1], k[:1003], v[:1003])).all())
+    k[5] = 0
+    k[1002] = math.nan
+    assert bool(torch.isnan(ops.attention(q[:1], k[:1003], v[:1003])).all())
+    ops.check_device()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_many_sets(tb, dtype):
     from trellis_cpp_b200 import ops
@@ -282,6 +348,7 @@ def test_rows_far_apart(tb, dtype):
     kk.copy_(k)
     vv.copy_(v)
     assert torch.equal(ops.attention(q, kk, vv), ops.attention(q, k, v))
+    assert torch.equal(ops.attention(q[:5], kk, vv), ops.attention(q[:5], k, v))
     ops.check_device()
 
 
