@@ -1,13 +1,14 @@
 // Attention within packed sets of few query rows (bf16 / f16 operands): a new token or a few against
 // the keys so far. The mathematics and the entry point are in tb_attention.cu.
 //
-// Bound by reading the keys and values once, so the kernel is laid out for loads in flight: a CTA takes
-// 16 rows (a row is a token and one of the heads that share a key head) and a range of the keys, its
-// four warps every fourth 16 keys of them. A warp has a ring of its own that one lane fills by TMA,
-// runs its own softmax and meets the others at the end only. Its products are warp-level m16n8k16
-// MMAs: the rows fill one fragment, where the 128-row tiles of tb_attention_tc.cu would run the
-// softmax of 128 rows for them. 64 tokens of 32/8 heads of 128 against 2048 keys each: 83 us, 6.5 TB/s;
-// 16 against 1 to 8192 keys (63k): 57 us, 4.7 TB/s, the longest set's CTAs last.
+// Bound by reading the keys and values once, so the kernel is laid out for loads under way: a CTA takes
+// 16 rows (a row is a token and one of the heads that share a key head) and a range of the keys, its W
+// warps every W-th 16 keys of them. A warp has a ring of its own (24 KB) that one lane fills by TMA, runs
+// its own softmax and meets the others at the end only. Its products are warp-level m16n8k16 MMAs: the
+// rows fill one fragment, where the 128-row tiles of tb_attention_tc.cu would run the softmax of 128
+// rows for them. 64 tokens of 32/8 heads of 128 against 2048 keys each: 82 us, 6.5 TB/s; 16 against 1
+// to 8192 keys (63k): 54 us, 5.0 TB/s, the longest set's CTAs last. (The next step's scores before this
+// one's softmax: 61 us, the ring then holds one step less under way.)
 #include "tb_packed.cuh"
 #include "tb_tc_ptx.cuh"
 
@@ -20,9 +21,8 @@ namespace {
 using namespace tbtc;
 using namespace tbpk;
 
-constexpr int kFewRows = 16, kFewWarps = 4, kFewThreads = 32 * kFewWarps;
+constexpr int kFewRows = 16;
 constexpr int kStep = 16;              // keys of a warp's step
-constexpr int kBlock = kStep * kFewWarps;
 
 template <int D> struct FewGeom {
     static constexpr int kBoxes = D / 64;
@@ -30,15 +30,14 @@ template <int D> struct FewGeom {
     static constexpr int kBytes = 2 * kBoxes * kBox;              // a step's K and V
     static constexpr int kStages = 24576 / kBytes;
     static constexpr int kRing = kStages * kBytes;                // of a warp
-    static constexpr size_t kSmem = (size_t)kFewWarps * kRing + 1024;
 };
 
 __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, __nv_bfloat16) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, __half) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void load_frag(uint32_t addr, uint32_t* r) {
@@ -54,15 +53,16 @@ template <int D> __device__ __forceinline__ uint32_t word_at(uint32_t base, int 
     return base + (w >> 3) * FewGeom<D>::kBox + row * 128 + (((w ^ row) & 7) << 4);
 }
 
-template <class T, class O, int D>
-__global__ void __launch_bounds__(kFewThreads, 2)
+template <class T, class O, int D, int W>
+__global__ void __launch_bounds__(32 * W, 8 / W)
 k_attn_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnArgs a) {
     using G = FewGeom<D>;
+    constexpr int kBlock = kStep * W;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Item it;
     __shared__ uint32_t scan[32];
-    __shared__ uint64_t bars[kFewWarps * G::kStages];
-    __shared__ float s_max[kFewWarps][kFewRows], s_sum[kFewWarps][kFewRows];
+    __shared__ uint64_t bars[W * G::kStages];
+    __shared__ float s_max[W][kFewRows], s_sum[W][kFewRows];
     __shared__ int s_abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, col = lane & 3;
     uint32_t idx = blockIdx.x;
@@ -70,7 +70,7 @@ k_attn_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUt
     idx /= a.nsplit;
     const int kvh = idx % a.kv_heads;
     if (threadIdx.x == 0) s_abort = 0;
-    if (threadIdx.x < kFewWarps * G::kStages) {
+    if (threadIdx.x < W * G::kStages) {
         mbar_init(smem_u32(bars + threadIdx.x), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -232,17 +232,17 @@ k_attn_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUt
     __syncthreads();
     if (s_abort) return;
     const uint8_t* rings = smem_align1024(smem_raw);
-    for (int w = threadIdx.x; w < rows * (D / 8); w += kFewThreads) {
+    for (int w = threadIdx.x; w < rows * (D / 8); w += 32 * W) {
         const int r = w / (D / 8), d = w % (D / 8) * 8;
         const int seen = a.causal ? max(0, min(nk, t0 + r / g + nk - nq + 1)) : nk;
         const bool none = min(seen, stop) <= first;     // a row without a key here
         float mx = s_max[0][r];
 #pragma unroll
-        for (int e = 1; e < kFewWarps; ++e) mx = fmaxf(mx, s_max[e][r]);
+        for (int e = 1; e < W; ++e) mx = fmaxf(mx, s_max[e][r]);
         const float ref = mx == -INFINITY ? 0.f : mx;
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < kFewWarps; ++e) {
+        for (int e = 0; e < W; ++e) {
             const float f = ex2(s_max[e][r] - ref);
             const float* from = reinterpret_cast<const float*>(rings + e * G::kRing) + r * D + d;
             sum = fmaf(f, s_sum[e][r], sum);
@@ -270,32 +270,43 @@ int64_t few_items(int64_t nq, int nset, int kv_heads, int group) {
     return ((nq + unit - 1) / unit + nset) * kv_heads;
 }
 
-template <class T, class O, int D>
+// CTAs of a call that cuts no keys, without the empty ones.
+int64_t few_ctas(int64_t nq, int nset, int kv_heads, int group) {
+    const int unit = kFewRows / group;
+    return std::max<int64_t>((nq + unit - 1) / unit, std::min<int64_t>(nset, nq)) * kv_heads;
+}
+
+template <class T, class O, int D, int W>
 tb_status launch(tb_ctx* ctx, const CUtensorMap& km, const CUtensorMap& vm, const AttnArgs& a, unsigned grid) {
-    constexpr size_t sm = FewGeom<D>::kSmem;
-    TB_CUDA_TRY(ctx, cudaFuncSetAttribute(k_attn_few<T, O, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
-    k_attn_few<T, O, D><<<grid, kFewThreads, sm, ctx->stream>>>(km, vm, a);
+    constexpr size_t sm = (size_t)W * FewGeom<D>::kRing + 1024;
+    TB_CUDA_TRY(ctx, cudaFuncSetAttribute(k_attn_few<T, O, D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
+    k_attn_few<T, O, D, W><<<grid, 32 * W, sm, ctx->stream>>>(km, vm, a);
     TB_LAUNCH_CHECK(ctx, "k_attn_few");
     return TB_OK;
 }
 template <class T, class O>
 tb_status launch_dim(tb_ctx* ctx, const CUtensorMap& km, const CUtensorMap& vm, const AttnArgs& a, unsigned grid) {
-    return a.dim <= 64 ? launch<T, O, 64>(ctx, km, vm, a, grid) : launch<T, O, 128>(ctx, km, vm, a, grid);
+    // one CTA an SM of eight warps, two of four where there are more (8 x 4 tokens, 16 heads of 128, 4096
+    // keys, 128 CTAs: 47 us with eight warps, 50 with four and the keys cut in two)
+    if (few_ctas(a.nq, a.nset, a.kv_heads, a.group) <= ctx->num_sms)
+        return a.dim <= 64 ? launch<T, O, 64, 8>(ctx, km, vm, a, grid) : launch<T, O, 128, 8>(ctx, km, vm, a, grid);
+    return a.dim <= 64 ? launch<T, O, 64, 4>(ctx, km, vm, a, grid) : launch<T, O, 128, 4>(ctx, km, vm, a, grid);
 }
 
 }  // namespace
 
-// Sets of 16 rows at most, on average. (16 tokens of 32/8 heads of 64 against 1 to 8192 keys: 44 us here, 61
+// Sets of 16 rows at most, on average. (16 tokens of 32/8 heads of 64 against 1 to 8192 keys: 40 us here, 61
 // in 128-row tiles; 16 x 12 heads of 64 against 300 keys: 8 and 15; 8 x 16 rows of 128 against 4096
-// keys: 55 both.)
+// keys: 48 and 55.)
 bool tb_attn_few(int64_t nq, int nset, int group) { return group <= kFewRows && (nq + nset - 1) / nset * group <= kFewRows; }
 
-// One wave of CTAs, two an SM, and 256 keys at least: a CTA costs some 8 us besides its keys. (One token,
-// 32/8 heads of 128, 8192 keys: 84 us whole, 17 cut in 32; 4 such tokens: 85 whole, 30 in 9, 45 in 32.)
+// Keys are cut only where one CTA an SM leaves SMs idle, into 512 keys at least: a CTA costs some 8 us
+// besides its keys and eight warps keep enough loads under way for the SM. (One token, 32/8 heads of
+// 128, 8192 keys: 84 us whole, 15 cut in 16; 4 such tokens: 30 us, with twice the ranges 33; 16 x
+// 1..8192: 54 whole, 56 in two.)
 int tb_attn_few_nsplit(const tb_ctx* ctx, int64_t nq, int64_t nk, int nset, int kv_heads, int group) {
-    const int unit = kFewRows / group;
-    const int64_t ctas = std::max<int64_t>((nq + unit - 1) / unit, std::min<int64_t>(nset, nq)) * kv_heads;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({2ll * ctx->num_sms / ctas, nk / nset / 256, 32}));
+    const int64_t ctas = few_ctas(nq, nset, kv_heads, group);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({ctx->num_sms / ctas, nk / nset / 512, 32}));
 }
 
 tb_status tb_attn_few_launch(tb_ctx* ctx, const AttnArgs& args, tb_dtype dtype, tb_dtype out_dtype) {
