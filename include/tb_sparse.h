@@ -253,8 +253,8 @@ tb_status tb_layer_norm(tb_ctx* ctx, const void* x, tb_dtype x_dtype, int64_t n,
  *     numbers of elements apart, multiples of 16 bytes, values of a head contiguous. head_dim a
  *     multiple of 8 up to 128, at most 64 heads a key head, scale > 0.
  *   - q_offsets and k_offsets are given together; their set s belong to each other.
- *   - dtype TB_BF16 / TB_F16: tcgen05 tensor cores, fp32 scores, softmax and accumulation; the
- *     p_j are rounded to the operand type before their product with v. TB_F32: CUDA cores.
+ *   - dtype TB_BF16 / TB_F16: tensor cores (tcgen05; warp-level products for sets of a few rows),
+ *     fp32 scores, softmax and accumulation; the p_j are rounded to the operand type before their product with v. TB_F32: CUDA cores.
  *   - out_dtype: TB_F32 or the operand dtype. out must not overlap q, k or v.
  *   - Values behind a set's last key have no effect, not a number included. A key that causal
  *     hides from some rows of its set must be finite: the rows' products multiply it by 0.
