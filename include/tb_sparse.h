@@ -269,12 +269,12 @@ tb_status tb_layer_norm(tb_ctx* ctx, const void* x, tb_dtype x_dtype, int64_t n,
  *     TB_ROPE_FREQS_JOINT f_p = theta^(-p/(head_dim/2)).
  *   - inverse != 0 turns by the negative angles (the transpose: carries gradients back).
  *   - x, out [n][heads][head_dim] of dtype, strides as in tb_attention; out may be x with the same
- *     strides. The first heads of wider rows (q and k of one q|k|v product) are one call. head_dim a
+ *     strides, and overlaps it in no other way. The first heads of wider rows (q and k of one q|k|v product) are one call. head_dim a
  *     multiple of 8 up to 256. Angles are reduced in 64 bits.
  *
  * tb_group_norm: out = act((x - mean) / sqrt(var + eps) * w + b), mean and variance of each set over
  * its rows and each group's c / groups consecutive channels. x [n][c] of x_dtype, out [n][c] of
- * out_dtype (TB_F32 or x_dtype; may be x); c a multiple of 8 up to 2048; w, b float32 [c], each may be
+ * out_dtype (TB_F32 or x_dtype; may be x, else apart from it); c a multiple of 8 up to 2048; w, b float32 [c], each may be
  * NULL. Statistics in fp32, of pieces joined in a fixed order: results repeat to the bit. */
 typedef enum tb_rope_layout { TB_ROPE_PAIRS = 0, TB_ROPE_HALVES = 1 } tb_rope_layout;
 typedef enum tb_rope_freqs { TB_ROPE_FREQS_AXIS = 0, TB_ROPE_FREQS_JOINT = 1 } tb_rope_freqs;

@@ -22,11 +22,13 @@ static void want(const char* what, tb_status got, tb_status exp) {
     if (got != exp) { std::printf("%s: got %d, want %d (%s)\n", what, (int)got, (int)exp, ctx.last_error.c_str()); failed = 1; }
 }
 alignas(16) static char mem[256];
+// addresses that nothing reads: the arrays are 1 MB apart
+static char* at(int i, int more = 0) { return reinterpret_cast<char*>((intptr_t)(i + 1) << 20) + more; }
 
 static tb_attention_params attn() {
     tb_attention_params p;
     std::memset(&p, 0, sizeof p);
-    p.q = mem; p.k = mem + 16; p.v = mem + 32; p.out = mem + 48;
+    p.q = at(0); p.k = at(1); p.v = at(2); p.out = at(3);
     p.q_offsets = p.k_offsets = (const int32_t*)mem;
     p.nq = 10; p.nk = 20; p.nset = 2; p.heads = 4; p.kv_heads = 2; p.head_dim = 64;
     p.q_row = p.out_row = 256; p.k_row = p.v_row = 128; p.q_head = p.k_head = p.v_head = p.out_head = 64;
@@ -36,7 +38,7 @@ static tb_attention_params attn() {
 static tb_rope_params rope() {
     tb_rope_params p;
     std::memset(&p, 0, sizeof p);
-    p.x = mem; p.out = mem + 16; p.coords = (const int32_t*)mem; p.n = 10;
+    p.x = at(0); p.out = at(1); p.coords = (const int32_t*)mem; p.n = 10;
     p.x_row = p.out_row = 256; p.x_head = p.out_head = 64; p.coord_stride = 4; p.axes = 3;
     p.sections[0] = p.sections[1] = p.sections[2] = 10;
     p.heads = 4; p.head_dim = 64; p.theta = 1e4; p.dtype = TB_BF16;
@@ -80,6 +82,10 @@ int main() {
     ATTN(p.out = nullptr, TB_ERR_INVALID_ARG);
     ATTN(p.k = mem + 8, TB_ERR_INVALID_ARG);
     ATTN(p.out = (void*)p.q, TB_ERR_INVALID_ARG);
+    ATTN(p.out = at(0, 512 * 9), TB_ERR_INVALID_ARG);                       // q's last row
+    ATTN(p.out = at(0, -512 * 9 - 496), TB_ERR_INVALID_ARG);                // out's last row ends in q's first
+    ATTN((p.k_row = p.v_row = 256, p.out = at(2, 512 + 240)), TB_ERR_INVALID_ARG);   // into v's head 1
+    ATTN(p.scale = 3e38f, TB_ERR_INVALID_ARG);
 
     want("null context", tb_rope(nullptr, nullptr), TB_ERR_INVALID_ARG);
     want("null parameters", tb_rope(&ctx, nullptr), TB_ERR_INVALID_ARG);
@@ -105,6 +111,13 @@ int main() {
     ROPE(p.out_row = 192, TB_ERR_INVALID_ARG);
     ROPE((p.out = (void*)p.x, p.out_row = 512), TB_ERR_INVALID_ARG);
     ROPE(p.n = (int64_t)1 << 31, TB_ERR_TOO_LARGE);
+    ROPE(p.out = at(0, 512), TB_ERR_INVALID_ARG);                           // one row on
+    ROPE((p.n = 1, p.out = at(0, 16)), TB_ERR_INVALID_ARG);
+    want("rows side by side", tb_rows_overlap({at(0), 10, 512, 256}, {at(0, 256), 10, 512, 256}) ? TB_ERR_INVALID_ARG : TB_OK, TB_OK);
+    want("rows behind", tb_rows_overlap({at(0), 10, 512, 512}, {at(0, 5120), 10, 512, 512}) ? TB_ERR_INVALID_ARG : TB_OK, TB_OK);
+    want("rows before", tb_rows_overlap({at(0, 5120), 10, 512, 512}, {at(0), 10, 512, 512}) ? TB_ERR_INVALID_ARG : TB_OK, TB_OK);
+    want("columns meet", tb_rows_overlap({at(0), 10, 512, 272}, {at(0, 256), 10, 512, 256}) ? TB_OK : TB_ERR_INVALID_ARG, TB_OK);
+    want("row past the edge", tb_rows_overlap({at(0, 512), 1, 0, 256}, {at(0, 272), 2, 512, 256}) ? TB_OK : TB_ERR_INVALID_ARG, TB_OK);
 
     const size_t need = tb_group_norm_workspace_bytes(&ctx, 10000, 32, 4, 1);
     auto gn = [&](const void* x, tb_dtype dt, const int32_t* off, int nset, int64_t n, int c, int groups, float eps, int act,
@@ -112,7 +125,7 @@ int main() {
         return tb_group_norm(&ctx, x, dt, off, nset, n, c, groups, nullptr, nullptr, eps, (tb_epilogue)act, od, out, ws, wb);
     };
     const int32_t* off = (const int32_t*)mem;
-    void* out = mem + 64;
+    void* out = at(5);
     want("gn no rows", gn(mem, TB_F32, off, 1, 0, 32, 4, 1e-5f, 0, TB_F32, out, nullptr, 0), TB_OK);
     want("gn no sets", gn(mem, TB_F32, off, 0, 100, 32, 4, 1e-5f, 0, TB_F32, out, nullptr, 0), TB_OK);
     want("gn dtype", gn(mem, (tb_dtype)5, off, 1, 100, 32, 4, 1e-5f, 0, TB_F32, out, mem, need), TB_ERR_INVALID_ARG);
@@ -129,6 +142,7 @@ int main() {
     want("gn null", gn(nullptr, TB_F32, off, 1, 100, 32, 4, 1e-5f, 0, TB_F32, out, mem, need), TB_ERR_INVALID_ARG);
     want("gn alignment", gn(mem + 4, TB_F32, off, 1, 100, 32, 4, 1e-5f, 0, TB_F32, out, mem, need), TB_ERR_INVALID_ARG);
     want("gn in place", gn(mem, TB_F16, off, 1, 100, 32, 4, 1e-5f, 0, TB_F32, mem, mem, need), TB_ERR_INVALID_ARG);
+    want("gn overlap", gn(at(5, 64), TB_F32, off, 1, 100, 32, 4, 1e-5f, 0, TB_F32, out, mem, need), TB_ERR_INVALID_ARG);
     want("gn workspace", gn(mem, TB_F32, off, 1, 10000, 32, 4, 1e-5f, 0, TB_F32, out, nullptr, 0), TB_ERR_INVALID_ARG);
     want("gn small workspace", gn(mem, TB_F32, off, 1, 10000, 32, 4, 1e-5f, 0, TB_F32, out, mem, need - 1), TB_ERR_INVALID_ARG);
     std::printf(failed ? "failed\n" : "refusals ok\n");

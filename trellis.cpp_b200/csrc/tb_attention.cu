@@ -288,7 +288,8 @@ tb_status attn_args(tb_ctx* ctx, const tb_attention_params* p, AttnArgs& a) {
         return tb_fail(ctx, TB_ERR_UNSUPPORTED, "tb_attention: at most 64 heads may share a key head");
     if (p->nset < 0 || (!p->q_offsets != !p->k_offsets) || (!p->q_offsets && p->nset != 1))
         return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_attention: give both offset tables, or neither with nset 1");
-    if (!(p->scale > 0.f) || !std::isfinite(p->scale))
+    // scores are taken in powers of two
+    if (!(p->scale > 0.f) || !std::isfinite(p->scale * 1.44269504088896340736f))
         return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_attention: scale must be positive and finite");
     // a tile past the last row still has a 32-bit row number
     if (p->nq > (int64_t)INT32_MAX - 1024 || p->nk > (int64_t)INT32_MAX - 1024 || p->nset > 65536 || p->heads > 65536)
@@ -305,8 +306,12 @@ tb_status attn_args(tb_ctx* ctx, const tb_attention_params* p, AttnArgs& a) {
     if (p->nk > 0 && (!p->k || !p->v)) return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_attention: null pointer");
     if (!tb_aligned16(p->q) || !tb_aligned16(p->k) || !tb_aligned16(p->v) || !tb_aligned16(p->out))
         return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_attention: q / k / v / out must be 16-byte aligned");
-    if (p->nq > 0 && (p->out == p->q || p->out == p->k || p->out == p->v))
-        return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_attention: out must not alias q, k or v");
+    const tb_rows o = tb_head_rows(p->out, p->nq, p->out_row, p->heads, p->out_head, p->head_dim, p->out_dtype);
+    if (p->nq > 0 && (p->out == p->q || p->out == p->k || p->out == p->v ||
+                      tb_rows_overlap(o, tb_head_rows(p->q, p->nq, p->q_row, p->heads, p->q_head, p->head_dim, p->dtype)) ||
+                      tb_rows_overlap(o, tb_head_rows(p->k, p->nk, p->k_row, p->kv_heads, p->k_head, p->head_dim, p->dtype)) ||
+                      tb_rows_overlap(o, tb_head_rows(p->v, p->nk, p->v_row, p->kv_heads, p->v_head, p->head_dim, p->dtype))))
+        return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_attention: out must not overlap q, k or v");
     a.q = p->q;
     a.k = p->k;
     a.v = p->v;

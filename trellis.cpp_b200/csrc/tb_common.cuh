@@ -96,6 +96,27 @@ inline bool tb_rows_disjoint(int64_t n, int64_t row, int64_t heads, int64_t head
     if (n <= 1 || heads <= 1) return (n <= 1 || row >= dim) && (heads <= 1 || head >= dim);
     return (head >= dim && row >= (heads - 1) * head + dim) || (row >= dim && head >= (n - 1) * row + dim);
 }
+// Rows of `len` bytes side by side, `row` bytes apart from `base` on (row: of no use with one row).
+struct tb_rows {
+    const void* base;
+    int64_t n, row, len;
+};
+// The rows of a [n][heads][dim] array, its strides in elements; n 0 where a head's values do not follow the
+// last one's, which tb_rows_overlap does not judge.
+inline tb_rows tb_head_rows(const void* base, int64_t n, int64_t row, int64_t heads, int64_t head, int64_t dim, tb_dtype t) {
+    const int64_t size = (int64_t)tb_dtype_size(t);
+    return {base, heads > 1 && head != dim ? 0 : n, row * size, heads * dim * size};
+}
+// Whether two arrays are sure to share a byte: rows equally far apart (or one row) whose columns meet.
+inline bool tb_rows_overlap(const tb_rows& a, const tb_rows& b) {
+    if (a.n <= 0 || b.n <= 0) return false;
+    const int64_t row = a.n > 1 ? a.row : b.n > 1 ? b.row : INT64_MAX / 4;
+    if ((b.n > 1 && b.row != row) || a.len > row || b.len > row) return false;
+    const int64_t at = (int64_t)reinterpret_cast<intptr_t>(b.base) - (int64_t)reinterpret_cast<intptr_t>(a.base);
+    if (at >= (a.n - 1) * row + a.len || -at >= (b.n - 1) * row + b.len) return false;
+    const int64_t d = (at % row + row) % row;
+    return d < a.len || d + b.len > row;
+}
 
 inline bool tb_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

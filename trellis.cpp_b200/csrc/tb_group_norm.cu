@@ -483,6 +483,9 @@ extern "C" tb_status tb_group_norm(tb_ctx* ctx, const void* x, tb_dtype x_dtype,
         return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_group_norm: x / out must be 16-byte aligned");
     if (out == x && out_dtype != x_dtype)
         return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_group_norm: in place needs out_dtype equal to x's dtype");
+    if (out != x && tb_rows_overlap({out, 1, 0, n * c * (int64_t)tb_dtype_size(out_dtype)},
+                                    {x, 1, 0, n * c * (int64_t)tb_dtype_size(x_dtype)}))
+        return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_group_norm: out must be x or not overlap it");
     const size_t need = tb_group_norm_workspace_bytes(ctx, n, c, groups, nset);
     if (need && (!workspace || workspace_bytes < need || !tb_aligned16(workspace)))
         return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_group_norm: workspace too small or not 16-byte aligned");

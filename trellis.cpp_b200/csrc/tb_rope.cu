@@ -192,6 +192,9 @@ extern "C" tb_status tb_rope(tb_ctx* ctx, const tb_rope_params* p) {
         return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: rows or heads of out overlap");
     if (p->out == p->x && ((rows && p->out_row != p->x_row) || (hds && p->out_head != p->x_head)))
         return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: in place needs equal strides");
+    if (p->out != p->x && tb_rows_overlap(tb_head_rows(p->out, p->n, p->out_row, p->heads, p->out_head, p->head_dim, p->dtype),
+                                          tb_head_rows(p->x, p->n, p->x_row, p->heads, p->x_head, p->head_dim, p->dtype)))
+        return tb_fail(ctx, TB_ERR_INVALID_ARG, "tb_rope: out must be x or not overlap it");
 
     RopeArgs r;
     r.x = p->x;
