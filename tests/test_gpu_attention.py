@@ -134,6 +134,32 @@ def test_few_rows_strides_and_float32_output(tb, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,start", [(33, 0), (1025, 700), (3001, 40)])
+def test_thousands_of_small_sets(tb, n, start, dtype):
+    from trellis_cpp_b200 import ops
+    g = torch.Generator().manual_seed(n)
+    ql = (torch.randint(0, 4, (n,), generator=g) * (torch.rand(n, generator=g) < 0.6)).tolist()
+    kl = torch.randint(0, 5, (n,), generator=g).tolist()
+    ql[n // 2] = 37
+    q, k, v = _inputs(24, sum(ql) + start, sum(kl), 4, 1, 64, dtype)
+    _check(ops, q, k, v, ref.offsets(ql, start), ref.offsets(kl), True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("qo,ko", [([0, 3, 2, 6], [0, 50, 90, 128]), ([-1, 2, 4, 6], [0, 50, 90, 128]),
+                                   ([0, 2, 4, 6], [0, 90, 50, 128]), ([0, 2, 4, 6], [0, 50, 90, 129]),
+                                   ([0, 0, 0, 6], [0, 50, 40, 128])])
+def test_few_rows_bad_tables_are_reported(tb, qo, ko, dtype):
+    from trellis_cpp_b200 import ops
+    q, k, v = _inputs(25, 6, 128, 2, 2, 64, dtype)
+    ops.attention(q, k, v, ref.table(qo), ref.table(ko))
+    with pytest.raises(ops.TBError) as e:
+        ops.check_device()
+    assert e.value.status == 5 and "offset table" in str(e.value)
+    _check(ops, q, k, v, [0, 2, 6], [0, 50, 128])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("scale,spread", [(1e-4, 1.0), (0.125, 20.0), (2.0, 3.0)])
 def test_few_rows_flat_steep_and_rising_scores(tb, scale, spread, dtype):
     from trellis_cpp_b200 import ops

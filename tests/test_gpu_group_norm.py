@@ -165,6 +165,32 @@ def test_more_than_2_31_elements(tb):
     assert int(y[:-1000].count_nonzero()) == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_thousands_of_small_sets_in_three_passes(tb, dtype):
+    from trellis_cpp_b200 import ops
+    g = torch.Generator().manual_seed(3)
+    lengths = torch.randint(0, 9, (2000,), generator=g).tolist()
+    lengths[700], lengths[1999] = 1300, 0
+    off = ref.offsets(lengths, 100)
+    x, w, b = _inputs(12, off[-1] + 50, 64, dtype)
+    x[:100] = float("nan")
+    x[off[-1]:] = float("nan")
+    y = torch.full_like(x, 3.0)
+    _check(ops, x, 8, w, b, off, eps=1e-3, act="silu", out=y)
+    assert bool((y[:100] == 3).all()) and bool((y[off[-1]:] == 3).all())
+
+
+@pytest.mark.parametrize("off", [[0, 6000, 3000, 10000], [-3, 5000, 10000, 10000], [0, 50, 100, 17000]])
+def test_bad_tables_of_long_arrays_are_reported(tb, off):
+    from trellis_cpp_b200 import ops
+    x, w, b = _inputs(13, 10000, 32, torch.bfloat16)
+    ops.group_norm(x, 4, w, b, ref.table(off))
+    with pytest.raises(ops.TBError) as e:
+        ops.check_device()
+    assert e.value.status == 5 and "offset table" in str(e.value)
+    _check(ops, x, 4, w, b, [0, 5000, 10000])
+
+
 @pytest.mark.parametrize("off", [[0, 60, 30, 100], [-3, 50, 100, 100], [0, 50, 100, 170]])
 def test_bad_tables_are_reported(tb, off):
     from trellis_cpp_b200 import ops

@@ -71,13 +71,13 @@ __global__ void __launch_bounds__(kCcThreads, 2) k_attn_cc(const __grid_constant
     float* sk = sq + kCcRows * LD;                  // [64][LD], then the weights [64][68]
     float* sv = sk + kCcKeys * LD;                  // [D][68]: values of a column side by side
     float* sp = sk;
-    __shared__ Item it;
-    __shared__ uint32_t scan[32];
     uint32_t idx = blockIdx.x;
     const int split = idx % a.nsplit;
     idx /= a.nsplit;
     const int kvh = idx % a.kv_heads;
-    find_item(a.q_off, a.nset, a.nq, a.unit, idx / a.kv_heads, a.err, &it, scan);
+    check_table(a.q_off, a.nset, a.nq, a.err);
+    check_table(a.k_off, a.nset, a.nk, a.err);
+    const Item it = find_item(a.q_off, a.nset, a.nq, a.unit, idx / a.kv_heads, a.err);
     if (it.set < 0) return;
     // causal: the last rows of a set see the most keys; they go first
     const int piece = a.causal ? (int)(it.items - 1 - it.item) : (int)it.item;

@@ -59,8 +59,6 @@ k_attn_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUt
     using G = FewGeom<D>;
     constexpr int kBlock = kStep * W;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ Item it;
-    __shared__ uint32_t scan[32];
     __shared__ uint64_t bars[W * G::kStages];
     __shared__ float s_max[W][kFewRows], s_sum[W][kFewRows];
     __shared__ int s_abort;
@@ -74,8 +72,11 @@ k_attn_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUt
         mbar_init(smem_u32(bars + threadIdx.x), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    find_item(a.q_off, a.nset, a.nq, a.unit, idx / a.kv_heads, a.err, &it, scan);      // the block meets in it
+    check_table(a.q_off, a.nset, a.nq, a.err);
+    check_table(a.k_off, a.nset, a.nk, a.err);
+    const Item it = find_item(a.q_off, a.nset, a.nq, a.unit, idx / a.kv_heads, a.err);
     if (it.set < 0) return;
+    __syncthreads();                                    // the barriers
     int64_t k0, k1;
     set_range(a.k_off, it.set, a.nk, k0, k1, a.err);
     const int nq = (int)(it.hi - it.lo), nk = (int)(k1 - k0), g = a.group;

@@ -284,10 +284,9 @@ __device__ __forceinline__ void gn_write(const GnArgs& a, const f2* mean, const 
 
 template <class T>
 __global__ void __launch_bounds__(kGnThreads, 2) k_gn_stats(const __grid_constant__ GnArgs a) {
-    __shared__ Item it;
-    __shared__ uint32_t scan[32];
     extern __shared__ float4 ent[];
-    find_item(a.off, a.nset, a.n, a.unit, blockIdx.x, a.err, &it, scan);
+    check_table(a.off, a.nset, a.n, a.err);
+    const Item it = find_item(a.off, a.nset, a.n, a.unit, blockIdx.x, a.err);
     if (it.set < 0) return;
     const int tc = a.c / 8, lanes = kGnThreads / tc;
     const int ry = threadIdx.x / tc, tx = threadIdx.x % tc;
@@ -303,23 +302,11 @@ __global__ void __launch_bounds__(kGnThreads, 2) k_gn_stats(const __grid_constan
 
 // One block joins the pieces of a set's groups, one group after another.
 __global__ void __launch_bounds__(128) k_gn_merge(const __grid_constant__ GnArgs a) {
-    __shared__ uint32_t first_s;
     __shared__ float acc[2][4];
     const int set = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int64_t lo, hi;
     set_range(a.off, set, a.n, lo, hi, a.err);
     if (hi == lo) return;
-    // the set's first piece: the pieces of the sets before it
-    uint32_t before = 0;
-    for (int s = threadIdx.x; s < set; s += 128) {
-        int64_t l, h;
-        set_range(a.off, s, a.n, l, h, a.err);
-        before += (uint32_t)((h - l + a.unit - 1) / a.unit);
-    }
-    if (threadIdx.x == 0) first_s = 0;
-    __syncthreads();
-    if (before) atomicAdd(&first_s, before);
-    __syncthreads();
     const int pieces = (int)((hi - lo + a.unit - 1) / a.unit);
     const float cg = (float)(a.c / a.groups), each = (float)a.unit * cg;
     const float last = (float)(hi - lo - (int64_t)(pieces - 1) * a.unit) * cg, share = 1.f / ((float)(hi - lo) * cg);
@@ -339,7 +326,7 @@ __global__ void __launch_bounds__(128) k_gn_merge(const __grid_constant__ GnArgs
         __syncthreads();
     };
     for (int g = blockIdx.y; g < a.groups; g += gridDim.y) {
-        const float2* p = a.part + (int64_t)first_s * a.groups + g;
+        const float2* p = a.part + (int64_t)first_item(a.off, set, a.n, a.unit) * a.groups + g;
         float m = 0.f, d = 0.f, q = 0.f;
 #pragma unroll 4
         for (int i = threadIdx.x; i < pieces; i += 128) m = fmaf(i == pieces - 1 ? last : each, p[(int64_t)i * a.groups].x, m);
@@ -371,9 +358,7 @@ __device__ __forceinline__ void gn_factors(const GnArgs& a, const float2* stat, 
 
 template <class T, class O>
 __global__ void __launch_bounds__(kGnThreads, sizeof(T) == 4 ? 3 : 4) k_gn_apply(const __grid_constant__ GnArgs a) {
-    __shared__ Item it;
-    __shared__ uint32_t scan[32];
-    find_item(a.off, a.nset, a.n, a.unit_out, gridDim.x - 1 - blockIdx.x, a.err, &it, scan);
+    const Item it = find_item(a.off, a.nset, a.n, a.unit_out, gridDim.x - 1 - blockIdx.x, a.err);
     if (it.set < 0) return;
     const int tc = a.c / 8, lanes = kGnThreads / tc;
     const int ry = threadIdx.x / tc, ch = (threadIdx.x % tc) * 8;

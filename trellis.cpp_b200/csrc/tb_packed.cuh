@@ -25,56 +25,46 @@ __device__ __forceinline__ void set_range(const int32_t* off, int s, int64_t n, 
     hi = b < lo ? lo : (b > n ? n : b);
 }
 
+// Reports every bad offset of a table once, the blocks of the launch together.
+__device__ __forceinline__ void check_table(const int32_t* off, int nset, int64_t n, int* err) {
+    int64_t lo, hi;
+    if (off)
+        for (int64_t s = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; s < nset; s += (int64_t)gridDim.x * blockDim.x)
+            set_range(off, (int)s, n, lo, hi, err);
+}
+
+// The sets cut into pieces of `unit` rows, in order. Set s has the numbers from first_item(s) =
+// offsets[s] / unit + s on, at least as many as it has pieces (a few stay without one), so a set's
+// numbers need one entry of the table and the set of a number is found by search. Numbers are below
+// n / unit + nset, 32 bits.
+__device__ __forceinline__ uint32_t first_item(const int32_t* off, int s, int64_t n, int unit) {
+    const int64_t o = off ? off[s] : 0;
+    return (uint32_t)(o < 0 ? 0 : o > n ? n : o) / (uint32_t)unit + (uint32_t)s;
+}
 struct Item {
-    int set;        // -1: the index is past the last item
+    int set;        // -1: the number is without a piece
     uint32_t item;  // which piece of the set
     uint32_t items; // pieces of the set
     int64_t lo, hi; // the set's rows
 };
-
-// Piece `idx` of the list that cuts every set, in order, into pieces of `unit` rows. All threads of
-// the block call it (at most 1024); each sums the pieces of its share of the sets, a scan over the
-// threads finds the owner of `idx`, which walks its share. One table read per thread up to
-// blockDim.x sets. `res` and `warp_sum` (32 words) are shared memory.
-__device__ __forceinline__ void find_item(const int32_t* off, int nset, int64_t n, int unit, uint32_t idx, int* err,
-                                          Item* res, uint32_t* warp_sum) {
-    const int t = threadIdx.x, nt = blockDim.x, lane = t & 31, warp = t >> 5;
-    const int per = (nset + nt - 1) / nt;
-    const int s0 = min(nset, t * per), s1 = min(nset, s0 + per);
-    uint32_t sum = 0;
-    int64_t lo = 0, hi = 0;
-    for (int s = s0; s < s1; ++s) {
-        set_range(off, s, n, lo, hi, err);
-        sum += (uint32_t)((hi - lo + unit - 1) / unit);
+// Piece number `idx`, by whole warps: a step looks at 32 places, three steps find one of 32768 sets.
+__device__ __forceinline__ Item find_item(const int32_t* off, int nset, int64_t n, int unit, uint32_t idx, int* err) {
+    const int lane = threadIdx.x & 31;
+    int s = 0;
+    for (int span = nset; span > 1;) {
+        const int step = (span + 31) / 32, at = lane * step;
+        const uint32_t below = __ballot_sync(0xffffffffu, at < span && first_item(off, s + min(at, span - 1), n, unit) <= idx);
+        const int k = below ? 31 - __clz(below) : 0;
+        s += k * step;
+        span = min(step, span - k * step);
     }
-    uint32_t inc = sum;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, d);
-        if (lane >= d) inc += v;
-    }
-    if (lane == 31) warp_sum[warp] = inc;
-    if (t == 0) res->set = -1;
-    __syncthreads();
-    uint32_t base = 0;
-    for (int w = 0; w < warp; ++w) base += warp_sum[w];
-    uint32_t first = base + inc - sum;
-    if (idx >= first && idx - first < sum) {
-        for (int s = s0; s < s1; ++s) {
-            if (s1 - s0 > 1) set_range(off, s, n, lo, hi, err);
-            const uint32_t c = (uint32_t)((hi - lo + unit - 1) / unit);
-            if (idx - first < c) {
-                res->set = s;
-                res->item = idx - first;
-                res->items = c;
-                res->lo = lo;
-                res->hi = hi;
-                break;
-            }
-            first += c;
-        }
-    }
-    __syncthreads();
+    Item it;
+    set_range(off, s, n, it.lo, it.hi, err);
+    const uint32_t first = first_item(off, s, n, unit);
+    it.items = (uint32_t)((it.hi - it.lo + unit - 1) / unit);
+    it.item = idx - first;
+    it.set = idx >= first && it.item < it.items ? s : -1;
+    return it;
 }
 
 // ---- two 32-bit values in one instruction ----------------------------------------------------------
