@@ -533,6 +533,7 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
         // The warpgroups take turns over the blocks of all tiles.
         const int wg = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
         const uint32_t lane_base = (uint32_t)(quad * 32) << 16, to = tmem_o + lane_base;
+        const int rt = r / a.group;           // the row's token in a tile
         const float c = a.scale_log2;
         // p in f16 starts at 2^7 instead of 1 (2^15 after the largest rise): small p keep their digits
         constexpr float lift = std::is_same<T, __half>::value ? 7.f : 0.f;
@@ -543,9 +544,9 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
             const int n = job->n;
             // the keys from the tile's first block on that the row sees; rows past the set see all
             auto rows = [&](int& t, int& h) {
-                t = job->first + (int)rank * p.tile_tokens + r / a.group;
-                h = job->kvh * a.group + r % a.group;
-                return r < p.tile_tokens * a.group && t < job->nq;
+                t = job->first + (int)rank * p.tile_tokens + rt;
+                h = job->kvh * a.group + r - rt * a.group;
+                return rt < p.tile_tokens && t < job->nq;
             };
             int lim, wlim;
             {
@@ -576,9 +577,13 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 tmem_wait_ld();
                 const bool masked = wlim < (b + 1) * kKeys;
                 if (masked) {
-                    const int left = lim - b * kKeys;
+                    const int left = lim - b * kKeys, least = wlim - b * kKeys;
 #pragma unroll
-                    for (int q = 0; q < kKeys; ++q) s[q] = q < left ? s[q] : -INFINITY;
+                    for (int e = 0; e < kKeys; e += 32) {
+                        if (least >= e + 32) continue;   // all of it
+#pragma unroll
+                        for (int q = e; q < e + 32; ++q) s[q] = q < left ? s[q] : -INFINITY;
+                    }
                 }
                 float mx[4];
 #pragma unroll
@@ -643,12 +648,12 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
             int t, h;
             const bool valid = rows(t, h), none = n == 0 || lim <= 0;      // none: the row sees no key here
             const float inv = none ? 0.f : 1.f / total;
-            const float lg = none ? -INFINITY : ref - lift + log2f(total);
             const int64_t row = (int64_t)job->q0 + t;
             const int64_t at = ((int64_t)job->split * a.nq + row) * a.heads + h;
-            if (valid && wg == 0) {
+            if (valid && wg == 0 && (a.part || a.lse)) {
+                const float lg = none ? -INFINITY : ref - lift + log2f(total);
                 if (a.part) a.part_lse[at] = lg;
-                else if (a.lse) a.lse[row * a.heads + h] = lg * 0.69314718055994530942f;
+                else a.lse[row * a.heads + h] = lg * 0.69314718055994530942f;
             }
             float* part = a.part + at * a.dim;
             O* out = reinterpret_cast<O*>(a.out) + row * a.out_row + (int64_t)h * a.out_head;
