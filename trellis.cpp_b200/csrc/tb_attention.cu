@@ -204,11 +204,15 @@ int64_t cc_items(int64_t nq, int nset, int kv_heads, int group) {
     const int unit = kCcRows / group;
     return ((nq + unit - 1) / unit + nset) * kv_heads;
 }
-// Fewer blocks than three an SM are cut into ranges of at least two blocks of keys (800 and 600 rows,
-// 8 heads of 64, 192 blocks: 104 us whole, 92 us with the keys cut in two and joined).
+// Fewer CTAs than three an SM are cut, down to a block of keys each for sets of the average length or to two
+// if all keys are one set's, which the host does not know: a block takes a lone CTA 4 to 11 us, a range
+// without keys next to nothing. (800 and 600 rows, 8 heads of 64, 192 CTAs: 104 us whole, 93 cut in two
+// and joined; 870 rows beside four small sets, one head of 128: 150 and 34; 57 and 91 rows, 8 heads of
+// 128: 29 and 22; three sets of 64, one block each: 13 us, 16 if cut all the same.)
 int cc_nsplit(const tb_ctx* ctx, int64_t nq, int64_t nk, int nset, int kv_heads, int group) {
-    const int64_t items = cc_items(nq, nset, kv_heads, group), blocks = (nk / nset + kCcKeys - 1) / kCcKeys;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({3ll * ctx->num_sms / items, blocks / 2, 32}));
+    const int64_t items = cc_items(nq, nset, kv_heads, group);
+    const int64_t blocks = std::max((nk / nset + kCcKeys - 1) / kCcKeys, nk / kCcKeys / 2);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({3ll * ctx->num_sms / items, blocks, 32}));
 }
 
 template <class O, int D>
