@@ -728,8 +728,10 @@ struct Plan {
 // Pairs for wide heads where an average set's rows fill more than one CTA (16384 rows, 12 heads of 128:
 // 1.55 ms, a CTA a tile 1.59; eight causal sets of 1 to 4096 rows, 16/4 heads: 183 us and 202; where rows
 // fill one CTA at most a pair's other half is idle: 62 us and 118 for 16 single rows). Keys are cut
-// where the CTAs would not fill the SMs, into ranges of eight blocks at least (two sets of 40 rows, 16
-// heads, 8192 keys: 34 us, whole 60; 100 rows, 12 heads, 20000 keys: 32 and 129).
+// where the CTAs would not fill the SMs, into ranges of four blocks at least in a set of the average
+// length, of eight if all keys are one set's (100 rows, 12 heads, 20000 keys: 32 us, whole 129; 300 rows, 8
+// heads, 2048 keys: 14 and 16; 100 rows against 8000 keys beside three sets of 3, 4 heads: 20 and 37; two
+// sets of 40 rows, 16 heads, 8192 keys: 38, 34 with ranges twice as long, whole 60).
 Plan attn_plan(int num_sms, int64_t nq, int64_t nk, int nset, int kv_heads, int group, int dim) {
     Plan l;
     l.tile_tokens = 128 / group;
@@ -737,9 +739,9 @@ Plan attn_plan(int num_sms, int64_t nq, int64_t nk, int nset, int kv_heads, int 
     l.unit = l.pair ? 2 * l.tile_tokens : l.tile_tokens;
     const int64_t pieces = (nq + l.unit - 1) / l.unit;
     const int64_t ctas = std::max<int64_t>(pieces, std::min<int64_t>(nset, nq)) * kv_heads * (l.pair ? 2 : 1);
-    const int64_t blocks = (nk / nset + kKeys - 1) / kKeys;          // of an average set
+    const int64_t blocks = std::max((nk / nset + kKeys - 1) / kKeys / 4, nk / kKeys / 8);
     l.nsplit = 1;
-    if (ctas < num_sms) l.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({4ll * num_sms / ctas, blocks / 8, 32}));
+    if (ctas < num_sms) l.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({4ll * num_sms / ctas, blocks, 32}));
     l.items = (pieces + nset) * kv_heads * l.nsplit;
     return l;
 }
