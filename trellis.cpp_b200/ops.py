@@ -32,7 +32,6 @@ from ._lib import TBError, check  # noqa: F401
 _DT = {torch.float32: _lib.TB_F32, torch.float16: _lib.TB_F16, torch.bfloat16: _lib.TB_BF16}
 _EPI = {"none": _lib.TB_EPI_NONE, None: _lib.TB_EPI_NONE, "silu": _lib.TB_EPI_SILU}
 _ctxs: dict = {}
-_streams: dict = {}      # the stream each context is bound to
 
 
 def _raw_stream(index: int) -> int:
@@ -55,8 +54,9 @@ def _ptr(t) -> ctypes.c_void_p:
 
 def context(device=None):
     """The per-device tb_ctx, bound to torch's current stream on that device (the current device
-    when `device` is None or names no index). One context per device is shared by every caller
-    in the process; like the C contexts it wraps, it is not safe to use from two threads at once."""
+    when `device` is None or names no index) by every call, whatever stream it had before. One
+    context per device is shared by every caller in the process; like the C contexts it wraps, it
+    is not safe to use from two threads at once."""
     idx = device
     if type(idx) is not int:
         idx = None if device is None else torch.device(device).index
@@ -64,15 +64,15 @@ def context(device=None):
             idx = torch.cuda.current_device()
     lib = _lib.load()
     h = _ctxs.get(idx)
-    stream = _raw_stream(idx)
     if h is None:
+        # by the Stream object: it brings CUDA up in a process that has made no tensor yet
+        stream = torch.cuda.current_stream(idx).cuda_stream
         h = ctypes.c_void_p()
         check(lib.tb_ctx_create(idx, ctypes.c_void_p(stream), ctypes.byref(h)), "tb_ctx_create")
         _ctxs[idx] = h
-        _streams[idx] = stream
-    elif _streams[idx] != stream:
-        check(lib.tb_ctx_set_stream(h, ctypes.c_void_p(stream)), "tb_ctx_set_stream", h)
-        _streams[idx] = stream
+    else:
+        # every time: a caller may have set another stream on the handle
+        check(lib.tb_ctx_set_stream(h, ctypes.c_void_p(_raw_stream(idx))), "tb_ctx_set_stream", h)
     return h
 
 
