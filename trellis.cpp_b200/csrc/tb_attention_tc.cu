@@ -298,10 +298,8 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
         if (warp == kList) {
             // -------------------------------------------------------------- the list
             // Tiles in the order set, piece of the set (causal: the last ones, which see the most keys, come
-            // first), key head, range of keys. A lane holds one of 32 sets; numbers only grow.
-            int set0 = -32;
-            uint32_t base = 0, total = 0, inc = 0, cnt = 0;
-            int64_t qlo = 0, qhi = 0, klo = 0, khi = 0;
+            // first), key head, range of keys; taken over in whatever order they are given.
+            SetWalk walk;
             uint32_t number = PAIR ? cluster_id_x() : blockIdx.x, jobs = 0;
             for (uint32_t k = 0;; ++k) {
                 const bool over = number == 0xffffffffu;         // none left to take over
@@ -309,33 +307,14 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 const int split = idx % a.nsplit;
                 idx /= a.nsplit;
                 const int kvh = idx % a.kv_heads;
-                const uint32_t piece = idx / a.kv_heads;
-                while (!over && piece >= base + total && set0 + 32 < a.nset) {
-                    base += total;
-                    set0 += 32;
-                    cnt = 0;
-                    if (set0 + lane < a.nset) {
-                        set_range(a.q_off, set0 + lane, a.nq, qlo, qhi, a.err);
-                        set_range(a.k_off, set0 + lane, a.nk, klo, khi, a.err);
-                        cnt = (uint32_t)((qhi - qlo + a.unit - 1) / a.unit);
-                    }
-                    inc = cnt;
-#pragma unroll
-                    for (int d = 1; d < 32; d *= 2) {
-                        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, d);
-                        if (lane >= d) inc += v;
-                    }
-                    total = __shfl_sync(0xffffffffu, inc, 31);
-                }
-                const bool found = !over && piece < base + total;       // the launch has some more than there are
-                const int src = found ? __ffs(__ballot_sync(0xffffffffu, base + inc > piece)) - 1 : 0;
-                const uint32_t cs = __shfl_sync(0xffffffffu, cnt, src), at = piece - base - (__shfl_sync(0xffffffffu, inc, src) - cs);
+                SetWalk::Piece at{};                             // the launch has some more tiles than there are
+                const bool found = !over && walk.find(a.q_off, a.k_off, a.nset, a.nq, a.nk, a.unit, idx / a.kv_heads, lane, a.err, at);
                 Job o;
-                o.q0 = (int)__shfl_sync(0xffffffffu, qlo, src);
-                o.nq = (int)__shfl_sync(0xffffffffu, qhi, src) - o.q0;
-                o.k0 = (int)__shfl_sync(0xffffffffu, klo, src);
-                o.nk = (int)__shfl_sync(0xffffffffu, khi, src) - o.k0;
-                o.first = (int)(a.causal ? cs - 1 - at : at) * a.unit;
+                o.q0 = at.q0;
+                o.nq = at.nq;
+                o.k0 = at.k0;
+                o.nk = at.nk;
+                o.first = (int)(a.causal ? at.of - 1 - at.at : at.at) * a.unit;
                 const int end = a.causal ? max(0, min(o.nk, min(o.first + a.unit, o.nq) + o.nk - o.nq)) : o.nk;
                 const int all = (end + kKeys - 1) / kKeys;
                 o.blk0 = (int)((int64_t)all * split / a.nsplit);

@@ -7,23 +7,9 @@
 #include <cuda_fp16.h>
 
 #include "tb_common.cuh"
+#include "tb_set_walk.cuh"
 
 namespace tbpk {
-
-// Rows [lo, hi) of a set. The table lives in device memory, so it is checked here: an offset that
-// is negative, smaller than the one before it or past the array's n rows is clamped (no kernel
-// reads or writes outside the array) and reported through the context's error word.
-__device__ __forceinline__ void set_range(const int32_t* off, int s, int64_t n, int64_t& lo, int64_t& hi, int* err) {
-    if (!off) {
-        lo = 0;
-        hi = n;
-        return;
-    }
-    const int64_t a = off[s], b = off[s + 1];
-    if (a < 0 || b < a || b > n) atomicCAS(err, 0, TB_DEVERR_BAD_OFFSETS);
-    lo = a < 0 ? 0 : (a > n ? n : a);
-    hi = b < lo ? lo : (b > n ? n : b);
-}
 
 // Reports every bad offset of a table once, the blocks of the launch together.
 __device__ __forceinline__ void check_table(const int32_t* off, int nset, int64_t n, int* err) {
