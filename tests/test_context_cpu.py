@@ -19,7 +19,7 @@ class _Library:
 
     def tb_ctx_set_stream(self, handle, stream):
         assert handle.value == 0x1000
-        self.stream = stream.value
+        self.stream = getattr(stream, "value", stream)
         return 0
 
     def tb_ctx_last_error(self, handle):

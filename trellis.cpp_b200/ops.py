@@ -72,7 +72,9 @@ def context(device=None):
         _ctxs[idx] = h
     else:
         # every time: a caller may have set another stream on the handle
-        check(lib.tb_ctx_set_stream(h, ctypes.c_void_p(_raw_stream(idx))), "tb_ctx_set_stream", h)
+        st = lib.tb_ctx_set_stream(h, _raw_stream(idx))
+        if st:
+            check(st, "tb_ctx_set_stream", h)
     return h
 
 
