@@ -1,7 +1,8 @@
 // Rotary positions with several axes: the pair p of every head of row i turns by the angle
 //   pos[i][axis(p)] * f_p,   (a, b) -> (a cos - b sin, a sin + b cos),
 // where the first sections[0] pairs of a head take axis 0 (a voxel's x), the next sections[1] axis
-// 1, and so on; pairs past the last section keep their values. f_p = theta^(-j / sections[axis])
+// 1, and so on; pairs past the last section keep their bits (no product with a sine of 0, which would
+// carry a value that is no number to its partner). f_p = theta^(-j / sections[axis])
 // with j the pair's place in its section, or theta^(-p / (head_dim/2)) with frequencies shared by
 // the axes. inverse turns by the negative angle, which is the transpose: the gradient's way back.
 //
@@ -27,8 +28,9 @@ struct RopeArgs {
     const int32_t* pos;       // column of axis 0 of row 0
     int64_t n, x_row, x_head, out_row, out_head;
     int pos_stride, heads, half, chunks, heads_per;
+    int turned;               // pairs that turn; those behind are kept
     float sign;               // -1 turns backwards
-    double freq[kRopeMaxPairs];      // revolutions per position; 0: the pair is kept
+    double freq[kRopeMaxPairs];      // revolutions per position
     uint8_t axis[kRopeMaxPairs];
 };
 
@@ -54,35 +56,32 @@ template <class T, int P, bool PAIRS> struct Pairs {
             for (int i = 0; i < kWords; ++i)
                 __stcs(reinterpret_cast<W*>(h + (PAIRS ? 2 * p0 : r * half + p0)) + i, w[r * kWords + i]);
     }
-    // turns the pairs by c, s
-    __device__ __forceinline__ void turn(const float* c, const float* s) {
+    // turns the first `left` pairs by c, s
+    __device__ __forceinline__ void turn(const float* c, const float* s, int left) {
         uint32_t* u = reinterpret_cast<uint32_t*>(w);
         constexpr int per = 4 / (int)sizeof(T);                   // elements of a 32-bit word
 #pragma unroll
         for (int i = 0; i < P; i += (PAIRS ? 1 : per)) {
-            float a[per], b[per];
             if (PAIRS) {
-                get(u, 2 * i, a, b);
-            } else {
-#pragma unroll
-                for (int e = 0; e < per; ++e) {
-                    a[e] = value(u, i + e);
-                    b[e] = value(u, P + i + e);
-                }
-            }
-            if (PAIRS) {
-                put(u, 2 * i, a[0] * c[i] - b[0] * s[i], a[0] * s[i] + b[0] * c[i]);
+                float a, b;
+                get(u, 2 * i, &a, &b);
+                if (i < left) put(u, 2 * i, a * c[i] - b * s[i], a * s[i] + b * c[i]);
             } else {
                 float x[2], y[2];
 #pragma unroll
                 for (int e = 0; e < per; ++e) {
-                    x[e] = a[e] * c[i + e] - b[e] * s[i + e];
-                    y[e] = a[e] * s[i + e] + b[e] * c[i + e];
+                    const float a = value(u, i + e), b = value(u, P + i + e);
+                    x[e] = a * c[i + e] - b * s[i + e];
+                    y[e] = a * s[i + e] + b * c[i + e];
                 }
                 if (per == 2) {
+                    const uint32_t ka = u[i / 2], kb = u[(P + i) / 2];
+                    const uint32_t m = i + 1 < left ? 0xffffffffu : i < left ? 0xffffu : 0u;   // the halves that turn
                     put(u, i, x[0], x[1]);
                     put(u, P + i, y[0], y[1]);
-                } else {
+                    u[i / 2] = (u[i / 2] & m) | (ka & ~m);
+                    u[(P + i) / 2] = (u[(P + i) / 2] & m) | (kb & ~m);
+                } else if (i < left) {
                     u[i] = __float_as_uint(x[0]);
                     u[P + i] = __float_as_uint(y[0]);
                 }
@@ -138,7 +137,7 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope(const __grid_constant__ R
 #pragma unroll
         for (int q = 0; q < kBatch; ++q)
             if (h + q < h1) {
-                v[q].turn(c, s);
+                v[q].turn(c, s, r.turned - p0);
                 v[q].store(o + q * r.out_head, p0, r.half);
             }
         x += kBatch * r.x_head;
@@ -217,6 +216,7 @@ extern "C" tb_status tb_rope(tb_ctx* ctx, const tb_rope_params* p) {
             r.freq[q] = turn * std::exp2(-power * lg);
             r.axis[q] = (uint8_t)a;
         }
+    r.turned = q;
     for (; q < half; ++q) {
         r.freq[q] = 0.0;
         r.axis[q] = 0;
