@@ -123,13 +123,7 @@ tb_status tb_ctx_check_device(tb_ctx* ctx) {
     if (h != TB_DEVERR_NONE) {
         TB_CUDA_TRY(ctx, cudaMemsetAsync(ctx->d_err, 0, sizeof(int), ctx->stream));
         TB_CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream));
-        const char* what = h == TB_DEVERR_HASH_PROBE ? "hash probe bound exceeded"
-                         : h == TB_DEVERR_WAIT_TIMEOUT ? "bounded mbarrier wait timed out in the conv kernel"
-                         : h == TB_DEVERR_TMEM_ALLOC ? "TMEM allocation failed"
-                         : h == TB_DEVERR_SMEM_BASE ? "shared memory is not aligned for the attention kernel"
-                         : h == TB_DEVERR_BAD_OFFSETS ? "an offset table of packed sets descends or leaves the array"
-                         : "unknown device error";
-        return tb_fail(ctx, TB_ERR_DEVICE, what);
+        return tb_fail(ctx, TB_ERR_DEVICE, tb_device_error_text(h));
     }
     return TB_OK;
 }

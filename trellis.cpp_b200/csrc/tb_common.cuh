@@ -13,11 +13,23 @@
 enum tb_device_error : int {
     TB_DEVERR_NONE = 0,
     TB_DEVERR_HASH_PROBE = 1,     // hash insert/lookup exceeded its probe bound
-    TB_DEVERR_WAIT_TIMEOUT = 2,   // a bounded mbarrier wait in the conv kernel ran out
+    TB_DEVERR_WAIT_TIMEOUT = 2,   // a bounded mbarrier wait ran out (any tensor-core kernel)
     TB_DEVERR_TMEM_ALLOC = 3,     // TMEM allocation returned an unusable address
-    TB_DEVERR_SMEM_BASE = 5,      // dynamic shared memory starts too far from a multiple of 1024
     TB_DEVERR_BAD_OFFSETS = 4,    // an offset table of packed sets descends or leaves the array
+    TB_DEVERR_SMEM_BASE = 5,      // dynamic shared memory starts too far from a multiple of 1024
 };
+
+// What tb_ctx_check_device reports for the word.
+inline const char* tb_device_error_text(int e) {
+    switch (e) {
+        case TB_DEVERR_HASH_PROBE: return "hash probe bound exceeded";
+        case TB_DEVERR_WAIT_TIMEOUT: return "a kernel's bounded mbarrier wait timed out";
+        case TB_DEVERR_TMEM_ALLOC: return "TMEM allocation failed";
+        case TB_DEVERR_BAD_OFFSETS: return "an offset table of packed sets descends or leaves the array";
+        case TB_DEVERR_SMEM_BASE: return "shared memory is not aligned for the attention kernel";
+        default: return "unknown device error";
+    }
+}
 
 struct tb_ctx {
     int device = 0;
