@@ -248,7 +248,8 @@ tb_status tb_layer_norm(tb_ctx* ctx, const void* x, tb_dtype x_dtype, int64_t n,
  *   out[i][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q_i . k_j)
  * over the set's keys j; causal keeps j <= i + keys - queries (i, j from the sets' first rows), so
  * the last query sees every key, and one query row is a new token against all keys. lse (float32
- * [nq][heads], may be NULL) = log sum_j p_j. A row that sees no key gives 0, and -inf in lse.
+ * [nq][heads], may be NULL) = log sum_j p_j. A row that sees no key, or whose scores are all -inf,
+ * gives 0, and -inf in lse.
  *   - q [nq][heads][head_dim], k, v [nk][kv_heads][head_dim], out as q: rows and heads are the given
  *     numbers of elements apart, multiples of 16 bytes, values of a head contiguous. head_dim a
  *     multiple of 8 up to 128, at most 64 heads a key head, scale > 0.

@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kCcThreads, 2) k_attn_cc(const __grid_constant
         if (r >= rows) continue;
         const int64_t t = it.lo + t0 + r / g;
         const int h = kvh * g + r % g;
-        const bool none = min(lim[i], stop) <= first;       // a row without a key: out 0, lse -inf
+        const bool none = sum == 0.f;       // a row without a key, or without a score above -inf: out 0, lse -inf
         const float lg = none ? -INFINITY : m[i] + log2f(sum);
         const float inv = none ? 0.f : 1.f / sum;
         if (a.part) {

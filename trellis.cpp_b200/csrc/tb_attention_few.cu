@@ -235,8 +235,6 @@ k_attn_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUt
     const uint8_t* rings = smem_align1024(smem_raw);
     for (int w = threadIdx.x; w < rows * (D / 8); w += 32 * W) {
         const int r = w / (D / 8), d = w % (D / 8) * 8;
-        const int seen = a.causal ? max(0, min(nk, t0 + r / g + nk - nq + 1)) : nk;
-        const bool none = min(seen, stop) <= first;     // a row without a key here
         float mx = s_max[0][r];
 #pragma unroll
         for (int e = 1; e < W; ++e) mx = fmaxf(mx, s_max[e][r]);
@@ -250,6 +248,7 @@ k_attn_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUt
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = fmaf(f, from[j], v[j]);
         }
+        const bool none = sum == 0.f;                   // a row without a key here, or without a score above -inf
         const float inv = none ? 0.f : 1.f / sum, lg = none ? -INFINITY : mx - lift + log2f(sum);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = none ? 0.f : v[j] * inv;

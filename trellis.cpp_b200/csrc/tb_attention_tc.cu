@@ -625,7 +625,7 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
             }
             if (!ok) break;
             int t, h;
-            const bool valid = rows(t, h), none = n == 0 || lim <= 0;      // none: the row sees no key here
+            const bool valid = rows(t, h), none = total == 0.f;            // the row sees no key here, or none above -inf
             const float inv = none ? 0.f : 1.f / total;
             const int64_t row = (int64_t)job->q0 + t;
             const int64_t at = ((int64_t)job->split * a.nq + row) * a.heads + h;

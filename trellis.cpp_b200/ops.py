@@ -325,9 +325,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torc
     h // (H // Hk)); rows and heads may be strided (views of one q|k|v product). Set s has query rows
     q_offsets[s]:q_offsets[s+1] and key rows k_offsets[s]:k_offsets[s+1] (int32, device; k_offsets
     None: the same table; both None: one set). ``causal``: a query sees the keys up to its own
-    place, counted from the ends of both. ``scale``: 1/sqrt(D) when None. Rows without a key give
-    0; rows outside every set are not written (with ``out`` None: undefined). ``return_lse``: also
-    the float32 [Nq, H] log of each row's softmax sum."""
+    place, counted from the ends of both. ``scale``: 1/sqrt(D) when None. Rows without a key (or
+    with none whose score is above -inf) give 0; rows outside every set are not written (with
+    ``out`` None: undefined). ``return_lse``: also the float32 [Nq, H] log of each row's softmax
+    sum."""
     _need_heads(q, "q")
     _need_heads(k, "k")
     _need_heads(v, "v")
