@@ -1,6 +1,6 @@
 """Attention (tb_attention) at the ends of what scores and lengths may be: rows whose scores are all
--inf, in calls whose keys are cut into ranges and in others. The tolerance is that of
-packed_ref.attention_tolerance."""
+-inf, in calls whose keys are cut into ranges and in others; rows of hundreds of thousands to hundreds
+of millions of keys. The tolerance is that of packed_ref.attention_tolerance where nothing else is said."""
 import math
 
 import pytest
@@ -41,3 +41,99 @@ def test_scores_that_are_all_minus_infinity(tb, ql, kl, causal, dtype, d):
     none = wlse == -math.inf
     assert bool(none[:ql[0]].all())
     assert bool((lse == -math.inf)[none].all()) and bool((out[none] == 0).all()) and bool(torch.isfinite(lse[~none]).all())
+
+
+def _sampled(ops, q, k, v, qo, ko, rows, causal=False, **kw):
+    """The call against the 64-bit form at some rows: (set, row of the set)."""
+    out, lse = ops.attention(q, k, v, ref.table(qo), ref.table(ko), causal=causal, return_lse=True, **kw)
+    ops.check_device()
+    d, f = q.shape[2], ref.HALF[torch.float32]
+    for s, t in rows:
+        n, a, b = qo[s + 1] - qo[s], ko[s], ko[s + 1]
+        end = max(a, b - (n - 1 - t)) if causal else b
+        i = qo[s] + t
+        want, wlse, wgt, reach = ref.attention(q[i:i + 1], k[a:end], v[a:end], [0, 1], [0, end - a], False, d ** -0.5)
+        tol = ref.attention_tolerance(want, wgt, reach, d, end - a, q.dtype, out.dtype)
+        assert ref.close(out[i:i + 1], want, tol) <= 1.0, (s, t)
+        e = (d + 3) * f * reach + (64 + (end - a) / 64) * f + 2 ** -13 + 4 * f * (1 + wlse.abs())
+        assert bool(((lse[i:i + 1].double() - wlse).abs() <= e).all() or end == a), (s, t)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("order", ["flat", "rising", "falling"])
+@pytest.mark.parametrize("ql,kl,h,d", [
+    ([5120], [100003], 4, 64), ([5120], [100003], 4, 128), ([5120], [98304], 4, 72),     # one range of keys
+    ([100] + [3] * 160, [70001] + [40] * 160, 1, 128), ([20] * 170, [70001] + [300] * 169, 1, 40),
+    ([1280], [600000], 4, 64), ([300, 5], [700001, 9], 8, 128),                          # several, each a long one
+])
+def test_ranges_of_more_keys_than_one_accumulation_takes(tb, ql, kl, h, d, order, dtype):
+    from trellis_cpp_b200 import ops
+    qo, ko = ref.offsets(ql), ref.offsets(kl)
+    g = torch.Generator(device="cuda").manual_seed(d + ql[0])
+    q = torch.randn((qo[-1], h, d), device="cuda", generator=g).to(dtype)
+    k = torch.randn((ko[-1], h, d), device="cuda", generator=g)
+    v = torch.randn((ko[-1], h, d), device="cuda", generator=g).to(dtype)
+    if order != "flat":
+        q = q.abs()
+        ramp = torch.linspace(0.1, 3, ko[-1], device="cuda")[:, None, None]
+        k = k.abs() * (ramp if order == "rising" else ramp.flip(0))
+    k = k.to(dtype)
+    rows = [(0, 0), (0, ql[0] // 2), (0, ql[0] - 1)] + [(len(ql) - 1, t) for t in (0, ql[-1] - 1) if len(ql) > 1]
+    _sampled(ops, q, k, v, qo, ko, rows)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_causal_rows_around_an_accumulations_end(tb, d, dtype):
+    # tiles whose rows see 32768 keys, one more or one less: some rows have keys in the second segment
+    from trellis_cpp_b200 import ops
+    n = 33500
+    g = torch.Generator(device="cuda").manual_seed(d)
+    q, k, v = (torch.randn((n, 1, d), device="cuda", generator=g).to(dtype) for _ in range(3))
+    _sampled(ops, q, k, v, [0, n], [0, n], [(0, t) for t in (0, 127, 32640, 32767, 32768, 32769, 32895, 33023, 33499)], True)
+    k[32770] = math.nan                              # seen by the rows from 32770 on; the values there are numbers
+    out = ops.attention(q, k, v, causal=True)
+    assert bool(torch.isfinite(out[:32770]).all()) and bool(torch.isnan(out[32770:]).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_sums_over_millions_of_keys(tb, d, dtype):
+    """Equal weights (p = 1, exact) and values in [1, 2). An accumulation of 32768 keys is 2048 additions of
+    16 products to the sum so far, each of the 17 cut by less than a step (2 half steps) of a sum that ends
+    at its largest: at most 2048 * 34 half steps of it. The 128 segments add up in 128 more roundings."""
+    from trellis_cpp_b200 import ops
+    nk = 1 << 22
+    nq = torch.cuda.get_device_properties(0).multi_processor_count * 128 * (d // 64)      # one range of keys
+    g = torch.Generator(device="cuda").manual_seed(d)
+    q = torch.zeros((nq, 1, d), dtype=dtype, device="cuda")
+    k = torch.randn((nk, 1, d), device="cuda", generator=g).to(dtype)
+    v = (1 + torch.rand((nk, 1, d), device="cuda", generator=g)).to(dtype)
+    want = v.double().mean(0)
+    out, lse = ops.attention(q, k, v, out_dtype=torch.float32, return_lse=True)
+    ops.check_device()
+    f = ref.HALF[torch.float32]
+    assert float(((out[[0, 1, nq // 2, nq - 1]].double() - want).abs() / want).max()) <= (2048 * 34 + 2 * 128) * f
+    assert bool((out == out[:1]).all())
+    assert float((lse.double() - math.log(nk)).abs().max()) <= 2 ** -13 + (64 + 128) * f + 4 * f * math.log(nk)
+
+
+def test_a_tile_of_seconds(tb):
+    """450 million keys, 8 columns, on one tile an SM: each tile takes longer than the 4e9 cycles (2 s) that
+    a wait may last, and no wait is as long as a tile."""
+    from trellis_cpp_b200 import ops
+    nk, nq = 450_000_000, torch.cuda.get_device_properties(0).multi_processor_count * 128
+    q = torch.zeros((nq, 1, 8), dtype=torch.bfloat16, device="cuda")
+    k = torch.zeros((nk, 1, 8), dtype=torch.bfloat16, device="cuda")
+    v = torch.ones((nk, 1, 8), dtype=torch.bfloat16, device="cuda")
+    v[nk // 2:] = 2.0
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    out = ops.attention(q, k, v, out_dtype=torch.float32)
+    b.record()
+    ops.check_device()
+    f = ref.HALF[torch.float32]
+    # segments of one value are exact (32768 and 65536); their 13733 sums round once each
+    assert float((out - 1.5).abs().max()) <= 1.5 * 2 * 13734 * f
+    print("ms:", a.elapsed_time(b))

@@ -47,6 +47,11 @@ constexpr int kKeys = 128;             // keys of a block
 constexpr int kJobs = 2;               // tiles read ahead of the one in work, and it
 constexpr int kBufs = 3;               // S buffers
 constexpr float kRaise = 8.f;          // the reference follows when a block's maximum is 2^8 above it
+// Blocks of one accumulation in TMEM (32768 keys). The tensor core cuts what it adds to O below O's last
+// place instead of rounding it, so long sums come out short, by a share that grows with their length: at
+// 2^18, 2^20 and 2^22 keys of equal weight -0.14, -0.65 and -2.7% in f16 (-0.02, -0.45 and -2.5% in
+// bf16). A longer range is taken in segments, whose O the softmax threads add up in 32 bits.
+constexpr int kChain = 256;
 struct TcArgs {
     AttnArgs a;
     int tile_tokens;                   // tokens of a 128-row tile
@@ -134,13 +139,15 @@ template <int N> struct Ring {
     }
 };
 
-// A tile of the list: query rows of a set, a key head, a range of its key blocks. 12 words.
+// A job of the list: a tile (query rows of a set, a key head, a range of its key blocks) or a segment of
+// one. 12 words.
 struct Job {
     int q0, nq, k0, nk;    // the set's rows
     int first;             // the tile's first token, in the set
     int blk0, n;           // key blocks
     int kvh, split, end;   // end: the list is done
-    int pad[2];
+    int seg;               // of a tile in segments: bit 0 some came before, bit 1 some follow
+    int pad;
 };
 
 // 32 values of a row at p, as far as `left` says (a multiple of 8). Lanes are rows, so each store is a
@@ -280,6 +287,10 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
             if (ok) ok = __all_sync(0xffffffffu, wait_bar<PAIR>(bar, par, s_abort, a.err));
             return ok;
         };
+        auto wait_own = [&](uint32_t bar, uint32_t par) {        // a barrier that this CTA alone takes part in
+            ok = __all_sync(0xffffffffu, mbar_wait(bar, par, s_abort, a.err));
+            return ok;
+        };
         // The rows of V behind the set's last key belong to others and may hold no numbers, which a p
         // of 0 would not cancel: those of the last 16 that the products read become 0.
         auto clean = [&](uint32_t st, int keys) {
@@ -318,24 +329,28 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 const int end = a.causal ? max(0, min(o.nk, min(o.first + a.unit, o.nq) + o.nk - o.nq)) : o.nk;
                 const int all = (end + kKeys - 1) / kKeys;
                 o.blk0 = (int)((int64_t)all * split / a.nsplit);
-                o.n = (int)((int64_t)all * (split + 1) / a.nsplit) - o.blk0;
+                const int stop = over ? o.blk0 : (int)((int64_t)all * (split + 1) / a.nsplit);
                 o.kvh = kvh;
                 o.split = split;
                 o.end = over ? 1 : 0;
-                if (found || over) {
-                    if (jobs >= kJobs && !__all_sync(0xffffffffu, mbar_wait(jempty(jr.at), jr.round ^ 1, s_abort, a.err))) break;
+                o.seg = 0;
+                // The wait for a place takes a job's time at most: a segment's, not a tile's of any length.
+                for (bool go = found || over; go; o.blk0 += o.n, o.seg |= 1, go = o.blk0 < stop) {
+                    o.n = min(stop - o.blk0, kChain);
+                    o.seg = (o.seg & 1) | (o.blk0 + o.n < stop ? 2 : 0);
+                    if (jobs >= kJobs && !wait_own(jempty(jr.at), jr.round ^ 1)) break;
                     if (lane == 0) {
                         int4* dst = reinterpret_cast<int4*>(s_job + jr.at);
                         dst[0] = make_int4(o.q0, o.nq, o.k0, o.nk);
                         dst[1] = make_int4(o.first, o.blk0, o.n, o.kvh);
-                        dst[2] = make_int4(o.split, o.end, 0, 0);
+                        dst[2] = make_int4(o.split, o.end, o.seg, 0);
                         mbar_arrive(jfull(jr.at));
                     }
                     __syncwarp();
                     jr.step();
                     ++jobs;
-                    if (over) break;
                 }
+                if (over || !ok) break;
                 if (leader) {
                     if (elect_one()) {
                         mbar_arrive_expect_tx(taken, 16);
@@ -517,10 +532,17 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
         // p in f16 starts at 2^7 instead of 1 (2^15 after the largest rise): small p keep their digits
         constexpr float lift = std::is_same<T, __half>::value ? 7.f : 0.f;
         Ring<kBufs> u;
-        uint32_t tiles = 0, blocks = 0, turns = 0;   // tiles with keys, blocks of all tiles, hand-offs received
+        // A tile in segments: the thread's columns of O and the row's sum so far, against the reference in
+        // keep[W]. Indexed from a number that the compiler does not know, so that it lies in local memory and
+        // takes no registers from the softmax.
+        constexpr int W = D / 2;                     // each warpgroup writes half of the head's columns
+        float keep[W + 2];
+        int zero = 0;
+        asm volatile("" : "+r"(zero));
+        uint32_t tiles = 0, blocks = 0, turns = 0;   // jobs with keys, blocks of all jobs, hand-offs received
         bool ok = true;
         while (const Job* job = ok ? next_job() : nullptr) {
-            const int n = job->n;
+            const int n = job->n, seg = job->seg;
             // the keys from the tile's first block on that the row sees; rows past the set see all
             auto rows = [&](int& t, int& h) {
                 t = job->first + (int)rank * p.tile_tokens + rt;
@@ -624,20 +646,28 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 total = s_sum[r] + s_sum[128 + r];
             }
             if (!ok) break;
+            float mine = 1.f, before = 0.f;          // what O and the columns so far are scaled by
+            if (__builtin_expect(seg, 0)) {
+                const float had = seg & 1 ? keep[zero + W] : -INFINITY, top = fmaxf(had, ref);
+                mine = ref == -INFINITY ? 0.f : ex2(ref - top);
+                before = had == -INFINITY ? 0.f : ex2(had - top);
+                total = fmaf(total, mine, seg & 1 ? keep[zero + W + 1] * before : 0.f);
+                ref = top;
+                keep[zero + W] = ref;
+                keep[zero + W + 1] = total;
+            }
             int t, h;
             const bool valid = rows(t, h), none = total == 0.f;            // the row sees no key here, or none above -inf
             const float inv = none ? 0.f : 1.f / total;
             const int64_t row = (int64_t)job->q0 + t;
             const int64_t at = ((int64_t)job->split * a.nq + row) * a.heads + h;
-            if (valid && wg == 0 && (a.part || a.lse)) {
+            if (valid && wg == 0 && !(seg & 2) && (a.part || a.lse)) {
                 const float lg = none ? -INFINITY : ref - lift + log2f(total);
                 if (a.part) a.part_lse[at] = lg;
                 else a.lse[row * a.heads + h] = lg * 0.69314718055994530942f;
             }
             float* part = a.part + at * a.dim;
             O* out = reinterpret_cast<O*>(a.out) + row * a.out_row + (int64_t)h * a.out_head;
-            // each warpgroup writes half of the head's columns
-            constexpr int W = D / 2;
 #pragma unroll 1
             for (int w = 0; w < W; w += 32) {
                 const int q = wg * W + w;
@@ -655,7 +685,14 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                         }
                     }
                 }
-                if (!valid || (a.part && none)) continue;
+                if (__builtin_expect(seg, 0)) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        o[e] = fmaf(o[e], mine, seg & 1 ? keep[zero + w + e] * before : 0.f);
+                        keep[zero + w + e] = o[e];
+                    }
+                }
+                if (!valid || seg & 2 || (a.part && none)) continue;
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = none ? 0.f : o[e] * inv;
                 if (a.part) store_row<float>(part + q, o, a.dim - q, p.wide);
