@@ -137,3 +137,40 @@ def test_a_tile_of_seconds(tb):
     # segments of one value are exact (32768 and 65536); their 13733 sums round once each
     assert float((out - 1.5).abs().max()) <= 1.5 * 2 * 13734 * f
     print("ms:", a.elapsed_time(b))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("h,lg", [(150, 22), (1, 24)])
+def test_new_token_sums_over_millions_of_keys(tb, h, lg, dtype):
+    # as above; a warp's accumulation holds 32768 keys, and there are at most 32 in a row, 8 warps, 32 ranges
+    from trellis_cpp_b200 import ops
+    nk, d = (1 << lg) + 77, 8
+    g = torch.Generator(device="cuda").manual_seed(lg)
+    q = torch.zeros((1, h, d), dtype=dtype, device="cuda")
+    k = torch.zeros((nk, h, d), dtype=dtype, device="cuda")
+    v = (1 + torch.rand((nk, 1, d), device="cuda", generator=g)).to(dtype).expand(nk, h, d).contiguous()
+    want = v[:, 0].double().mean(0)
+    out, lse = ops.attention(q, k, v, out_dtype=torch.float32, return_lse=True)
+    ops.check_device()
+    f = ref.HALF[torch.float32]
+    assert float(((out[0].double() - want).abs() / want).max()) <= (2048 * 34 + 2 * 300) * f
+    assert float((lse.double() - math.log(nk)).abs().max()) <= 2 ** -13 + (64 + 512) * f + 4 * f * math.log(nk)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("order", ["flat", "rising", "falling"])
+@pytest.mark.parametrize("h,d,nk", [(150, 8, 300003), (160, 72, 140001)])
+def test_new_tokens_against_more_keys_than_one_accumulation_takes(tb, h, d, nk, order, dtype):
+    from trellis_cpp_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(d)
+    q = torch.randn((3, h, d), device="cuda", generator=g).to(dtype)
+    k = torch.randn((nk, h, d), device="cuda", generator=g, dtype=dtype)
+    v = torch.randn((nk, h, d), device="cuda", generator=g, dtype=dtype)
+    if order != "flat":
+        q, ramp = q.abs(), torch.linspace(0.1, 3, nk, device="cuda").to(dtype)[:, None, None]
+        k.abs_().mul_(ramp if order == "rising" else ramp.flip(0))
+    out = ops.attention(q, k, v, causal=True)
+    ops.check_device()
+    for a in (0, h - 1):
+        want, _, wgt, reach = ref.attention(q[:, a:a + 1], k[:, a:a + 1], v[:, a:a + 1], [0, 3], [0, nk], True, d ** -0.5)
+        assert ref.close(out[:, a:a + 1], want, ref.attention_tolerance(want, wgt, reach, d, nk, dtype, dtype)) <= 1.0

@@ -23,6 +23,10 @@ using namespace tbpk;
 
 constexpr int kFewRows = 16;
 constexpr int kStep = 16;              // keys of a warp's step
+// Steps of one accumulation of a warp's MMAs (32768 keys): they cut what they add below the sum's last
+// place instead of rounding it, and long sums come out short (a warp's 65536, 262144 and 1M keys of equal
+// weight in f16: -0.02, -0.14 and -0.65%). Further ones are added up in 32 bits.
+constexpr int kChain = 2048;
 
 template <int D> struct FewGeom {
     static constexpr int kBoxes = D / 64;
@@ -126,9 +130,37 @@ k_attn_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUt
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
 
+    // What came before this accumulation, against the maxima in keep[D / 2 + e]. Indexed from a number
+    // that the compiler does not know, so that it lies in local memory and takes no registers.
+    float keep[D / 2 + 2];
+    int zero = 0;
+    asm volatile("" : "+r"(zero));
+    auto add_kept = [&]() {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float had = keep[zero + D / 2 + e], f = had == -INFINITY ? 0.f : ex2(had - m[e]);
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+                for (int x = 2 * e; x < 2 * e + 2; ++x) o[n][x] = fmaf(keep[zero + 4 * n + x], f, o[n][x]);
+        }
+    };
+
     int st = 0, round = 0;
     bool ok = true;
     for (int i = 0; i < steps; ++i) {
+        if (__builtin_expect(i > 0 && i % kChain == 0, 0)) {
+            if (i > kChain) add_kept();
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    keep[zero + 4 * n + x] = o[n][x];
+                    o[n][x] = 0.f;
+                }
+            keep[zero + D / 2] = m[0];
+            keep[zero + D / 2 + 1] = m[1];
+        }
         ok = __all_sync(0xffffffffu, mbar_wait(bar0 + 8 * st, round, &s_abort, a.err));
         if (!ok) break;
         const uint32_t ks = ring0 + st * G::kBytes, vs = ks + G::kBoxes * G::kBox;
@@ -210,6 +242,7 @@ k_attn_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUt
             round ^= 1;
         }
     }
+    if (steps > kChain) add_kept();
     if (!ok) {                                          // loads may still be in flight
         const long long w0 = clock64();
         while (clock64() - w0 < 20000000) { }
