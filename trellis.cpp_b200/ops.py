@@ -68,7 +68,8 @@ def context(device=None):
         # by the Stream object: it brings CUDA up in a process that has made no tensor yet
         stream = torch.cuda.current_stream(idx).cuda_stream
         h = ctypes.c_void_p()
-        check(lib.tb_ctx_create(idx, ctypes.c_void_p(stream), ctypes.byref(h)), "tb_ctx_create")
+        with torch.cuda.device(idx):        # creation makes the device current; the caller's comes back
+            check(lib.tb_ctx_create(idx, ctypes.c_void_p(stream), ctypes.byref(h)), "tb_ctx_create")
         _ctxs[idx] = h
     else:
         # every time: a caller may have set another stream on the handle
