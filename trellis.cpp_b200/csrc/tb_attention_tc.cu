@@ -319,36 +319,39 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 idx /= a.nsplit;
                 const int kvh = idx % a.kv_heads;
                 SetWalk::Piece at{};                             // the launch has some more tiles than there are
-                const bool found = !over && walk.find(a.q_off, a.k_off, a.nset, a.nq, a.nk, a.unit, idx / a.kv_heads, lane, a.err, at);
-                Job o;
-                o.q0 = at.q0;
-                o.nq = at.nq;
-                o.k0 = at.k0;
-                o.nk = at.nk;
-                o.first = (int)(a.causal ? at.of - 1 - at.at : at.at) * a.unit;
-                const int end = a.causal ? max(0, min(o.nk, min(o.first + a.unit, o.nq) + o.nk - o.nq)) : o.nk;
-                const int all = (end + kKeys - 1) / kKeys;
-                o.blk0 = (int)((int64_t)all * split / a.nsplit);
-                const int stop = over ? o.blk0 : (int)((int64_t)all * (split + 1) / a.nsplit);
-                o.kvh = kvh;
-                o.split = split;
-                o.end = over ? 1 : 0;
-                o.seg = 0;
-                // The wait for a place takes a job's time at most: a segment's, not a tile's of any length.
-                for (bool go = found || over; go; o.blk0 += o.n, o.seg |= 1, go = o.blk0 < stop) {
-                    o.n = min(stop - o.blk0, kChain);
-                    o.seg = (o.seg & 1) | (o.blk0 + o.n < stop ? 2 : 0);
-                    if (jobs >= kJobs && !wait_own(jempty(jr.at), jr.round ^ 1)) break;
-                    if (lane == 0) {
-                        int4* dst = reinterpret_cast<int4*>(s_job + jr.at);
-                        dst[0] = make_int4(o.q0, o.nq, o.k0, o.nk);
-                        dst[1] = make_int4(o.first, o.blk0, o.n, o.kvh);
-                        dst[2] = make_int4(o.split, o.end, o.seg, 0);
-                        mbar_arrive(jfull(jr.at));
-                    }
-                    __syncwarp();
-                    jr.step();
-                    ++jobs;
+                if (over || walk.find(a.q_off, a.k_off, a.nset, a.nq, a.nk, a.unit, idx / a.kv_heads, lane, a.err, at)) {
+                    Job o;
+                    o.q0 = at.q0;
+                    o.nq = at.nq;
+                    o.k0 = at.k0;
+                    o.nk = at.nk;
+                    o.first = (int)(a.causal ? at.of - 1 - at.at : at.at) * a.unit;
+                    const int end = a.causal ? max(0, min(o.nk, min(o.first + a.unit, o.nq) + o.nk - o.nq)) : o.nk;
+                    const int all = (end + kKeys - 1) / kKeys;
+                    o.blk0 = (int)((int64_t)all * split / a.nsplit);
+                    const int stop = over ? o.blk0 : (int)((int64_t)all * (split + 1) / a.nsplit);
+                    o.kvh = kvh;
+                    o.split = split;
+                    o.end = over ? 1 : 0;
+                    o.seg = 0;
+                    // The wait for a place takes a job's time at most: a segment's, not a tile's of any length.
+                    do {
+                        o.n = min(stop - o.blk0, kChain);
+                        o.seg = (o.seg & 1) | (o.blk0 + o.n < stop ? 2 : 0);
+                        if (jobs >= kJobs && !wait_own(jempty(jr.at), jr.round ^ 1)) break;
+                        if (lane == 0) {
+                            int4* dst = reinterpret_cast<int4*>(s_job + jr.at);
+                            dst[0] = make_int4(o.q0, o.nq, o.k0, o.nk);
+                            dst[1] = make_int4(o.first, o.blk0, o.n, o.kvh);
+                            dst[2] = make_int4(o.split, o.end, o.seg, 0);
+                            mbar_arrive(jfull(jr.at));
+                        }
+                        __syncwarp();
+                        jr.step();
+                        ++jobs;
+                        o.blk0 += o.n;
+                        o.seg |= 1;
+                    } while (o.blk0 < stop);
                 }
                 if (over || !ok) break;
                 if (leader) {
@@ -646,22 +649,49 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 total = s_sum[r] + s_sum[128 + r];
             }
             if (!ok) break;
-            float mine = 1.f, before = 0.f;          // what O and the columns so far are scaled by
+            auto o_read = [&]() {                    // O may be written again
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (PAIR) mbar_arrive_cluster_relaxed(oempty, 0);
+                    else mbar_arrive(oempty);
+                }
+            };
             if (__builtin_expect(seg, 0)) {
+                // O and what the thread has of the segments before: to be kept, after the last one back into TMEM
                 const float had = seg & 1 ? keep[zero + W] : -INFINITY, top = fmaxf(had, ref);
-                mine = ref == -INFINITY ? 0.f : ex2(ref - top);
-                before = had == -INFINITY ? 0.f : ex2(had - top);
+                const float mine = ref == -INFINITY ? 0.f : ex2(ref - top), before = had == -INFINITY ? 0.f : ex2(had - top);
                 total = fmaf(total, mine, seg & 1 ? keep[zero + W + 1] * before : 0.f);
                 ref = top;
                 keep[zero + W] = ref;
                 keep[zero + W + 1] = total;
+#pragma unroll 1
+                for (int w = 0; w < W; w += 32) {
+                    float o[32];
+                    __syncwarp();
+                    tmem_ld_x32(to + wg * W + w, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        o[e] = fmaf(o[e], mine, seg & 1 ? keep[zero + w + e] * before : 0.f);
+                        keep[zero + w + e] = o[e];
+                    }
+                    if (!(seg & 2)) tmem_st_x32(to + wg * W + w, reinterpret_cast<const uint32_t*>(o));
+                }
+                tmem_wait_st();
+                if (seg & 2) {
+                    o_read();
+                    ++tiles;
+                    release_job();
+                    continue;
+                }
             }
             int t, h;
             const bool valid = rows(t, h), none = total == 0.f;            // the row sees no key here, or none above -inf
             const float inv = none ? 0.f : 1.f / total;
             const int64_t row = (int64_t)job->q0 + t;
             const int64_t at = ((int64_t)job->split * a.nq + row) * a.heads + h;
-            if (valid && wg == 0 && !(seg & 2) && (a.part || a.lse)) {
+            if (valid && wg == 0 && (a.part || a.lse)) {
                 const float lg = none ? -INFINITY : ref - lift + log2f(total);
                 if (a.part) a.part_lse[at] = lg;
                 else a.lse[row * a.heads + h] = lg * 0.69314718055994530942f;
@@ -676,23 +706,9 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                 if (n > 0) {
                     tmem_ld_x32(to + q, o);
                     tmem_wait_ld();
-                    if (w + 32 >= W) {               // O may be written again
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if (PAIR) mbar_arrive_cluster_relaxed(oempty, 0);
-                            else mbar_arrive(oempty);
-                        }
-                    }
+                    if (w + 32 >= W) o_read();
                 }
-                if (__builtin_expect(seg, 0)) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        o[e] = fmaf(o[e], mine, seg & 1 ? keep[zero + w + e] * before : 0.f);
-                        keep[zero + w + e] = o[e];
-                    }
-                }
-                if (!valid || seg & 2 || (a.part && none)) continue;
+                if (!valid || (a.part && none)) continue;
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = none ? 0.f : o[e] * inv;
                 if (a.part) store_row<float>(part + q, o, a.dim - q, p.wide);

@@ -29,7 +29,7 @@ struct SetWalk {
     int set0 = -32;
     uint32_t base = 0, total = 0;       // pieces of the sets before those in hand, of those
     uint32_t inc = 0, cnt = 0;          // pieces up to and with the lane's set, of it
-    int64_t qlo = 0, qhi = 0, klo = 0, khi = 0;
+    int qlo = 0, qn = 0, klo = 0, kn = 0;   // the lane's set: first rows and counts, below 2^31
 
     struct Piece {
         int q0, nq, k0, nk;             // the set's query rows and keys
@@ -47,9 +47,14 @@ struct SetWalk {
             set0 += 32;
             cnt = 0;
             if (set0 + lane < nset) {
-                set_range(q_off, set0 + lane, nq, qlo, qhi, err);
-                set_range(k_off, set0 + lane, nk, klo, khi, err);
-                cnt = (uint32_t)((qhi - qlo + unit - 1) / unit);
+                int64_t lo, hi;
+                set_range(q_off, set0 + lane, nq, lo, hi, err);
+                qlo = (int)lo;
+                qn = (int)(hi - lo);
+                set_range(k_off, set0 + lane, nk, lo, hi, err);
+                klo = (int)lo;
+                kn = (int)(hi - lo);
+                cnt = ((uint32_t)qn + (uint32_t)unit - 1) / (uint32_t)unit;
             }
             inc = cnt;
 #pragma unroll
@@ -59,15 +64,15 @@ struct SetWalk {
             }
             total = __shfl_sync(0xffffffffu, inc, 31);
         }
-        const bool found = number < base + total;
-        const int src = found ? __ffs(__ballot_sync(0xffffffffu, base + inc > number)) - 1 : 0;
+        if (number >= base + total) return false;
+        const int src = __ffs(__ballot_sync(0xffffffffu, base + inc > number)) - 1;
         p.of = __shfl_sync(0xffffffffu, cnt, src);
         p.at = number - base - (__shfl_sync(0xffffffffu, inc, src) - p.of);
-        p.q0 = (int)__shfl_sync(0xffffffffu, qlo, src);
-        p.nq = (int)__shfl_sync(0xffffffffu, qhi, src) - p.q0;
-        p.k0 = (int)__shfl_sync(0xffffffffu, klo, src);
-        p.nk = (int)__shfl_sync(0xffffffffu, khi, src) - p.k0;
-        return found;
+        p.q0 = __shfl_sync(0xffffffffu, qlo, src);
+        p.nq = __shfl_sync(0xffffffffu, qn, src);
+        p.k0 = __shfl_sync(0xffffffffu, klo, src);
+        p.nk = __shfl_sync(0xffffffffu, kn, src);
+        return true;
     }
 };
 
