@@ -1,6 +1,6 @@
 """Forms of attention (tb_attention) beside those of test_gpu_attention.py: sets that CTA pairs take with
 heads of 72 to 120 columns, whose second half of V is partly behind the head's end; caches that grow in
-place; hundreds of sets in 128-row tiles."""
+place; hundreds of sets in 128-row tiles; rows that see one key."""
 import math
 
 import pytest
@@ -89,3 +89,26 @@ def test_many_sets_of_many_rows(tb, n, top, h, hk, d, start, dtype):
         want, _, wgt, reach = ref.attention(q, k, v, qo, ko, causal, d ** -0.5)
         assert ref.close(out, want, ref.attention_tolerance(want, wgt, reach, d, max(kl), dtype, dtype)) <= 1.0
         assert bool((out[:start] == 4).all()) and bool((out[qo[-1]:] == 4).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,h,hk,d", [(40, 2, 2, 64), (300, 2, 2, 64), (300, 4, 2, 128), (40, 1, 1, 72), (1, 4, 2, 128), (3, 8, 2, 64)])
+def test_one_key_gives_its_value(tb, rows, h, hk, d, dtype):
+    """The softmax of one score is 1: the value itself, to the bit. p and its sum are off by 2^-20 at most
+    (scores below 2^4), far less than the half step within which the quotient rounds to the value. So for
+    sets of one key, and for the first row of a causal set."""
+    from trellis_cpp_b200 import ops
+    sets = 6
+    g = torch.Generator(device="cuda").manual_seed(rows + d)
+    q = torch.randn((sets * rows, h, d), device="cuda", generator=g).to(dtype)
+    k = torch.randn((sets, hk, d), device="cuda", generator=g).to(dtype)
+    v = torch.randn((sets, hk, d), device="cuda", generator=g).to(dtype)
+    qo = ref.table(list(range(0, sets * rows + 1, rows)))
+    out = ops.attention(q, k, v, qo, ref.table(list(range(sets + 1))))
+    want = v.repeat_interleave(h // hk, 1).repeat_interleave(rows, 0)
+    assert torch.equal(out, want)
+    k = torch.randn((sets * rows, hk, d), device="cuda", generator=g).to(dtype)
+    v = torch.randn((sets * rows, hk, d), device="cuda", generator=g).to(dtype)
+    out = ops.attention(q, k, v, qo, causal=True)
+    assert torch.equal(out[::rows], v[::rows].repeat_interleave(h // hk, 1))
+    ops.check_device()

@@ -14,8 +14,10 @@
 // of V for P V. Per CTA that halves the keys' way from L2 and the shared-memory reads, which a lone
 // CTA's products would saturate.
 //
-// The rows' reference (the running maximum, as a whole power of two) moves only when a block's maximum
-// exceeds it by more than 2^8: until then p grows to at most 2^8, which the 32-bit sums hold as well.
+// The rows' reference starts as the first block's maximum and moves only when a later block's exceeds it
+// by more than 2^8: until then p grows to at most 2^8, which the 32-bit sums hold as well. It is that
+// maximum itself, whose p is 1 and loses nothing where p is rounded to the operand type: a row that sees
+// one key gives its value (with the next whole power of two, p came out up to half a step off).
 // The warpgroups hand it on from block to block through shared memory; the one that raises it waits
 // until the block before has been added and scales O.
 //
@@ -601,7 +603,7 @@ __device__ __forceinline__ void attn_tc(const CUtensorMap& qmap, const CUtensorM
                                        max2(s[kKeys - 2], s[kKeys - 1])) * c;
                 const bool raise = !(top - now <= kRaise) && !(top == -INFINITY && now == -INFINITY);
                 if (b == 0 || __any_sync(0xffffffffu, raise || now != ref)) {
-                    const float next = raise ? rintf(top) : now;
+                    const float next = raise ? top : now;
                     refs[r] = next;
                     if (b > 0 && __any_sync(0xffffffffu, raise)) {
                         // O is at rest once the block before has been added
