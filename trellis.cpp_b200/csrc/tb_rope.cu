@@ -56,8 +56,8 @@ template <class T, int P, bool PAIRS> struct Pairs {
             for (int i = 0; i < kWords; ++i)
                 __stcs(reinterpret_cast<W*>(h + (PAIRS ? 2 * p0 : r * half + p0)) + i, w[r * kWords + i]);
     }
-    // turns the first `left` pairs by c, s
-    __device__ __forceinline__ void turn(const float* c, const float* s, int left) {
+    // turns the pairs by c, s; KEPT: the first `left` of them
+    template <bool KEPT> __device__ __forceinline__ void turn(const float* c, const float* s, int left) {
         uint32_t* u = reinterpret_cast<uint32_t*>(w);
         constexpr int per = 4 / (int)sizeof(T);                   // elements of a 32-bit word
 #pragma unroll
@@ -65,7 +65,7 @@ template <class T, int P, bool PAIRS> struct Pairs {
             if (PAIRS) {
                 float a, b;
                 get(u, 2 * i, &a, &b);
-                if (i < left) put(u, 2 * i, a * c[i] - b * s[i], a * s[i] + b * c[i]);
+                if (!KEPT || i < left) put(u, 2 * i, a * c[i] - b * s[i], a * s[i] + b * c[i]);
             } else {
                 float x[2], y[2];
 #pragma unroll
@@ -76,12 +76,12 @@ template <class T, int P, bool PAIRS> struct Pairs {
                 }
                 if (per == 2) {
                     const uint32_t ka = u[i / 2], kb = u[(P + i) / 2];
-                    const uint32_t m = i + 1 < left ? 0xffffffffu : i < left ? 0xffffu : 0u;   // the halves that turn
+                    const uint32_t m = !KEPT || i + 1 < left ? 0xffffffffu : i < left ? 0xffffu : 0u;   // the halves that turn
                     put(u, i, x[0], x[1]);
                     put(u, P + i, y[0], y[1]);
                     u[i / 2] = (u[i / 2] & m) | (ka & ~m);
                     u[(P + i) / 2] = (u[(P + i) / 2] & m) | (kb & ~m);
-                } else if (i < left) {
+                } else if (!KEPT || i < left) {
                     u[i] = __float_as_uint(x[0]);
                     u[P + i] = __float_as_uint(y[0]);
                 }
@@ -112,7 +112,9 @@ private:
     }
 };
 
-template <class T, int P, bool PAIRS>
+// KEPT: some pairs keep their bits. A kernel of its own, since the choice costs 2% where all turn (131072 x
+// 16 heads of 128, halves, f16: 180 us against 176).
+template <class T, int P, bool PAIRS, bool KEPT>
 __global__ void __launch_bounds__(kRopeThreads) k_rope(const __grid_constant__ RopeArgs r) {
     constexpr int kBatch = 4;                       // heads whose loads go before the first store
     const int64_t t = (int64_t)blockIdx.x * kRopeThreads + threadIdx.x;
@@ -137,7 +139,7 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope(const __grid_constant__ R
 #pragma unroll
         for (int q = 0; q < kBatch; ++q)
             if (h + q < h1) {
-                v[q].turn(c, s, r.turned - p0);
+                v[q].template turn<KEPT>(c, s, r.turned - p0);
                 v[q].store(o + q * r.out_head, p0, r.half);
             }
         x += kBatch * r.x_head;
@@ -148,11 +150,16 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope(const __grid_constant__ R
     }
 }
 
+template <class T, bool KEPT>
+void launch_rope(const RopeArgs& r, bool pairs, int per, dim3 grid, cudaStream_t stream) {
+    if (pairs) k_rope<T, 4, true, KEPT><<<grid, kRopeThreads, 0, stream>>>(r);
+    else if (per == 8) k_rope<T, 8, false, KEPT><<<grid, kRopeThreads, 0, stream>>>(r);
+    else k_rope<T, 4, false, KEPT><<<grid, kRopeThreads, 0, stream>>>(r);
+}
 template <class T>
 void launch_rope(const RopeArgs& r, bool pairs, int per, dim3 grid, cudaStream_t stream) {
-    if (pairs) k_rope<T, 4, true><<<grid, kRopeThreads, 0, stream>>>(r);
-    else if (per == 8) k_rope<T, 8, false><<<grid, kRopeThreads, 0, stream>>>(r);
-    else k_rope<T, 4, false><<<grid, kRopeThreads, 0, stream>>>(r);
+    if (r.turned < r.half) launch_rope<T, true>(r, pairs, per, grid, stream);
+    else launch_rope<T, false>(r, pairs, per, grid, stream);
 }
 
 }  // namespace
