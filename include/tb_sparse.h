@@ -255,10 +255,12 @@ tb_status tb_layer_norm(tb_ctx* ctx, const void* x, tb_dtype x_dtype, int64_t n,
  *     multiple of 8 up to 128, at most 64 heads a key head, scale > 0.
  *   - q_offsets and k_offsets are given together; their set s belong to each other.
  *   - dtype TB_BF16 / TB_F16: tensor cores (tcgen05; warp-level products for sets of a few rows),
- *     fp32 scores, softmax and accumulation; the p_j are rounded to the operand type before their product with v. TB_F32: CUDA cores.
+ *     fp32 scores, softmax and sums (over more than 32768 keys in pieces that are added up). The
+ *     p_j are rounded to the operand type before their product with v; the error against 64 bits is
+ *     up to 1.4 times that of rounding the result. TB_F32: CUDA cores, no such rounding.
  *   - out_dtype: TB_F32 or the operand dtype. out must not overlap q, k or v.
- *   - Values behind a set's last key have no effect, not a number included. A key that causal
- *     hides from some rows of its set must be finite: the rows' products multiply it by 0.
+ *   - Keys and values behind a set's last one have no effect, not a number included. A value that
+ *     causal hides from some rows of its set must be finite: the rows' products multiply it by 0.
  *
  * tb_rope: rotary positions along 1 to 4 axes. Pair p of each head of row i turns by
  * pos[i][axis(p)] * f_p: (a, b) -> (a cos - b sin, a sin + b cos). The first sections[0] pairs of a
@@ -270,13 +272,14 @@ tb_status tb_layer_norm(tb_ctx* ctx, const void* x, tb_dtype x_dtype, int64_t n,
  *     TB_ROPE_FREQS_JOINT f_p = theta^(-p/(head_dim/2)).
  *   - inverse != 0 turns by the negative angles (the transpose: carries gradients back).
  *   - x, out [n][heads][head_dim] of dtype, strides as in tb_attention; out may be x with the same
- *     strides, and overlaps it in no other way. The first heads of wider rows (q and k of one q|k|v product) are one call. head_dim a
- *     multiple of 8 up to 256. Angles are reduced in 64 bits.
+ *     strides, and overlaps it in no other way. The first heads of wider rows (q and k of one q|k|v
+ *     product) are one call. head_dim a multiple of 8 up to 256. Angles are reduced in 64 bits.
  *
  * tb_group_norm: out = act((x - mean) / sqrt(var + eps) * w + b), mean and variance of each set over
  * its rows and each group's c / groups consecutive channels. x [n][c] of x_dtype, out [n][c] of
- * out_dtype (TB_F32 or x_dtype; may be x, else apart from it); c a multiple of 8 up to 2048; w, b float32 [c], each may be
- * NULL. Statistics in fp32, of pieces joined in a fixed order: results repeat to the bit. */
+ * out_dtype (TB_F32 or x_dtype; may be x, else apart from it); c a multiple of 8 up to 2048; w, b
+ * float32 [c], each may be NULL. Statistics in fp32, of pieces joined in a fixed order: results
+ * repeat to the bit. */
 typedef enum tb_rope_layout { TB_ROPE_PAIRS = 0, TB_ROPE_HALVES = 1 } tb_rope_layout;
 typedef enum tb_rope_freqs { TB_ROPE_FREQS_AXIS = 0, TB_ROPE_FREQS_JOINT = 1 } tb_rope_freqs;
 

@@ -12,8 +12,10 @@
 // tile, so 16 bytes are two pairs of neighbours of the summed axis for packed FMAs, and the two halves
 // of a pair's sum meet at the end. Bound by what feeds the FMAs: a warp's step is 12 16-byte loads, 4
 // cycles of the SM's shared-memory path each, and 64 packed FMAs, 2 cycles of its scheduler each, so
-// the path is busy 192 cycles for 128 of the four schedulers' FMAs. 800 and 600 rows, 8 heads of 64:
-// 92 us, 22 TFLOP/s (4 x 4 values a thread, 256 threads, unpacked: 107 us).
+// the path is busy 192 cycles for 128 of the four schedulers' FMAs: 47 us of the 94 (22 TFLOP/s) that 800
+// and 600 rows, 8 heads of 64 take (4 x 4 values a thread, 256 threads, unpacked: 107 us). The rest: blocks
+// of keys are loaded between two barriers and used at once, 368 CTAs fill one wave of two an SM and part of
+// another, and the parts' join takes 10 us.
 #include "tb_packed.cuh"
 
 #include <algorithm>

@@ -225,6 +225,7 @@ k_attn_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUt
                     l[e] += p[n][2 * e + x];
                 }
         }
+        // rounded to the operands' type, which the MMA takes (what that costs: exp_block in tb_attention_tc.cu)
         const uint32_t pf[4] = {pack2(p[0][0], p[0][1], T()), pack2(p[0][2], p[0][3], T()), pack2(p[1][0], p[1][1], T()),
                                 pack2(p[1][2], p[1][3], T())};
 #pragma unroll

@@ -95,11 +95,14 @@ __device__ __forceinline__ float max2(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
-// p = 2^(s c + ref) of a row's 128 scores, rounded to T into the TMEM columns from `ts`; returns their
-// sum. The exponential unit (4 lanes a cycle and scheduler: 1024 cycles a block, as long as the block's
-// products) sets the pace and the sum's additions fill slots that it leaves. (A share of the
-// exponentials by a cubic on the FMA pipes, 1 or 2 of 8, cost as many cycles in issue as it saved
-// there: 1507 -> 1559 and 1659 us at 16384 x 12 x 128.)
+// p = 2^(s c + ref) of a row's 128 scores, rounded to T into the TMEM columns from `ts`; returns the sum of
+// the unrounded ones. T, since the tensor core takes P in V's type: a second product with what the rounding
+// leaves would double P V, and the rounded result is as far off by itself (bf16 1.7e-3 against 64 bits, with
+// this 2.1 to 2.3e-3); 32-bit operands have a kernel without it. The exponentials take 1024 cycles of their
+// unit a block, as long as the products of a wide block, but neither sets the pace (59 and 58% busy at 128
+// columns, 52 and 25% at 64): a turn of a softmax warpgroup does, some 3400 cycles with two under way.
+// (A share of the exponentials by a cubic on the FMA pipes, 1 or 2 of 8: 1507 -> 1559 and 1659 us at 16384 x
+// 12 x 128; not measured at 64 columns.)
 template <class T> __device__ __forceinline__ float exp_block(const float* s, float c, float ref, uint32_t ts) {
     const f2 c2 = pack(c, c), ref2 = pack(ref, ref);
     f2 sum[2];
@@ -760,7 +763,7 @@ struct Plan {
 };
 
 // Pairs for wide heads where an average set's rows fill more than one CTA (16384 rows, 12 heads of 128:
-// 1.55 ms, a CTA a tile 1.59; eight causal sets of 1 to 4096 rows, 16/4 heads: 183 us and 202; where rows
+// 1.53 ms, a CTA a tile 1.59; eight causal sets of 1 to 4096 rows, 16/4 heads: 183 us and 202; where rows
 // fill one CTA at most a pair's other half is idle: 62 us and 118 for 16 single rows). Keys are cut
 // where the CTAs would not fill the SMs, into ranges of four blocks at least in a set of the average
 // length, of eight if all keys are one set's (100 rows, 12 heads, 20000 keys: 32 us, whole 129; 300 rows, 8

@@ -14,7 +14,7 @@
 // costs no digits); entries are joined as
 //   mean = sum n_i mean_i / N,  M2 = sum M2_i + sum n_i (mean_i - mean)^2
 // always in the same order, so results repeat to the bit. Bound by memory: 262144 x 512 of bf16 in
-// 8 sets take 148 us, 58 of them for the statistics (4.6 TB/s).
+// 8 sets take 148 us; under the profiler 53 of 152 are the statistics (5.1 TB/s) and 7 their join.
 #include "tb_packed.cuh"
 
 #include <algorithm>
@@ -402,7 +402,9 @@ int gn_slab(int c, int cg, int size) {
 }
 
 // One launch where three would take longer than a second reading by few blocks (800 x 128: 7 us in one,
-// 12 in three; 8192 x 512: 24 and 17).
+// 12 in three; 8192 x 512: 24 and 17). Measured with 32 groups. The rule looks at rows alone, and a set of
+// few wide groups has few blocks: 4096 x 2048 of bf16 takes 39 us with 32 groups, 268 with 4 and 1060 with
+// one, where three launches take 18 (4097 rows).
 constexpr int kGnSmall = 4096;
 // Pieces an SM: one wave of k_gn_stats's blocks, whose join costs as much as some rows (16384 x 512:
 // 22 us with two, 32 with eight); one of k_gn_apply's, or two smaller ones where the array is larger
